@@ -325,7 +325,7 @@ def _own_linear_ce(s):
         o = {k: torch.empty(m, device=x.device) for k, m in (("loss", 1), ("row_loss", t), ("lse", t))}
         if c["train"]:
             o["dx"], o["dw"], o["dbias"] = _like(x, w, bias)
-        return {k: b for k, b in o.items() if b is not None}, torch.empty(n, dtype=torch.uint8, device=x.device)
+        return {k: b for k, b in o.items() if b is not None}, torch.zeros(n, dtype=torch.uint8, device=x.device)
 
     o, scratch = _buffers(s, make)
     st = _stream()
@@ -348,7 +348,7 @@ def _own_distill_topk(s):
         n = L.tl_distill_topk_scratch_bytes(t)
         o = {q: torch.empty(m, device=z.device) for q, m in (("loss", 1), ("row_loss", t), ("lse", t))}
         o["dz"] = torch.empty_like(z)
-        return o, torch.empty(n, dtype=torch.uint8, device=z.device)
+        return o, torch.zeros(n, dtype=torch.uint8, device=z.device)
 
     o, scratch = _buffers(s, make)
     # the loss and its gradient from one read of the logits
@@ -370,7 +370,7 @@ def _own_residual_norm(s):
         if c["train"]:
             o.update(zip(("dx", "du", "dgate", "dw_post", "dw_pre"), _like(x, u, gate, wa, wb)))
             n = L.tl_residual_norm_scratch_bytes(t, d)
-        return {k: b for k, b in o.items() if b is not None}, torch.empty(n, dtype=torch.uint8, device=x.device)
+        return {k: b for k, b in o.items() if b is not None}, torch.zeros(n, dtype=torch.uint8, device=x.device)
 
     o, scratch = _buffers(s, make)
     st = _stream()
