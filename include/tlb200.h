@@ -379,6 +379,101 @@ int  tl_head_ce(const float* A, int64_t lda, const float* W, int64_t ldw, const 
                 float* z, float* p, float* dp, float* dz, float* dx, int64_t lddx,
                 const float* mask, int64_t ldm, int64_t M, int64_t N, int64_t K, void* stream);
 
+/* ---- language-model head and block-boundary operators ---------------------
+ * No reference counterpart as single calls: each fuses a chain of the
+ * reference's ops over shapes it could not hold (a vocabulary of logits) or
+ * passes it would repeat.  Element types: TL_F32 (what a program's tensors
+ * are) or TL_BF16 (storage only: products of bf16 values are exact, sums,
+ * softmax statistics and norms are held in 32 bits, each output is rounded
+ * once).  Matrices are row-major with a leading dimension in elements, at
+ * least the row's length; rows may start at any element.
+ *
+ * Class indices are read as TL_IDX_F32 (float values, as cross_entropy's
+ * targets), TL_IDX_I32 or TL_IDX_I64; an index outside [0, classes) -- or a
+ * float that is no whole number -- names no class, and a row (or list entry)
+ * without a class takes no part: loss 0, gradient 0, not counted.
+ *
+ * `divisor` > 0 divides the summed loss and its gradients (the mean over a
+ * global batch, as tl_ce_softmax_backward takes it); 0 divides by the number
+ * of rows that count (at least 1).  `upstream` (one float on the device, or
+ * null for 1) multiplies the gradients, not the loss.
+ *
+ * `scratch`: at least the *_scratch_bytes() of the same sizes, 16-byte
+ * aligned, zero-filled when it is allocated and left ready for the next call;
+ * calls that may overlap on the GPU need scratch of their own, and scratch
+ * that one operator has used is zeroed before another kind of call takes it.  A dimension
+ * of 0 or a size past the stated limits returns TL_ERR_INVALID_ARG or
+ * TL_ERR_UNSUPPORTED before anything is launched, except that rows == 0 is an
+ * empty call: sums over rows (loss, weight gradients) come out as 0. */
+#define TL_F32 0
+#define TL_BF16 1
+#define TL_IDX_F32 0
+#define TL_IDX_I32 1
+#define TL_IDX_I64 2
+
+/* Norms around a block, its gate and the scaled residual:
+ *   y = alpha * x + gate * (norm(u) * w_post)      n = norm(y) * w_pre
+ * norm(v) = (v - mean(v)) / sqrt(var(v) + eps) (TL_NORM_LAYER, population
+ * statistics as layer_norm, kernel_generator.py:1667-1810) or
+ * v / sqrt(mean(v^2) + eps) (TL_NORM_RMS), along each row of `cols` elements.
+ * gate: TL_GATE_NONE (1), _CHANNEL [cols], _TOKEN [rows], _FULL [rows, cols]
+ * (leading dimension ldg).  u may be null (no block: y = alpha * x, and then
+ * w_post and gate are not read), w_post and w_pre may be null (1), y or n may
+ * be null (not wanted, not both).  n is computed from y before y is rounded.
+ * y may be x or u, n may be u or x, with the same leading dimension. */
+#define TL_NORM_LAYER 0
+#define TL_NORM_RMS 1
+#define TL_GATE_NONE 0
+#define TL_GATE_CHANNEL 1
+#define TL_GATE_TOKEN 2
+#define TL_GATE_FULL 3
+int  tl_residual_norm(int dtype, int kind, int64_t rows, int64_t cols, const void* x, int64_t ldx,
+                      const void* u, int64_t ldu, const void* w_post, const void* gate,
+                      int gate_mode, int64_t ldg, float alpha, const void* w_pre, float eps,
+                      void* y, int64_t ldy, void* n, int64_t ldn, void* stream);
+/* Its gradients, from x, u, the weights and the gradients dy of y and dn of n
+ * (either may be null: zero): dx, du, dgate (gate's shape), dw_post, dw_pre
+ * [cols]; each may be null (not wanted).  accumulate: a sum of TL_ACC_*, for
+ * outputs to be added to instead of overwritten.  dx may be dy and du may be
+ * dn, with the same leading dimension. */
+#define TL_ACC_DX 1
+#define TL_ACC_DU 2
+#define TL_ACC_DGATE 4
+#define TL_ACC_DW_POST 8
+#define TL_ACC_DW_PRE 16
+size_t tl_residual_norm_scratch_bytes(int64_t rows, int64_t cols);
+int  tl_residual_norm_backward(int dtype, int kind, int64_t rows, int64_t cols, const void* x,
+                               int64_t ldx, const void* u, int64_t ldu, const void* w_post,
+                               const void* gate, int gate_mode, int64_t ldg, float alpha,
+                               const void* w_pre, float eps, const void* dy, int64_t lddy,
+                               const void* dn, int64_t lddn, void* dx, int64_t lddx, void* du,
+                               int64_t lddu, void* dgate, int64_t lddg, void* dw_post,
+                               void* dw_pre, int accumulate, void* scratch, size_t scratch_bytes,
+                               void* stream);
+
+/* Distillation from a teacher's top logits: for every row, with the list
+ * (index[k], teacher[k]), k < top,
+ *   q = softmax(teacher / temperature) over the list's valid entries
+ *   p = softmax(z / temperature)       over the vocabulary of `classes`
+ *   row_loss = temperature^2 * sum_k q_k (log q_k - log p[index_k])
+ *   loss = sum(row_loss) / divisor
+ *   dz = temperature * (p - q) * upstream / divisor   (q of equal indices add)
+ * An entry whose teacher logit is -inf is not valid; a row without a valid
+ * entry does not count.  lse is log sum exp(z / temperature); a row whose
+ * logits are all -inf has lse = -inf, p = 0 and, where it counts, loss +inf.
+ * z [rows, classes] and teacher [rows, top] have the element type, index
+ * [rows, top] the index type; loss [1], row_loss and lse [rows] are float and
+ * may be null.  dz may be z (not with accumulate, which adds to dz).  With dz
+ * null this is the loss alone, with only dz the gradient alone; one read of z
+ * gives both.  top <= 1024; classes * element size <= 1536 KB. */
+size_t tl_distill_topk_scratch_bytes(int64_t rows);
+int  tl_distill_topk(int dtype, int64_t rows, int64_t classes, int64_t top, const void* z,
+                     int64_t ldz, const void* teacher, int64_t ldt, const void* index,
+                     int64_t ldi, int index_type, float temperature, float divisor,
+                     const float* upstream, float* loss, float* row_loss, float* lse, void* dz,
+                     int64_t lddz, int accumulate, void* scratch, size_t scratch_bytes,
+                     void* stream);
+
 /* Device-side error flag (TL_ERR_TIMEOUT after a bounded wait in a kernel
  * gave up; 0 if none).  reset != 0 clears it. */
 int  tl_device_error(int* code, int reset);

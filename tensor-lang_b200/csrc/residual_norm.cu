@@ -1,0 +1,662 @@
+// The norms around a block, its gate and the scaled residual, and their
+// gradients:
+//
+//   y = alpha x + gate * (norm(u) w_post)        n = norm(y) w_pre
+//
+// with norm the layer norm of kernel_generator.py:1667-1810 (population
+// statistics) or the root-mean-square norm.  Unfused this is six passes over
+// [rows, cols]; fused, the forward reads x and u and writes y and n, and the
+// backward reads x, u, dy, dn and writes dx, du (and a full gate's gradient).
+//
+// Gradients, with hat(v) = norm(v), r(v) its 1 / scale, c = cols:
+//   G    = dy + N(dn w_pre; y)             dx = alpha G
+//   P    = G gate                          du = N(P w_post; u)
+//   N(g; v) = r(v) (g - [mean g] - hat(v) mean(g hat(v)))   ([.]: layer norm only)
+//   dgate = G hat(u) w_post                dw_post = sum_rows P hat(u)
+//   dw_pre = sum_rows dn hat(y)
+// y is recomputed from x and u in the backward: it costs the same bytes as
+// reading a saved y, and is the unrounded value the forward's n came from.
+#include <math.h>
+
+#include <algorithm>
+
+#include "lm_common.cuh"
+
+namespace tl {
+namespace {
+
+struct NormArgs {
+  int64_t rows, cols;
+  const void* x;
+  int64_t ldx;
+  const void* u;  // null: no block
+  int64_t ldu;
+  const void* w_post;
+  const void* gate;
+  int gate_mode;
+  int64_t ldg;
+  float alpha;
+  const void* w_pre;
+  float eps;
+  // forward
+  void* y;
+  int64_t ldy;
+  void* n;
+  int64_t ldn;
+  // backward
+  const void* dy;
+  int64_t lddy;
+  const void* dn;
+  int64_t lddn;
+  void* dx;
+  int64_t lddx;
+  void* du;
+  int64_t lddu;
+  void* dgate;
+  int64_t lddg;
+  void* dw_post;
+  void* dw_pre;
+  int accumulate;
+  float* part;  // [grid][3][cols]: sums of dw_post, dw_pre, dgate (channel)
+};
+
+// Sums of a row's threads (NT threads; one warp, or the whole block).
+template <int NT, int K>
+__device__ __forceinline__ void row_sum(float (&v)[K], float* sh) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
+  if constexpr (NT > 32) {
+    constexpr int NW = NT / 32;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    __syncthreads();  // the previous sum's readers are done
+    if (lane == 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) sh[k * NW + w] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const float t = lane < NW ? sh[k * NW + lane] : 0.f;
+      v[k] = warp_sum(t);
+    }
+  }
+}
+
+// v becomes hat(v) for the elements a thread holds; returns 1 / scale.  Lanes
+// past the row hold zeros and must stay out of the centred sum (`in`).
+template <int NT, int E, bool LAYER, typename In>
+__device__ __forceinline__ float normalise(float (&v)[E], float cols, float inv_c, float eps, float* sh,
+                                           In in) {
+  float s[1];
+  if constexpr (LAYER) {
+    s[0] = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) s[0] += v[i];
+    row_sum<NT, 1>(s, sh);
+    const float mean = s[0] / cols;  // divided: the mean of a constant row is that constant
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = in(i) ? v[i] - mean : 0.f;
+  }
+  s[0] = 0.f;
+#pragma unroll
+  for (int i = 0; i < E; ++i) s[0] = fmaf(v[i], v[i], s[0]);
+  row_sum<NT, 1>(s, sh);
+  const float r = 1.f / sqrtf(s[0] * inv_c + eps);
+#pragma unroll
+  for (int i = 0; i < E; ++i) v[i] *= r;
+  return r;
+}
+
+// A thread's elements of a row: vector j of VEC elements at (j * NT + t) * VEC.
+template <typename T, int NT, int VEC, int NV>
+struct RowIo {
+  static constexpr int E = VEC * NV;
+  int64_t cols;
+  int t;
+  __device__ __forceinline__ int64_t at(int j) const { return ((int64_t)j * NT + t) * VEC; }
+  __device__ __forceinline__ bool in(int i) const { return at(i / VEC) < cols; }
+  __device__ __forceinline__ void load(const T* p, float (&v)[E]) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float q[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) q[i] = 0.f;
+      if (at(j) < cols) ld_vec<VEC>(p + at(j), q);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[j * VEC + i] = q[i];
+    }
+  }
+  __device__ __forceinline__ void store(T* p, const float (&v)[E], bool add) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (at(j) >= cols) continue;
+      float q[VEC];
+      if (add) {
+        ld_vec<VEC>(p + at(j), q);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) q[i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) q[i] += v[j * VEC + i];
+      st_vec<VEC>(p + at(j), q);
+    }
+  }
+  // v *= p (a weight or gate; null is 1)
+  __device__ __forceinline__ void scale(const T* p, float (&v)[E]) const {
+    if (!p) return;
+    float q[E];
+    load(p, q);
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] *= q[i];
+  }
+};
+
+// v *= gate, for row r
+template <typename T, typename Io, int E>
+__device__ __forceinline__ void apply_gate(const NormArgs& a, const Io& io, int64_t r,
+                                           float (&v)[E]) {
+  const T* g = static_cast<const T*>(a.gate);
+  if (a.gate_mode == TL_GATE_CHANNEL) {
+    io.scale(g, v);
+  } else if (a.gate_mode == TL_GATE_FULL) {
+    io.scale(g + r * a.ldg, v);
+  } else if (a.gate_mode == TL_GATE_TOKEN) {
+    const float q = to_f32(g[r]);
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] *= q;
+  }
+}
+
+constexpr int threads_of(int nt) { return nt == 32 ? 256 : nt; }
+
+template <typename T, int NT, int VEC, int NV, bool LAYER>
+__global__ void __launch_bounds__(threads_of(NT)) residual_norm_kernel(NormArgs a) {
+  using Io = RowIo<T, NT, VEC, NV>;
+  constexpr int E = Io::E;
+  __shared__ float sh[32];
+  const Io io{a.cols, (int)(threadIdx.x % NT)};
+  const int64_t r = (int64_t)blockIdx.x * (threads_of(NT) / NT) + threadIdx.x / NT;
+  if (r >= a.rows) return;  // NT > 32: the whole block; NT == 32: a warp, and no block barrier follows
+  const float inv_c = 1.f / (float)a.cols;
+  auto in = [&](int i) { return io.in(i); };
+  float y[E];
+  io.load(static_cast<const T*>(a.x) + r * a.ldx, y);
+  if (a.u) {
+    float v[E];
+    io.load(static_cast<const T*>(a.u) + r * a.ldu, v);
+    normalise<NT, E, LAYER>(v, (float)a.cols, inv_c, a.eps, sh, in);
+    io.scale(static_cast<const T*>(a.w_post), v);
+    apply_gate<T>(a, io, r, v);
+#pragma unroll
+    for (int i = 0; i < E; ++i) y[i] = fmaf(a.alpha, y[i], v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) y[i] *= a.alpha;
+  }
+  if (a.y) io.store(static_cast<T*>(a.y) + r * a.ldy, y, false);
+  if (a.n) {
+    normalise<NT, E, LAYER>(y, (float)a.cols, inv_c, a.eps, sh, in);
+    io.scale(static_cast<const T*>(a.w_pre), y);
+    io.store(static_cast<T*>(a.n) + r * a.ldn, y, false);
+  }
+}
+
+// Block b takes rows b, b + grid, ...: the column sums stay in its threads'
+// registers and leave as one row of partials, which norm_sums_kernel adds in
+// block order (no atomics: results do not depend on the order blocks end).
+template <typename T, int NT, int VEC, int NV, bool LAYER>
+__global__ void __launch_bounds__(NT) residual_norm_bwd_kernel(NormArgs a) {
+  using Io = RowIo<T, NT, VEC, NV>;
+  constexpr int E = Io::E;
+  __shared__ float sh[3 * 32];
+  const Io io{a.cols, (int)threadIdx.x};
+  const float inv_c = 1.f / (float)a.cols;
+  auto in = [&](int i) { return io.in(i); };
+  float s_post[E], s_pre[E], s_gate[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) s_post[i] = s_pre[i] = s_gate[i] = 0.f;
+  const T* w_post = static_cast<const T*>(a.w_post);
+  const T* w_pre = static_cast<const T*>(a.w_pre);
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    float y[E], hu[E], G[E];
+    io.load(static_cast<const T*>(a.x) + r * a.ldx, y);
+    float ru = 0.f;
+    if (a.u) {
+      io.load(static_cast<const T*>(a.u) + r * a.ldu, hu);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) hu[i] = 0.f;
+    }
+    if (a.dy) {
+      io.load(static_cast<const T*>(a.dy) + r * a.lddy, G);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) G[i] = 0.f;
+    }
+    if (a.u) ru = normalise<NT, E, LAYER>(hu, (float)a.cols, inv_c, a.eps, sh, in);
+    if (a.dn) {
+      float d[E];
+      io.load(static_cast<const T*>(a.dn) + r * a.lddn, d);
+      {
+        float v[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] = hu[i];
+        io.scale(w_post, v);
+        apply_gate<T>(a, io, r, v);
+#pragma unroll
+        for (int i = 0; i < E; ++i) y[i] = a.u ? fmaf(a.alpha, y[i], v[i]) : a.alpha * y[i];
+      }
+      const float ry = normalise<NT, E, LAYER>(y, (float)a.cols, inv_c, a.eps, sh, in);  // y: hat(y)
+#pragma unroll
+      for (int i = 0; i < E; ++i) s_pre[i] = fmaf(d[i], y[i], s_pre[i]);
+      io.scale(w_pre, d);
+      float c[2] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        c[0] = fmaf(d[i], y[i], c[0]);
+        c[1] += d[i];
+      }
+      row_sum<NT, 2>(c, sh);
+      const float m1 = c[0] * inv_c, m0 = LAYER ? c[1] * inv_c : 0.f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) G[i] = fmaf(ry, d[i] - m0 - y[i] * m1, G[i]);
+    }
+    if (a.dx) {
+      float v[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) v[i] = a.alpha * G[i];
+      io.store(static_cast<T*>(a.dx) + r * a.lddx, v, a.accumulate & TL_ACC_DX);
+    }
+    if (!a.u) continue;
+    if (a.dgate) {
+      float v[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) v[i] = G[i] * hu[i];
+      io.scale(w_post, v);
+      if (a.gate_mode == TL_GATE_CHANNEL) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) s_gate[i] += v[i];
+      } else if (a.gate_mode == TL_GATE_FULL) {
+        // the gate is read below: a full gate's gradient may not overwrite it
+        io.store(static_cast<T*>(a.dgate) + r * a.lddg, v, a.accumulate & TL_ACC_DGATE);
+      } else {
+        float s[1] = {0.f};
+#pragma unroll
+        for (int i = 0; i < E; ++i) s[0] += v[i];
+        row_sum<NT, 1>(s, sh);
+        if (threadIdx.x == 0) {
+          T* p = static_cast<T*>(a.dgate) + r;
+          from_f32(p, (a.accumulate & TL_ACC_DGATE) ? to_f32(*p) + s[0] : s[0]);
+        }
+      }
+    }
+    apply_gate<T>(a, io, r, G);  // P
+#pragma unroll
+    for (int i = 0; i < E; ++i) s_post[i] = fmaf(G[i], hu[i], s_post[i]);
+    if (a.du) {
+      io.scale(w_post, G);
+      float c[2] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        c[0] = fmaf(G[i], hu[i], c[0]);
+        c[1] += G[i];
+      }
+      row_sum<NT, 2>(c, sh);
+      const float m1 = c[0] * inv_c, m0 = LAYER ? c[1] * inv_c : 0.f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) G[i] = ru * (G[i] - m0 - hu[i] * m1);
+      io.store(static_cast<T*>(a.du) + r * a.lddu, G, a.accumulate & TL_ACC_DU);
+    }
+  }
+  float* part = a.part + (int64_t)blockIdx.x * 3 * a.cols;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int64_t c = io.at(i / VEC) + i % VEC;
+    if (c >= a.cols) continue;
+    if (a.dw_post) part[c] = s_post[i];
+    if (a.dw_pre) part[a.cols + c] = s_pre[i];
+    if (a.dgate && a.gate_mode == TL_GATE_CHANNEL) part[2 * a.cols + c] = s_gate[i];
+  }
+}
+
+// Adds the partials of `blocks` blocks: 32 columns of one of the three sums
+// per block; warp w adds partial rows w, w + 8, ... in turn, then the warps
+// in order.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_sums_kernel(NormArgs a, int64_t blocks) {
+  __shared__ float sh[8][33];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, which = blockIdx.y;
+  T* out = static_cast<T*>(which == 0 ? a.dw_post : which == 1 ? a.dw_pre : a.dgate);
+  if (!out || (which == 2 && a.gate_mode != TL_GATE_CHANNEL)) return;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  float s = 0.f;
+  if (c < a.cols)
+    for (int64_t b = w; b < blocks; b += 8) s += a.part[(b * 3 + which) * a.cols + c];
+  sh[w][lane] = s;
+  __syncthreads();
+  if (w == 0 && c < a.cols) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t += sh[k][lane];
+    const int flag = which == 0 ? TL_ACC_DW_POST : which == 1 ? TL_ACC_DW_PRE : TL_ACC_DGATE;
+    from_f32(out + c, (a.accumulate & flag) ? to_f32(out[c]) + t : t);
+  }
+}
+
+// Rows longer than the register kernels take: every pass reads the row again
+// (from L2), one block per row.
+constexpr int kLong = 1024;
+
+template <typename T, bool LAYER>
+struct LongRow {
+  const NormArgs& a;
+  int64_t r;
+  float* sh;
+  float inv_c;
+  __device__ float sum(float v) const {
+    float s[1] = {v};
+    row_sum<kLong, 1>(s, sh);
+    return s[0];
+  }
+  template <typename F>
+  __device__ float total(F f) const {
+    float s = 0.f;
+    for (int64_t c = threadIdx.x; c < a.cols; c += kLong) s += f(c);
+    return sum(s);
+  }
+  // mean and 1 / scale of the values f(c)
+  template <typename F>
+  __device__ float2 stats(F f) const {
+    const float mean = LAYER ? total(f) / (float)a.cols : 0.f;
+    const float q = total([&](int64_t c) { const float d = f(c) - mean; return d * d; });
+    return make_float2(mean, 1.f / sqrtf(q * inv_c + a.eps));
+  }
+  __device__ float at(const void* p, int64_t i) const { return to_f32(static_cast<const T*>(p)[i]); }
+  __device__ float w_post(int64_t c) const { return a.w_post ? at(a.w_post, c) : 1.f; }
+  __device__ float w_pre(int64_t c) const { return a.w_pre ? at(a.w_pre, c) : 1.f; }
+  __device__ float gate(int64_t c) const {
+    return a.gate_mode == TL_GATE_CHANNEL ? at(a.gate, c)
+           : a.gate_mode == TL_GATE_TOKEN ? at(a.gate, r)
+           : a.gate_mode == TL_GATE_FULL  ? at(a.gate, r * a.ldg + c)
+                                          : 1.f;
+  }
+  __device__ float u(int64_t c) const { return at(a.u, r * a.ldu + c); }
+  __device__ float y(int64_t c, float2 su) const {
+    const float v = a.alpha * at(a.x, r * a.ldx + c);
+    return a.u ? v + (u(c) - su.x) * su.y * w_post(c) * gate(c) : v;
+  }
+};
+
+template <typename T, bool LAYER>
+__global__ void __launch_bounds__(kLong) residual_norm_long_kernel(NormArgs a) {
+  __shared__ float sh[32];
+  const float inv_c = 1.f / (float)a.cols;
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const LongRow<T, LAYER> R{a, r, sh, inv_c};
+    const float2 su = a.u ? R.stats([&](int64_t c) { return R.u(c); }) : make_float2(0.f, 0.f);
+    float2 sy = make_float2(0.f, 0.f);
+    if (a.n) sy = R.stats([&](int64_t c) { return R.y(c, su); });
+    for (int64_t c = threadIdx.x; c < a.cols; c += kLong) {
+      const float y = R.y(c, su);
+      if (a.y) from_f32(static_cast<T*>(a.y) + r * a.ldy + c, y);
+      if (a.n) from_f32(static_cast<T*>(a.n) + r * a.ldn + c, (y - sy.x) * sy.y * R.w_pre(c));
+    }
+  }
+}
+
+template <typename T, bool LAYER>
+__global__ void __launch_bounds__(kLong) residual_norm_bwd_long_kernel(NormArgs a) {
+  __shared__ float sh[32];
+  const float inv_c = 1.f / (float)a.cols;
+  float* part = a.part + (int64_t)blockIdx.x * 3 * a.cols;
+  for (int64_t c = threadIdx.x; c < 3 * a.cols; c += kLong) part[c] = 0.f;
+  __syncthreads();  // column c's partials belong to thread c % kLong below
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const LongRow<T, LAYER> R{a, r, sh, inv_c};
+    const float2 su = a.u ? R.stats([&](int64_t c) { return R.u(c); }) : make_float2(0.f, 0.f);
+    float2 sy = make_float2(0.f, 0.f);
+    float m1 = 0.f, m0 = 0.f;
+    auto hat_y = [&](int64_t c) { return (R.y(c, su) - sy.x) * sy.y; };
+    auto gn = [&](int64_t c) { return R.at(a.dn, r * a.lddn + c) * R.w_pre(c); };
+    if (a.dn) {
+      sy = R.stats([&](int64_t c) { return R.y(c, su); });
+      m1 = R.total([&](int64_t c) { return gn(c) * hat_y(c); }) * inv_c;
+      if (LAYER) m0 = R.total(gn) * inv_c;
+    }
+    auto G = [&](int64_t c) {
+      float g = a.dy ? R.at(a.dy, r * a.lddy + c) : 0.f;
+      if (a.dn) g += sy.y * (gn(c) - m0 - hat_y(c) * m1);
+      return g;
+    };
+    auto hat_u = [&](int64_t c) { return (R.u(c) - su.x) * su.y; };
+    float e1 = 0.f, e0 = 0.f;
+    if (a.u) {
+      if (a.du) {
+        e1 = R.total([&](int64_t c) { return G(c) * R.gate(c) * R.w_post(c) * hat_u(c); }) * inv_c;
+        if (LAYER) e0 = R.total([&](int64_t c) { return G(c) * R.gate(c) * R.w_post(c); }) * inv_c;
+      }
+      if (a.dgate && a.gate_mode == TL_GATE_TOKEN) {
+        const float s = R.total([&](int64_t c) { return G(c) * hat_u(c) * R.w_post(c); });
+        if (threadIdx.x == 0) {
+          T* p = static_cast<T*>(a.dgate) + r;
+          from_f32(p, (a.accumulate & TL_ACC_DGATE) ? to_f32(*p) + s : s);
+        }
+      }
+    }
+    // every element's inputs are read before its outputs are written (dx may
+    // be dy, du may be dn), and no pass over the row follows
+    for (int64_t c = threadIdx.x; c < a.cols; c += kLong) {
+      const float g = G(c);
+      if (a.dn) part[a.cols + c] += R.at(a.dn, r * a.lddn + c) * hat_y(c);
+      float du = 0.f, dg = 0.f;
+      if (a.u) {
+        const float p = g * R.gate(c), h = hat_u(c);
+        part[c] += p * h;
+        dg = g * h * R.w_post(c);
+        if (a.gate_mode == TL_GATE_CHANNEL) part[2 * a.cols + c] += dg;
+        du = su.y * (p * R.w_post(c) - e0 - h * e1);
+      }
+      if (a.dx) {
+        T* p = static_cast<T*>(a.dx) + r * a.lddx + c;
+        from_f32(p, ((a.accumulate & TL_ACC_DX) ? to_f32(*p) : 0.f) + a.alpha * g);
+      }
+      if (a.u && a.du) {
+        T* p = static_cast<T*>(a.du) + r * a.lddu + c;
+        from_f32(p, ((a.accumulate & TL_ACC_DU) ? to_f32(*p) : 0.f) + du);
+      }
+      if (a.u && a.dgate && a.gate_mode == TL_GATE_FULL) {
+        T* p = static_cast<T*>(a.dgate) + r * a.lddg + c;
+        from_f32(p, ((a.accumulate & TL_ACC_DGATE) ? to_f32(*p) : 0.f) + dg);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------- host side ---
+// Blocks of the backward (and rows of its partials): two per SM.
+int64_t bwd_blocks(int64_t rows) { return std::max<int64_t>(1, std::min<int64_t>(rows, 2LL * sm_count())); }
+
+// The register kernels hold a row in NT threads x VEC * NV elements.
+constexpr int64_t kMaxCols = 8192;
+
+template <typename T, int VEC, int NT, int NV>
+int launch_fwd(const NormArgs& a, int kind, cudaStream_t st) {
+  constexpr int per = threads_of(NT) / NT;
+  const unsigned grid = (unsigned)((a.rows + per - 1) / per);
+  if (kind == TL_NORM_LAYER)
+    residual_norm_kernel<T, NT, VEC, NV, true><<<grid, threads_of(NT), 0, st>>>(a);
+  else
+    residual_norm_kernel<T, NT, VEC, NV, false><<<grid, threads_of(NT), 0, st>>>(a);
+  return after_launch();
+}
+
+template <typename T, int VEC>
+int forward(const NormArgs& a, int kind, cudaStream_t st) {
+  constexpr int E = VEC == 1 ? 4 : VEC;  // elements of a thread with the fewest
+  constexpr int N1 = E / VEC;
+  const int64_t c = a.cols;
+  if (c <= 32 * E) return launch_fwd<T, VEC, 32, N1>(a, kind, st);
+  if (c <= 64 * E) return launch_fwd<T, VEC, 64, N1>(a, kind, st);
+  if (c <= 128 * E) return launch_fwd<T, VEC, 128, N1>(a, kind, st);
+  if (c <= 256 * E) return launch_fwd<T, VEC, 256, N1>(a, kind, st);
+  if (c <= 512 * E) return launch_fwd<T, VEC, 512, N1>(a, kind, st);
+  return launch_fwd<T, VEC, 512, kMaxCols / 512 / VEC>(a, kind, st);
+}
+
+template <typename T, int VEC, int NT, int NV>
+int launch_bwd(const NormArgs& a, int kind, cudaStream_t st) {
+  const unsigned grid = (unsigned)bwd_blocks(a.rows);
+  if (kind == TL_NORM_LAYER)
+    residual_norm_bwd_kernel<T, NT, VEC, NV, true><<<grid, NT, 0, st>>>(a);
+  else
+    residual_norm_bwd_kernel<T, NT, VEC, NV, false><<<grid, NT, 0, st>>>(a);
+  return after_launch();
+}
+
+template <typename T, int VEC>
+int backward(const NormArgs& a, int kind, cudaStream_t st) {
+  constexpr int E = VEC == 1 ? 4 : VEC;
+  constexpr int N1 = E / VEC;
+  const int64_t c = a.cols;
+  if (c <= 64 * E) return launch_bwd<T, VEC, 64, N1>(a, kind, st);
+  if (c <= 128 * E) return launch_bwd<T, VEC, 128, N1>(a, kind, st);
+  if (c <= 256 * E) return launch_bwd<T, VEC, 256, N1>(a, kind, st);
+  if (c <= 512 * E) return launch_bwd<T, VEC, 512, N1>(a, kind, st);
+  return launch_bwd<T, VEC, 512, kMaxCols / 512 / VEC>(a, kind, st);
+}
+
+// Whether rows of p (leading dimension ld) take 128-bit accesses.
+bool vec_rows(const void* p, int64_t ld, int64_t vec) {
+  return !p || (aligned_to(p, 16) && ld % vec == 0);
+}
+
+bool vec_ok(const NormArgs& a, int64_t vec) {
+  if (a.cols % vec) return false;
+  const bool gate_rows = a.gate_mode == TL_GATE_FULL, gate_vec = a.gate_mode == TL_GATE_CHANNEL;
+  if (gate_rows && !(vec_rows(a.gate, a.ldg, vec) && vec_rows(a.dgate, a.lddg, vec))) return false;
+  if (gate_vec && !(vec_rows(a.gate, 0, vec))) return false;
+  return vec_rows(a.x, a.ldx, vec) && vec_rows(a.u, a.ldu, vec) && vec_rows(a.w_post, 0, vec) &&
+         vec_rows(a.w_pre, 0, vec) && vec_rows(a.y, a.ldy, vec) && vec_rows(a.n, a.ldn, vec) &&
+         vec_rows(a.dy, a.lddy, vec) && vec_rows(a.dn, a.lddn, vec) &&
+         vec_rows(a.dx, a.lddx, vec) && vec_rows(a.du, a.lddu, vec);
+}
+
+template <typename T>
+int run_forward(const NormArgs& a, int kind, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  if (a.cols > kMaxCols) {
+    const unsigned grid = (unsigned)std::min<int64_t>(a.rows, 2LL * sm_count());
+    if (kind == TL_NORM_LAYER)
+      residual_norm_long_kernel<T, true><<<grid, kLong, 0, st>>>(a);
+    else
+      residual_norm_long_kernel<T, false><<<grid, kLong, 0, st>>>(a);
+    return after_launch();
+  }
+  return vec_ok(a, V) ? forward<T, V>(a, kind, st) : forward<T, 1>(a, kind, st);
+}
+
+template <typename T>
+int run_backward(const NormArgs& a, int kind, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  if (a.rows > 0) {
+    if (a.cols > kMaxCols) {
+      const unsigned grid = (unsigned)bwd_blocks(a.rows);
+      if (kind == TL_NORM_LAYER)
+        residual_norm_bwd_long_kernel<T, true><<<grid, kLong, 0, st>>>(a);
+      else
+        residual_norm_bwd_long_kernel<T, false><<<grid, kLong, 0, st>>>(a);
+      TL_TRY(after_launch());
+    } else {
+      TL_TRY((vec_ok(a, V) ? backward<T, V>(a, kind, st) : backward<T, 1>(a, kind, st)));
+    }
+  }
+  if (a.dw_post || a.dw_pre || (a.dgate && a.gate_mode == TL_GATE_CHANNEL)) {
+    norm_sums_kernel<T><<<dim3((unsigned)((a.cols + 31) / 32), 3), 256, 0, st>>>(
+        a, a.rows > 0 ? bwd_blocks(a.rows) : 0);
+    TL_TRY(after_launch());
+  }
+  return TL_OK;
+}
+
+// Arguments common to both directions.
+int check(int dtype, int kind, const NormArgs& a) {
+  if (!dtype_ok(dtype) || (kind != TL_NORM_LAYER && kind != TL_NORM_RMS)) return TL_ERR_INVALID_ARG;
+  if (a.rows < 0 || a.cols <= 0 || a.rows > INT32_MAX || a.cols > INT32_MAX)
+    return TL_ERR_INVALID_ARG;
+  if (a.rows > 0 && !a.x) return TL_ERR_INVALID_ARG;
+  if (a.gate_mode < TL_GATE_NONE || a.gate_mode > TL_GATE_FULL) return TL_ERR_INVALID_ARG;
+  if (a.rows > 0 && a.u && a.gate_mode != TL_GATE_NONE && !a.gate) return TL_ERR_INVALID_ARG;
+  if (!(a.eps >= 0.f) || a.alpha != a.alpha) return TL_ERR_INVALID_ARG;
+  if (a.ldx < a.cols || (a.u && a.ldu < a.cols)) return TL_ERR_INVALID_ARG;
+  if (a.u && a.gate_mode == TL_GATE_FULL && a.ldg < a.cols) return TL_ERR_INVALID_ARG;
+  return TL_OK;
+}
+
+}  // namespace
+}  // namespace tl
+
+extern "C" {
+
+int tl_residual_norm(int dtype, int kind, int64_t rows, int64_t cols, const void* x, int64_t ldx,
+                     const void* u, int64_t ldu, const void* w_post, const void* gate,
+                     int gate_mode, int64_t ldg, float alpha, const void* w_pre, float eps, void* y,
+                     int64_t ldy, void* n, int64_t ldn, void* stream) {
+  tl::NormArgs a{};
+  a.rows = rows; a.cols = cols; a.x = x; a.ldx = ldx; a.u = u; a.ldu = ldu;
+  a.w_post = u ? w_post : nullptr;
+  a.gate_mode = u ? gate_mode : TL_GATE_NONE;
+  a.gate = a.gate_mode == TL_GATE_NONE ? nullptr : gate;
+  a.ldg = ldg; a.alpha = alpha; a.w_pre = w_pre; a.eps = eps;
+  a.y = y; a.ldy = ldy; a.n = n; a.ldn = ldn;
+  if (gate_mode < TL_GATE_NONE || gate_mode > TL_GATE_FULL) return TL_ERR_INVALID_ARG;
+  TL_TRY(tl::check(dtype, kind, a));
+  if ((rows > 0 && !y && !n) || (y && ldy < cols) || (n && ldn < cols)) return TL_ERR_INVALID_ARG;
+  if (y && y == n) return TL_ERR_INVALID_ARG;
+  if (rows == 0) return TL_OK;
+  cudaStream_t st = tl::stream_or_default(stream);
+  return dtype == TL_BF16 ? tl::run_forward<__nv_bfloat16>(a, kind, st)
+                          : tl::run_forward<float>(a, kind, st);
+}
+
+size_t tl_residual_norm_scratch_bytes(int64_t rows, int64_t cols) {
+  if (rows < 0 || cols <= 0) return 0;
+  return (size_t)tl::bwd_blocks(rows) * 3 * (size_t)cols * sizeof(float);
+}
+
+int tl_residual_norm_backward(int dtype, int kind, int64_t rows, int64_t cols, const void* x,
+                              int64_t ldx, const void* u, int64_t ldu, const void* w_post,
+                              const void* gate, int gate_mode, int64_t ldg, float alpha,
+                              const void* w_pre, float eps, const void* dy, int64_t lddy,
+                              const void* dn, int64_t lddn, void* dx, int64_t lddx, void* du,
+                              int64_t lddu, void* dgate, int64_t lddg, void* dw_post, void* dw_pre,
+                              int accumulate, void* scratch, size_t scratch_bytes, void* stream) {
+  tl::NormArgs a{};
+  a.rows = rows; a.cols = cols; a.x = x; a.ldx = ldx; a.u = u; a.ldu = ldu;
+  a.w_post = u ? w_post : nullptr;
+  a.gate_mode = u ? gate_mode : TL_GATE_NONE;
+  a.gate = a.gate_mode == TL_GATE_NONE ? nullptr : gate;
+  a.ldg = ldg; a.alpha = alpha; a.w_pre = w_pre; a.eps = eps;
+  a.dy = dy; a.lddy = lddy; a.dn = dn; a.lddn = lddn;
+  a.dx = dx; a.lddx = lddx; a.du = du; a.lddu = lddu; a.dgate = dgate; a.lddg = lddg;
+  a.dw_post = dw_post; a.dw_pre = dw_pre; a.accumulate = accumulate;
+  a.part = static_cast<float*>(scratch);
+  if (gate_mode < TL_GATE_NONE || gate_mode > TL_GATE_FULL) return TL_ERR_INVALID_ARG;
+  TL_TRY(tl::check(dtype, kind, a));
+  if ((dy && lddy < cols) || (dn && lddn < cols) || (dx && lddx < cols) || (du && lddu < cols))
+    return TL_ERR_INVALID_ARG;
+  // gradients of what the call does not have
+  if (!u && (du || dw_post || dgate)) return TL_ERR_INVALID_ARG;
+  if (dgate && (gate_mode == TL_GATE_NONE || dgate == gate)) return TL_ERR_INVALID_ARG;
+  if (dgate && gate_mode == TL_GATE_FULL && lddg < cols) return TL_ERR_INVALID_ARG;
+  if (accumulate < 0 || accumulate > 31) return TL_ERR_INVALID_ARG;
+  if (!dx && !du && !dgate && !dw_post && !dw_pre) return TL_ERR_INVALID_ARG;
+  if (!scratch || !tl::aligned_to(scratch, 16) ||
+      scratch_bytes < tl_residual_norm_scratch_bytes(rows, cols))
+    return TL_ERR_INVALID_ARG;
+  cudaStream_t st = tl::stream_or_default(stream);
+  return dtype == TL_BF16 ? tl::run_backward<__nv_bfloat16>(a, kind, st)
+                          : tl::run_backward<float>(a, kind, st);
+}
+
+}  // extern "C"

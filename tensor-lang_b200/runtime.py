@@ -34,6 +34,11 @@ TL_ERR_UNSUPPORTED = 1008
 
 RED_SUM, RED_MEAN, RED_MAX, RED_MIN, RED_ARGMAX, RED_ARGMIN = range(6)
 EPI_NONE, EPI_RELU = 0, 1
+F32, BF16 = 0, 1                       # element types of the language-model operators
+IDX_F32, IDX_I32, IDX_I64 = 0, 1, 2    # class-index types
+NORM_LAYER, NORM_RMS = 0, 1
+GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_FULL = 0, 1, 2, 3
+ACC_DX, ACC_DU, ACC_DGATE, ACC_DW_POST, ACC_DW_PRE = 1, 2, 4, 8, 16
 
 
 class TLCudaError(RuntimeError):
@@ -133,6 +138,21 @@ _SIGS = [
     ("tl_head_ce", c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int,
                            c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                            c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p]),
+    ("tl_residual_norm", c_int, [c_int, c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+                                 c_int64, c_void_p, c_void_p, c_int, c_int64, c_float, c_void_p,
+                                 c_float, c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
+    ("tl_residual_norm_scratch_bytes", c_size_t, [c_int64, c_int64]),
+    ("tl_residual_norm_backward", c_int, [c_int, c_int, c_int64, c_int64, c_void_p, c_int64,
+                                          c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int64,
+                                          c_float, c_void_p, c_float, c_void_p, c_int64, c_void_p,
+                                          c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                          c_int64, c_void_p, c_void_p, c_int, c_void_p, c_size_t,
+                                          c_void_p]),
+    ("tl_distill_topk_scratch_bytes", c_size_t, [c_int64]),
+    ("tl_distill_topk", c_int, [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+                                c_int64, c_void_p, c_int64, c_int, c_float, c_float, c_void_p,
+                                c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p,
+                                c_size_t, c_void_p]),
     ("tl_device_error", c_int, [ctypes.POINTER(c_int), c_int]),
     ("tl_nccl_unique_id", c_int, [ctypes.c_char_p]),
     ("tl_nccl_comm_init", c_int, [ctypes.POINTER(c_void_p), c_int, ctypes.c_char_p, c_int, c_int]),
