@@ -474,6 +474,38 @@ int  tl_distill_topk(int dtype, int64_t rows, int64_t classes, int64_t top, cons
                      int64_t lddz, int accumulate, void* scratch, size_t scratch_bytes,
                      void* stream);
 
+/* Cross entropy of a linear layer over a large vocabulary, without keeping the
+ * logits:
+ *   z = x W (+ bias)      W [width, classes] (trans_w 0, as linear's weights)
+ *                         or stored [classes, width] (trans_w 1, tied embeddings)
+ *   lse = log sum exp(z)  row_loss = lse - z[target]  loss = sum(row_loss) / divisor
+ * x [rows, width] and W have the element type, bias [classes] is float or null,
+ * target [rows] the index type; loss [1], row_loss and lse [rows] are float and
+ * may be null.  A class whose bias is -inf takes no part; a row with no class
+ * left has lse = -inf, gradient -onehot and, where it counts, loss +inf, as has
+ * a row whose target is such a class. */
+size_t tl_linear_ce_scratch_bytes(int dtype, int trans_w, int64_t rows, int64_t classes,
+                                  int64_t width, int backward);
+int  tl_linear_ce(int dtype, int trans_w, int64_t rows, int64_t classes, int64_t width,
+                  const void* x, int64_t ldx, const void* W, int64_t ldw, const float* bias,
+                  const void* target, int index_type, float divisor, float* loss,
+                  float* row_loss, float* lse, void* scratch, size_t scratch_bytes,
+                  void* stream);
+/* Its gradients, from the lse that tl_linear_ce wrote:
+ *   g = (softmax(z) - onehot(target)) * upstream / divisor
+ *   dx = g W^T    dW = x^T g (W's shape and order)    dbias = sum over rows of g
+ * each may be null; none may overlap x or W.  accumulate: a sum of TL_ACC_DX,
+ * TL_ACC_DW and TL_ACC_DBIAS.  Scratch of tl_linear_ce_scratch_bytes(...,
+ * backward = 1) serves both calls. */
+#define TL_ACC_DW 2
+#define TL_ACC_DBIAS 4
+int  tl_linear_ce_backward(int dtype, int trans_w, int64_t rows, int64_t classes, int64_t width,
+                           const void* x, int64_t ldx, const void* W, int64_t ldw,
+                           const float* bias, const void* target, int index_type, float divisor,
+                           const float* lse, const float* upstream, void* dx, int64_t lddx,
+                           void* dW, int64_t lddw, float* dbias, int accumulate, void* scratch,
+                           size_t scratch_bytes, void* stream);
+
 /* Device-side error flag (TL_ERR_TIMEOUT after a bounded wait in a kernel
  * gave up; 0 if none).  reset != 0 clears it. */
 int  tl_device_error(int* code, int reset);

@@ -1,0 +1,1047 @@
+// Cross entropy of a linear layer over a large vocabulary, in pieces of the
+// vocabulary, without keeping the logits, and its gradients:
+//
+//   z = x W (+ bias)   lse_r = log sum_v exp z_rv   row_loss_r = lse_r - z_r,t
+//   g = (exp(z - lse) - onehot(t)) * upstream / divisor      (rows with a target)
+//   dx = g W^T    dW = x^T g    dbias = sum_rows g
+//
+// It is linear (kernel_generator.py:1584-1661), softmax (:564-640) and
+// cross_entropy (:1816-1885) with their VJPs as one operator: unfused, the
+// logits and the probabilities, [rows, classes] each, are written and read
+// several times, and kept until the backward.
+//
+// Forward: one matrix product whose epilogue reduces each row of a 256 x 256
+// tile of logits, still in registers, to (maximum, sum of exponentials) of 128
+// columns; a second kernel joins the columns of a row.  Backward, piece by
+// piece of the vocabulary: the same product again, its epilogue turning logits
+// into g (bf16 in scratch); then dx += g W^T (float32 in scratch) and dW = x^T g.
+// That is 8 x rows x classes x width operations instead of the 6 of an
+// unfused step; the two more buy not storing 4 bytes per logit.
+//
+// The product kernel computes 256 x 256 tiles by clusters of two CTAs
+// (tcgen05.mma.cta_group::2, operands by TMA in the 128-byte swizzle, two
+// accumulators of 256 columns in tensor memory), as gemm_tc.cu does for
+// float32 operands: warp 0 loads, warp 1 of the leading CTA issues the MMAs,
+// eight warps drain finished chunks of K into registers and run the epilogue
+// while the next chunk or tile is multiplied.  Operands are read in the major
+// order they have in memory (K-major or MN-major boxes); nothing is transposed.
+//
+// float32 operands: each is split exactly into three bf16 terms, a = a0 + a1 +
+// a2 (8 bits of the significand each), and six of the nine products are kept
+// (a0 b0, a0 b1, a1 b0, a1 b1, a0 b2, a2 b0; the others are below 2^-24), each
+// a bf16 product over the same K, exact up to its float32 sum.  Within a chunk
+// of K the small products come first: the tensor core's accumulator rounds
+// toward zero, and only a0 b0's additions meet a sum of full size.  The GEMM's
+// two-term scheme (gemm_tc.cu) has half the products and an error of 4e-6;
+// here that error would sit in gradients whose own size is a difference, p - 1,
+// and the float32 plain form's error is below 1e-6.
+//
+// g of bf16 operands is held in bf16, unscaled: each element is off by at most
+// 2^-9 of itself, independently of the others, so the sums dx and dW are off by
+// less than their own rounding to bf16.  The scale upstream / divisor is applied
+// in float32 afterwards.
+#include <math.h>
+
+#include <algorithm>
+#include <cstring>
+#include <mutex>
+
+#include "lm_common.cuh"
+#include "tc_ptx.cuh"
+
+namespace tl {
+namespace {
+
+constexpr int BK = 64;                   // bf16 per stage row: 128 bytes
+constexpr int TILE_BYTES = 128 * BK * 2; // 16 KB: 128 rows of A, or of B, per CTA
+constexpr int NST = 6;
+constexpr int EPI_WARPS = 8;
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int STG_TILE = 4096;           // per epilogue warp: 32 rows x 128 bytes
+constexpr int SMEM_BYTES = NST * 2 * TILE_BYTES + EPI_WARPS * STG_TILE + 1024 + 256;
+constexpr int TMEM_COLS = 512;
+static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
+
+// The six products of two three-term operands, smallest first; one product of
+// plain bf16 operands.
+constexpr int kTerms = 6;
+__device__ __constant__ const signed char kTermA[kTerms] = {2, 1, 0, 1, 0, 0};
+__device__ __constant__ const signed char kTermB[kTerms] = {0, 1, 2, 0, 1, 0};
+
+enum Epi { kStats, kGrad, kSum, kOut };
+
+struct TileParams {
+  int M, N, K;
+  int terms;      // 1, or kTerms
+  int kc;         // k-blocks per accumulation chunk
+  int splits;     // K split this many ways (kSum)
+  // kStats, kGrad
+  const float* bias;      // of this piece's columns, or null
+  const int32_t* target;  // [M]: class relative to the whole vocabulary, or -1
+  int col0;               // first class of this piece
+  float2* part;           // kStats: [slot][part_ld] (maximum, sum of exp)
+  int64_t part_ld;
+  float* zt;              // kStats: [M] logit of the target
+  const float* lse;       // kGrad
+  float* colsum;          // kGrad: [M / 32 rounded up][N] sums of g, or null
+  int planes;             // kGrad: terms of g (1 or 3)
+  // kSum
+  int add;                // add to the sums there
+  // kOut
+  const float* scale;     // one float on the device
+  void* out;
+  int64_t ldo;
+  int out_bf16, accumulate, tma_out;
+};
+
+// shared::cluster TMA load of a box at (c0, c1, plane), completing on the
+// leader's barrier
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                                 int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"((uint64_t)map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+// float32 sums in memory += a staged tile (one addition per element)
+__device__ __forceinline__ void tma_add_3d(const CUtensorMap* map, uint32_t src, int c0, int c1,
+                                           int c2) {
+  asm volatile(
+      "cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.bulk_group [%0, {%2, %3, %4}], [%1];"
+      ::"l"((uint64_t)map), "r"(src), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
+// Shared-memory matrix descriptors (128-byte swizzle), 16-deep k-step k.
+//   K-major tile: rows of 128 bytes, 8-row groups 1 KB apart; a k-step is 32
+//   bytes into the row.
+//   MN-major tile: chunks of 64 (M or N) x 64 k, 8 KB apart, a k a row of 128
+//   bytes; a k-step is 16 rows = 2 KB.
+template <int MN>
+__device__ __forceinline__ uint64_t tile_desc(uint32_t tile, int k) {
+  const uint32_t a = tile + (MN ? 2048u : 32u) * (uint32_t)k;
+  uint64_t d = 0;
+  d |= (uint64_t)((a >> 4) & 0x3FFF);
+  d |= (uint64_t)(((MN ? 8192 : 16) >> 4) & 0x3FFF) << 16;
+  d |= (uint64_t)((1024 >> 4) & 0x3FFF) << 32;
+  d |= (uint64_t)1 << 46;  // descriptor version for tcgen05
+  d |= (uint64_t)2 << 61;  // 128-byte swizzle
+  return d;
+}
+// kind::f16, bf16 operands, float32 accumulator, 256 x 256 over the CTA pair
+template <int A_MN, int B_MN>
+constexpr uint32_t idesc() {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16) |
+         ((uint32_t)(256 >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+}
+
+struct Tile {
+  int split, m0, n0, kb0, nk;
+};
+// Tile g: bands of eight M tiles, within a band M fastest (a wave of clusters
+// shares a few row blocks of A and of B in L2); splits of K outermost.
+__device__ __forceinline__ Tile tile_of(const TileParams& p, int g) {
+  constexpr int kBand = 8;
+  const int mt = (p.M + 255) / 256, nt = (p.N + 255) / 256, nk = (p.K + BK - 1) / BK;
+  Tile t;
+  t.split = g / (mt * nt);
+  const int r = g - t.split * mt * nt;
+  const int band = r / (kBand * nt), in = r - band * kBand * nt;
+  const int rows = min(kBand, mt - band * kBand);
+  t.m0 = (band * kBand + in % rows) * 256;
+  t.n0 = in / rows * 256;
+  t.kb0 = (int)((int64_t)t.split * nk / p.splits);
+  t.nk = (int)((int64_t)(t.split + 1) * nk / p.splits) - t.kb0;
+  return t;
+}
+
+__device__ __forceinline__ float exp_fast(float x) {  // e^x within 2 ulp of 2^(x log2 e)
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+  return r;
+}
+
+// bits of two bf16, and what their rounding left over
+__device__ __forceinline__ uint32_t take_bf16(float& a, float& b) {
+  const uint32_t w = pack2_bf16(a, b);
+  a -= __uint_as_float(w << 16);
+  b -= __uint_as_float(w & 0xffff0000u);
+  return w;
+}
+
+// 32 rows (a lane each) x 64 bf16 columns, w[j] holding columns 2j and 2j + 1:
+// staged in the tensor map's 128-byte swizzle, stored by TMA.
+__device__ __forceinline__ void store_slab16(const CUtensorMap* map, uint32_t stg, int lane,
+                                             const uint32_t (&w)[32], int c0, int r0, int plane) {
+  if (lane == 0) bulk_wait_read();
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                     stg + (uint32_t)lane * 128u + ((uint32_t)(j ^ (lane & 7)) << 4)),
+                 "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
+                 : "memory");
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    tma_store_3d(map, stg, c0, r0, plane);
+    bulk_commit();
+  }
+}
+
+// A: x, g or x^T ...; TA 0: stored [M][K], 1: [K][M].  TB 0: B stored [K][N], 1: [N][K].
+template <int TA, int TB, int EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+    vocab_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                      const __grid_constant__ CUtensorMap tmC, const TileParams p) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  unsigned char* staging = smem + NST * 2 * TILE_BYTES;
+  uint64_t* full = (uint64_t*)(staging + EPI_WARPS * STG_TILE);  // [NST] loads of both CTAs -> MMA
+  uint64_t* empty = full + NST;                                  // [NST] MMA -> each producer
+  uint64_t* acc_full = empty + NST;                              // [2] MMA -> each epilogue
+  uint64_t* acc_free = acc_full + 2;                             // [2] both epilogues -> MMA
+  uint32_t* tmem_slot = (uint32_t*)(acc_free + 2);
+
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tiles = p.splits * ((p.M + 255) / 256) * ((p.N + 255) / 256);
+  const int step = (int)(gridDim.x >> 1), first = (int)(blockIdx.x >> 1);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NST; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&acc_full[b]), 1);
+      mbar_init(smem_u32(&acc_free[b]), 2 * EPI_WARPS);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  cluster_sync_all();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // The stage ring (it) and the two accumulators (cg) run on across tiles, so
+  // the next tile's loads and MMAs overlap this one's epilogue.
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      const uint32_t full0 = mapa_shared(smem_u32(&full[0]), 0);
+      bool ok = true;
+      uint32_t it = 0;
+      for (int g = first; g < tiles && ok; g += step) {
+        const Tile t = tile_of(p, g);
+        const int m0 = t.m0 + 128 * (int)rank, n0 = t.n0 + 128 * (int)rank;
+        for (int c = 0; c < t.nk && ok; c += p.kc) {
+          const int cend = min(c + p.kc, t.nk);
+          for (int q = 0; q < p.terms && ok; ++q) {
+            const int pa = p.terms == 1 ? 0 : kTermA[q], pb = p.terms == 1 ? 0 : kTermB[q];
+            for (int kb = c; kb < cend; ++kb, ++it) {
+              const uint32_t s = it % NST, ph = (it / NST) & 1;
+              if (it >= NST && !mbar_wait(smem_u32(&empty[s]), ph ^ 1)) {
+                ok = false;
+                break;
+              }
+              const uint32_t sA = smem_u32(smem + s * 2 * TILE_BYTES), sB = sA + TILE_BYTES;
+              const uint32_t fb = full0 + 8u * s;
+              if (leader) mbar_expect_tx(smem_u32(&full[s]), 4 * TILE_BYTES);
+              const int k0 = (t.kb0 + kb) * BK;
+              if constexpr (TA == 0) {
+                tma_load_3d_pair(sA, &tmA, fb, k0, m0, pa);
+              } else {
+                tma_load_3d_pair(sA, &tmA, fb, m0, k0, pa);
+                tma_load_3d_pair(sA + 8192, &tmA, fb, m0 + 64, k0, pa);
+              }
+              if constexpr (TB == 1) {
+                tma_load_3d_pair(sB, &tmB, fb, k0, n0, pb);
+              } else {
+                tma_load_3d_pair(sB, &tmB, fb, n0, k0, pb);
+                tma_load_3d_pair(sB + 8192, &tmB, fb, n0 + 64, k0, pb);
+              }
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // --------------------------------------------------------- MMA (leader)
+    if (leader && lane == 0) {
+      bool ok = true;
+      uint32_t it = 0, cg = 0;
+      for (int g = first; g < tiles && ok; g += step) {
+        const Tile t = tile_of(p, g);
+        for (int c = 0; c < t.nk && ok; c += p.kc, ++cg) {
+          const int n = (min(c + p.kc, t.nk) - c) * p.terms;
+          const uint32_t b = cg & 1, acc = tmem + b * 256;
+          if (cg >= 2 && !mbar_wait(smem_u32(&acc_free[b]), ((cg >> 1) - 1) & 1)) {
+            ok = false;
+            break;
+          }
+          fence_after();
+          for (int i = 0; i < n; ++i, ++it) {
+            const uint32_t s = it % NST, ph = (it / NST) & 1;
+            if (!mbar_wait(smem_u32(&full[s]), ph)) {
+              ok = false;
+              break;
+            }
+            fence_after();
+            const uint32_t sA = smem_u32(smem + s * 2 * TILE_BYTES), sB = sA + TILE_BYTES;
+#pragma unroll
+            for (int k = 0; k < BK / 16; ++k)
+              mma2_bf16(acc, tile_desc<TA>(sA, k), tile_desc<1 - TB>(sB, k), idesc<TA, 1 - TB>(),
+                        (i == 0 && k == 0) ? 0u : 1u);
+            mma2_commit_both(smem_u32(&empty[s]));
+          }
+          mma2_commit_both(smem_u32(&acc_full[b]));
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ----------------------------------------------------------- epilogue
+    const int e = warp - 2, quarter = warp & 3, half = e >> 2;
+    const uint32_t free0 = mapa_shared(smem_u32(&acc_free[0]), 0);
+    const uint32_t tbase = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
+    const uint32_t stg = smem_u32(staging + e * STG_TILE);
+    float v[128];
+    bool ok = true;
+    uint32_t cg = 0;
+    for (int g = first; g < tiles && ok; g += step) {
+      const Tile t = tile_of(p, g);
+#pragma unroll
+      for (int j = 0; j < 128; ++j) v[j] = 0.f;
+      for (int c = 0; c < t.nk; c += p.kc, ++cg) {
+        const uint32_t b = cg & 1;
+        if (!mbar_wait(smem_u32(&acc_full[b]), (cg >> 1) & 1)) {
+          ok = false;
+          break;
+        }
+        fence_after();
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          float r[16];
+          tmem_ld16(tbase + b * 256 + q * 16, r);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[q * 16 + j] += r[j];
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(free0 + 8u * b);
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const int r0 = t.m0 + 128 * (int)rank + quarter * 32, row = r0 + lane;
+      const int n0 = t.n0 + half * 128;
+      const int cols = min(128, p.N - n0);  // of this warp; may be <= 0
+      if (r0 >= p.M || cols <= 0) continue;
+      const bool live = row < p.M;
+
+      if constexpr (EPI == kStats || EPI == kGrad) {
+        if (p.bias) {
+#pragma unroll
+          for (int j = 0; j < 128; ++j)
+            if (j < cols) v[j] += __ldg(p.bias + n0 + j);
+        }
+        const int target = live ? p.target[row] - p.col0 - n0 : -1;  // in this warp's columns
+        if constexpr (EPI == kStats) {
+          if (cols < 128) {
+#pragma unroll
+            for (int j = 0; j < 128; ++j)
+              if (j >= cols) v[j] = -INFINITY;
+          }
+          float m = v[0];
+#pragma unroll
+          for (int j = 1; j < 128; ++j) m = fmaxf(m, v[j]);
+          const float base = m == -INFINITY ? 0.f : m;
+          float s = 0.f;
+#pragma unroll
+          for (int j = 0; j < 128; ++j) s += exp_fast(v[j] - base);
+          if (live) {
+            p.part[(int64_t)(n0 >> 7) * p.part_ld + row] = make_float2(m, s);
+            if (target >= 0 && target < cols) {
+              float z = 0.f;
+#pragma unroll
+              for (int j = 0; j < 128; ++j) z = j == target ? v[j] : z;
+              p.zt[row] = z;
+            }
+          }
+        } else {
+          // g = p - onehot; 0 for rows without a target
+          const bool counts = live && p.target[row] >= 0;
+          const float lse = counts ? p.lse[row] : 0.f;
+          // nothing left of the row: p = 0
+          const bool none = lse == -INFINITY;
+#pragma unroll
+          for (int j = 0; j < 128; ++j) {
+            v[j] = counts && !none ? exp_fast(v[j] - lse) : 0.f;
+            if (counts && j == target) v[j] -= 1.f;
+          }
+          if (p.colsum) {  // before g is rounded
+            float* cs = p.colsum + (int64_t)(r0 >> 5) * p.N + n0;
+#pragma unroll
+            for (int sl = 0; sl < 4; ++sl) {
+              if (lane == 0) bulk_wait_read();
+              __syncwarp();
+              // element (row lane, column j) at j ^ lane: no bank conflicts either way
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(stg + 4u * (uint32_t)(lane * 32 + (j ^ lane))),
+                             "f"(v[32 * sl + j])
+                             : "memory");
+              __syncwarp();
+              float s = 0.f;
+#pragma unroll
+              for (int r = 0; r < 32; ++r) {
+                float q;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(q)
+                             : "r"(stg + 4u * (uint32_t)(r * 32 + (lane ^ r)))
+                             : "memory");
+                s += q;
+              }
+              if (32 * sl + lane < cols) cs[32 * sl + lane] = s;
+              __syncwarp();
+            }
+          }
+          for (int pl = 0; pl < p.planes; ++pl) {
+#pragma unroll
+            for (int sl = 0; sl < 2; ++sl) {
+              uint32_t w[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) w[j] = take_bf16(v[64 * sl + 2 * j], v[64 * sl + 2 * j + 1]);
+              if (64 * sl < cols) store_slab16(&tmC, stg, lane, w, n0 + 64 * sl, r0, pl);
+            }
+          }
+        }
+      } else if constexpr (EPI == kSum) {
+#pragma unroll
+        for (int sl = 0; sl < 4; ++sl) {
+          if (32 * sl >= cols) break;
+          if (lane == 0) bulk_wait_read();
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            st_shared_v4(stg + (uint32_t)lane * 128u + ((uint32_t)(j ^ (lane & 7)) << 4), v[32 * sl + 4 * j],
+                         v[32 * sl + 4 * j + 1], v[32 * sl + 4 * j + 2], v[32 * sl + 4 * j + 3]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (p.add)
+              tma_add_3d(&tmC, stg, n0 + 32 * sl, r0, t.split);
+            else
+              tma_store_3d(&tmC, stg, n0 + 32 * sl, r0, t.split);
+            bulk_commit();
+          }
+        }
+      } else {
+        const float scale = *p.scale;
+#pragma unroll
+        for (int j = 0; j < 128; ++j) v[j] *= scale;
+        if (p.tma_out) {
+          if (p.out_bf16) {
+#pragma unroll
+            for (int sl = 0; sl < 2; ++sl) {
+              if (64 * sl >= cols) break;
+              uint32_t w[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) w[j] = pack2_bf16(v[64 * sl + 2 * j], v[64 * sl + 2 * j + 1]);
+              store_slab16(&tmC, stg, lane, w, n0 + 64 * sl, r0, 0);
+            }
+          } else {
+#pragma unroll
+            for (int sl = 0; sl < 4; ++sl) {
+              if (32 * sl >= cols) break;
+              uint32_t w[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(v[32 * sl + j]);
+              store_slab16(&tmC, stg, lane, w, n0 + 32 * sl, r0, 0);
+            }
+          }
+        } else {
+          // any alignment, or adding to what is there: through shared memory,
+          // a row's 32 columns per access
+#pragma unroll
+          for (int sl = 0; sl < 4; ++sl) {
+            if (32 * sl >= cols) break;
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              asm volatile("st.shared.f32 [%0], %1;" ::"r"(stg + 4u * (uint32_t)(lane * 32 + (j ^ lane))),
+                           "f"(v[32 * sl + j])
+                           : "memory");
+            __syncwarp();
+            const int c = 32 * sl + lane, rows = min(32, p.M - r0);
+            for (int r = 0; r < rows; ++r) {
+              float q;
+              asm volatile("ld.shared.f32 %0, [%1];" : "=f"(q)
+                           : "r"(stg + 4u * (uint32_t)(r * 32 + (lane ^ r)))
+                           : "memory");
+              if (c >= cols) continue;
+              const int64_t at = (int64_t)(r0 + r) * p.ldo + n0 + c;
+              if (p.out_bf16) {
+                __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + at;
+                *o = __float2bfloat16_rn(p.accumulate ? __bfloat162float(*o) + q : q);
+              } else {
+                float* o = static_cast<float*>(p.out) + at;
+                *o = p.accumulate ? *o + q : q;
+              }
+            }
+          }
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_all();  // the staging outlives every TMA store's read
+    __syncwarp();
+  }
+  fence_before();
+  cluster_sync_all();  // neither CTA frees tensor memory or exits while the pair works
+  if (warp == 1) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS)
+                 : "memory");
+  }
+}
+
+// Scratch words before the arrays, zero between calls: [0] rows joined so far.
+struct Head {
+  unsigned joined;
+  unsigned pad0;
+  float scale;   // backward: upstream / divisor
+  float inv;     // unused slot kept for alignment
+};
+
+// Classes of the rows as int32 (-1: none); no order, no sums.
+__global__ void __launch_bounds__(256) targets_kernel(const void* target, int type, int64_t rows,
+                                                      int64_t classes, int32_t* out) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows; i += 256LL * gridDim.x)
+    out[i] = (int32_t)class_index(target, type, i, classes);
+}
+
+// Rows with a target, by one block; every thread gets the count.
+__device__ __forceinline__ int64_t count_targets(const int32_t* t, int64_t rows, long long* sh) {
+  long long n = 0;
+  for (int64_t i = threadIdx.x; i < rows; i += blockDim.x) n += t[i] >= 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = n;
+  __syncthreads();
+  n = 0;
+  for (unsigned i = 0; i < blockDim.x / 32; ++i) n += sh[i];
+  return n;
+}
+
+// scale = upstream / divisor
+__global__ void __launch_bounds__(1024) scale_kernel(const int32_t* t, int64_t rows, float divisor,
+                                                     const float* upstream, float* scale) {
+  __shared__ long long sh[32];
+  float d = divisor;
+  if (!(d > 0.f)) d = fmaxf(1.f, (float)count_targets(t, rows, sh));
+  if (threadIdx.x == 0) *scale = (upstream ? *upstream : 1.f) / d;
+}
+
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+  const float M = fmaxf(m, m2), base = M == -INFINITY ? 0.f : M;
+  s = s * exp_fast(m - base) + s2 * exp_fast(m2 - base);
+  m = M;
+}
+
+// Joins a piece's partials of 32 rows: warp w takes slots w, w + 8, ...; the
+// last piece writes lse and the losses, and the last block the mean.
+__global__ void __launch_bounds__(256) join_kernel(const float2* part, int64_t part_ld, int slots,
+                                                   int64_t rows, const int32_t* target,
+                                                   const float* zt, float2* run, int first, int last,
+                                                   float divisor, float* row_loss, float* lse,
+                                                   float* loss, Head* head) {
+  __shared__ float2 sh[8][33];
+  __shared__ unsigned ticket;
+  __shared__ long long shn[8];
+  __shared__ double shd[8];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * 32 + lane;
+  float m = -INFINITY, s = 0.f;
+  if (row < rows)
+    for (int i = w; i < slots; i += 8) {
+      const float2 q = __ldcs(part + (int64_t)i * part_ld + row);
+      join(m, s, q.x, q.y);
+    }
+  sh[w][lane] = make_float2(m, s);
+  __syncthreads();
+  if (w == 0 && row < rows) {
+    for (int i = 1; i < 8; ++i) join(m, s, sh[i][lane].x, sh[i][lane].y);
+    if (!first) join(m, s, run[row].x, run[row].y);
+    if (!last) {
+      run[row] = make_float2(m, s);
+    } else {
+      const float l = m + logf(s);  // a row of -inf: -inf
+      if (lse) lse[row] = l;
+      float v = 0.f;
+      // (m - zt) + log s: lse - zt would round lse first
+      if (target[row] >= 0) v = zt[row] == -INFINITY ? INFINITY : (m - zt[row]) + logf(s);
+      row_loss[row] = v;
+    }
+  }
+  if (!last || !loss) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) ticket = atomicAdd(&head->joined, 1u);
+  __syncthreads();
+  if (ticket != gridDim.x - 1) return;
+  __threadfence();
+  double t = 0.0;
+  for (int64_t i = threadIdx.x; i < rows; i += 256) t += (double)__ldcg(row_loss + i);
+  t = warp_sum(t);
+  if (lane == 0) shd[w] = t;
+  const int64_t n = divisor > 0.f ? 1 : count_targets(target, rows, shn);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    t = 0.0;
+    for (int i = 0; i < 8; ++i) t += shd[i];
+    const float d = divisor > 0.f ? divisor : fmaxf(1.f, (float)n);
+    *loss = (float)(t / (double)d);
+    head->joined = 0u;
+  }
+}
+
+// The terms of a matrix as bf16 planes [planes][rows][ld], columns past `cols`
+// zero: three that sum to a float32 matrix exactly, or a copy of a bf16 one
+// whose rows TMA cannot address.
+template <typename T>
+__global__ void __launch_bounds__(256) planes_kernel(const T* __restrict__ X, int64_t ldx, int64_t rows,
+                                                     int64_t cols, int planes,
+                                                     __nv_bfloat16* __restrict__ out, int64_t ld) {
+  const int64_t pairs = ld / 2, n = rows * pairs;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += 256LL * gridDim.x) {
+    const int64_t r = i / pairs, c = 2 * (i - r * pairs);
+    float a = c < cols ? to_f32(X[r * ldx + c]) : 0.f;
+    float b = c + 1 < cols ? to_f32(X[r * ldx + c + 1]) : 0.f;
+    for (int p = 0; p < planes; ++p)
+      *reinterpret_cast<uint32_t*>(out + ((int64_t)p * rows + r) * ld + c) = take_bf16(a, b);
+  }
+}
+
+// dx = scale * (sum of the splits' sums) (+ dx)
+template <typename T>
+__global__ void __launch_bounds__(256) dx_kernel(const float* __restrict__ sums, int splits, int64_t rows,
+                                                 int64_t cols, int64_t ld, const float* scale, T* dx,
+                                                 int64_t lddx, int accumulate) {
+  const float k = *scale;
+  const int64_t n = rows * cols;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += 256LL * gridDim.x) {
+    const int64_t r = i / cols, c = i - r * cols;
+    float s = 0.f;
+    for (int p = 0; p < splits; ++p) s += sums[((int64_t)p * rows + r) * ld + c];
+    T* o = dx + r * lddx + c;
+    from_f32(o, (accumulate ? to_f32(*o) : 0.f) + k * s);
+  }
+}
+
+// dbias of a piece: the row groups' column sums in order, four chains.
+__global__ void __launch_bounds__(256) dbias_kernel(const float* __restrict__ colsum, int64_t groups,
+                                                    int64_t cols, const float* scale, float* dbias,
+                                                    int accumulate) {
+  __shared__ float sh[8][33];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  float s = 0.f;
+  if (c < cols)
+    for (int64_t g = w; g < groups; g += 8) s += colsum[g * cols + c];
+  sh[w][lane] = s;
+  __syncthreads();
+  if (w == 0 && c < cols) {
+    for (int i = 1; i < 8; ++i) s += sh[i][lane];
+    dbias[c] = (accumulate ? dbias[c] : 0.f) + *scale * s;
+  }
+}
+
+// ------------------------------------------------------------- host side ---
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    cudaDriverEntryPointQueryResult q;
+    void* f = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return (EncodeTiled)f;
+  }();
+  return fn;
+}
+
+// [planes][rows][cols] with row stride ld and plane stride rows * ld, boxes of
+// box_c x box_r x 1 in the 128-byte swizzle.
+bool make_map3(CUtensorMap* m, const void* base, bool f32, int64_t planes, int64_t rows, int64_t cols,
+               int64_t ld, uint32_t box_c, uint32_t box_r) {
+  const EncodeTiled enc = encode_tiled();
+  if (!enc) return false;
+  const int64_t es = f32 ? 4 : 2;
+  // a single row or plane is never stepped over, but strides must be multiples of 16
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+  const cuuint64_t strides[2] = {(cuuint64_t)(ld * es), (cuuint64_t)(rows * ld * es)};
+  const cuuint32_t box[3] = {box_c, box_r, 1}, one[3] = {1, 1, 1};
+  return enc(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+             const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// An operand in memory that TMA can address: bf16 planes.
+struct Planes {
+  const __nv_bfloat16* p;
+  int64_t planes, rows, cols, ld;
+};
+// as the K-major operand (stored [MN][K]) or the MN-major one ([K][MN])
+bool k_major(CUtensorMap* m, const Planes& x) {
+  return make_map3(m, x.p, false, x.planes, x.rows, x.cols, x.ld, 64, 128);
+}
+bool mn_major(CUtensorMap* m, const Planes& x) {
+  return make_map3(m, x.p, false, x.planes, x.rows, x.cols, x.ld, 64, 64);
+}
+
+template <int TA, int TB, int EPI>
+int launch_tiles(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c, const TileParams& p,
+                 cudaStream_t st) {
+  auto kern = vocab_tile_kernel<TA, TB, EPI>;
+  TL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
+  const int64_t tiles = (int64_t)p.splits * ((p.M + 255) / 256) * ((p.N + 255) / 256);
+  if (tiles > INT32_MAX / 2) return TL_ERR_UNSUPPORTED;
+  const int64_t clusters = std::min<int64_t>(tiles, std::max(1, sm_count() / 2));
+  kern<<<(unsigned)(2 * clusters), THREADS, SMEM_BYTES, st>>>(a, b, c, p);
+  return after_launch();
+}
+
+constexpr int64_t up_to(int64_t n, int64_t k) { return (n + k - 1) / k * k; }
+
+struct Call {
+  int dtype, trans_w, index_type;
+  int64_t rows, classes, width;
+  const void* x;
+  int64_t ldx;
+  const void* w;
+  int64_t ldw;
+  const float* bias;
+  const void* target;
+  float divisor;
+  char* scratch;
+  cudaStream_t st;
+  bool f32() const { return dtype == TL_F32; }
+  int planes() const { return f32() ? 3 : 1; }
+  int terms() const { return f32() ? kTerms : 1; }
+  // chunks of K per accumulator: 1024 deep, or 256 (x 6 products)
+  int kc() const { return f32() ? 4 : 16; }
+};
+
+// How a call is cut: classes per piece, and where its arrays are in scratch.
+struct Plan {
+  int64_t fpiece, bpiece;          // classes per piece, forward and backward
+  int64_t part_ld;                 // rows of the forward's partials
+  int splits;                      // of K in dx
+  int64_t targets, xplanes, wplanes, zt, run, row_loss, part, g, sums, colsum, total;  // offsets
+};
+
+// splits of K that let few tiles of dx fill the GPU: whole waves of clusters
+int dx_splits(int64_t rows, int64_t width, int64_t piece) {
+  const int64_t tiles = ((rows + 255) / 256) * ((width + 255) / 256), nk = piece / BK;
+  const int64_t slots = std::max(1, sm_count() / 2);
+  int best = 1;
+  double eff = 0;
+  for (int s = 1; s <= 16 && (s == 1 || nk / s >= 8); ++s) {
+    const int64_t n = tiles * s, waves = (n + slots - 1) / slots;
+    const double f = (double)n / (double)(waves * slots);
+    if (f > eff + 0.02) {
+      eff = f;
+      best = s;
+    }
+    if (n >= 4 * slots) break;
+  }
+  return best;
+}
+
+Plan make_plan(int dtype, int trans_w, int64_t rows, int64_t classes, int64_t width, bool backward) {
+  Plan q{};
+  const int64_t P = dtype == TL_F32 ? 3 : 1, all = up_to(classes, 256);
+  auto piece = [&](int64_t bytes_per_class, int64_t cap) {
+    return std::min<int64_t>(all, std::max<int64_t>(256, cap / std::max<int64_t>(1, bytes_per_class) / 256 * 256));
+  };
+  q.part_ld = up_to(rows, 32);
+  const int64_t cap = 512LL << 20;
+  // the partials (8 bytes per row and 128 classes) and the terms of W
+  q.fpiece = std::min(piece(q.part_ld / 16, cap), piece(width * 2 * P, cap));
+  q.bpiece = std::min(piece(rows * 2 * P, cap), piece(width * 2 * P, cap));
+  q.splits = backward ? dx_splits(rows, width, q.bpiece) : 1;
+  int64_t at = 1024;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at = up_to(at + bytes, 1024);
+    return o;
+  };
+  q.targets = take(rows * 4);
+  q.xplanes = take(P * rows * up_to(width, 8) * 2);
+  const int64_t wp = backward ? std::max(q.fpiece, q.bpiece) : q.fpiece;
+  q.wplanes = take(P * (trans_w ? wp * up_to(width, 8) : width * up_to(wp, 8)) * 2);
+  const int64_t common = at;
+  q.zt = take(rows * 4);
+  q.run = take(rows * 8);
+  q.row_loss = take(rows * 4);
+  q.part = take(q.fpiece / 128 * q.part_ld * 8);
+  q.total = at;
+  if (backward) {
+    at = common;
+    q.g = take(P * rows * q.bpiece * 2);
+    q.sums = take((int64_t)q.splits * rows * up_to(width, 4) * 4);
+    q.colsum = take(up_to(rows, 32) / 32 * q.bpiece * 4);
+    q.total = std::max(q.total, at);
+  }
+  return q;
+}
+
+template <typename T>
+int write_planes(const T* X, int64_t ldx, int64_t rows, int64_t cols, int planes, __nv_bfloat16* out,
+                 int64_t ld, cudaStream_t st) {
+  const int64_t blocks = std::min<int64_t>((rows * (ld / 2) + 255) / 256, 16LL * sm_count());
+  planes_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(X, ldx, rows, cols, planes, out, ld);
+  return after_launch();
+}
+
+// rows x cols of X as planes: itself where TMA can address it, else a copy
+int as_planes(const Call& c, const void* X, int64_t ldx, int64_t rows, int64_t cols, int64_t scratch_at,
+              Planes* out) {
+  if (!c.f32() && ldx % 8 == 0 && aligned_to(X, 16)) {
+    *out = {static_cast<const __nv_bfloat16*>(X), 1, rows, cols, ldx};
+    return TL_OK;
+  }
+  __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(c.scratch + scratch_at);
+  *out = {dst, c.planes(), rows, cols, up_to(cols, 8)};
+  if (c.f32())
+    return write_planes(static_cast<const float*>(X), ldx, rows, cols, 3, dst, out->ld, c.st);
+  return write_planes(static_cast<const __nv_bfloat16*>(X), ldx, rows, cols, 1, dst, out->ld, c.st);
+}
+
+// classes c0 .. c0 + n of W
+int w_planes(const Call& c, const Plan& q, int64_t c0, int64_t n, Planes* out) {
+  const int64_t es = (int64_t)elem_bytes(c.dtype);
+  const char* w = static_cast<const char*>(c.w) + (c.trans_w ? c0 * c.ldw : c0) * es;
+  return c.trans_w ? as_planes(c, w, c.ldw, n, c.width, q.wplanes, out)
+                   : as_planes(c, w, c.ldw, c.width, n, q.wplanes, out);
+}
+
+// The logits' product over classes c0 .. c0 + n, with epilogue EPI.
+template <int EPI>
+int logits(const Call& c, const Planes& x, const Planes& w, const CUtensorMap& out, TileParams p,
+           int64_t c0, int64_t n) {
+  CUtensorMap a, b;
+  if (!k_major(&a, x) || !(c.trans_w ? k_major(&b, w) : mn_major(&b, w))) return TL_ERR_UNSUPPORTED;
+  p.M = (int)c.rows;
+  p.N = (int)n;
+  p.K = (int)c.width;
+  p.terms = c.terms();
+  p.kc = c.kc();
+  p.splits = 1;
+  p.bias = c.bias ? c.bias + c0 : nullptr;
+  p.col0 = (int)c0;
+  return c.trans_w ? launch_tiles<0, 1, EPI>(a, b, out, p, c.st)
+                   : launch_tiles<0, 0, EPI>(a, b, out, p, c.st);
+}
+
+int forward(const Call& c, const Plan& q, float* loss, float* row_loss, float* lse) {
+  int32_t* targets = reinterpret_cast<int32_t*>(c.scratch + q.targets);
+  targets_kernel<<<(unsigned)std::min<int64_t>((c.rows + 255) / 256, 4LL * sm_count()), 256, 0, c.st>>>(
+      c.target, c.index_type, c.rows, c.classes, targets);
+  TL_TRY(after_launch());
+  Planes x, w;
+  TL_TRY(as_planes(c, c.x, c.ldx, c.rows, c.width, q.xplanes, &x));
+  TileParams p{};
+  p.target = targets;
+  p.part = reinterpret_cast<float2*>(c.scratch + q.part);
+  p.part_ld = q.part_ld;
+  p.zt = reinterpret_cast<float*>(c.scratch + q.zt);
+  if (!row_loss) row_loss = reinterpret_cast<float*>(c.scratch + q.row_loss);
+  CUtensorMap none;
+  memset(&none, 0, sizeof(none));
+  for (int64_t c0 = 0; c0 < c.classes; c0 += q.fpiece) {
+    const int64_t n = std::min(q.fpiece, c.classes - c0);
+    TL_TRY(w_planes(c, q, c0, n, &w));
+    TL_TRY(logits<kStats>(c, x, w, none, p, c0, n));
+    join_kernel<<<(unsigned)(q.part_ld / 32), 256, 0, c.st>>>(
+        p.part, q.part_ld, (int)((n + 127) / 128), c.rows, targets, p.zt,
+        reinterpret_cast<float2*>(c.scratch + q.run), c0 == 0, c0 + n == c.classes, c.divisor, row_loss,
+        lse, loss, reinterpret_cast<Head*>(c.scratch));
+    TL_TRY(after_launch());
+  }
+  return TL_OK;
+}
+
+int backward(const Call& c, const Plan& q, const float* lse, const float* upstream, void* dx, int64_t lddx,
+             void* dW, int64_t lddw, float* dbias, int accumulate) {
+  int32_t* targets = reinterpret_cast<int32_t*>(c.scratch + q.targets);
+  float* scale = &reinterpret_cast<Head*>(c.scratch)->scale;
+  targets_kernel<<<(unsigned)std::min<int64_t>((c.rows + 255) / 256, 4LL * sm_count()), 256, 0, c.st>>>(
+      c.target, c.index_type, c.rows, c.classes, targets);
+  TL_TRY(after_launch());
+  scale_kernel<<<1, 1024, 0, c.st>>>(targets, c.rows, c.divisor, upstream, scale);
+  TL_TRY(after_launch());
+  Planes x, w;
+  TL_TRY(as_planes(c, c.x, c.ldx, c.rows, c.width, q.xplanes, &x));
+  const int64_t es = (int64_t)elem_bytes(c.dtype);
+  float* sums = reinterpret_cast<float*>(c.scratch + q.sums);
+  float* colsum = reinterpret_cast<float*>(c.scratch + q.colsum);
+  const int64_t sums_ld = up_to(c.width, 4);
+  for (int64_t c0 = 0; c0 < c.classes; c0 += q.bpiece) {
+    const int64_t n = std::min(q.bpiece, c.classes - c0);
+    TL_TRY(w_planes(c, q, c0, n, &w));
+    const Planes g{reinterpret_cast<__nv_bfloat16*>(c.scratch + q.g), c.planes(), c.rows, n, q.bpiece};
+    CUtensorMap a, b, o;
+    if (!make_map3(&o, g.p, false, g.planes, g.rows, g.cols, g.ld, 64, 32)) return TL_ERR_UNSUPPORTED;
+    TileParams p{};
+    p.target = targets;
+    p.lse = lse;
+    p.planes = c.planes();
+    p.colsum = dbias ? colsum : nullptr;
+    TL_TRY(logits<kGrad>(c, x, w, o, p, c0, n));
+    p = TileParams{};
+    p.terms = c.terms();
+    p.kc = c.kc();
+    p.scale = scale;
+    if (dx) {  // sums[rows][width] += g W^T
+      p.M = (int)c.rows;
+      p.N = (int)c.width;
+      p.K = (int)n;
+      p.splits = q.splits;
+      p.add = c0 > 0;
+      if (!k_major(&a, g) || !(c.trans_w ? mn_major(&b, w) : k_major(&b, w)) ||
+          !make_map3(&o, sums, true, q.splits, c.rows, c.width, sums_ld, 32, 32))
+        return TL_ERR_UNSUPPORTED;
+      TL_TRY((c.trans_w ? launch_tiles<0, 0, kSum>(a, b, o, p, c.st)
+                        : launch_tiles<0, 1, kSum>(a, b, o, p, c.st)));
+    }
+    if (dW) {  // [classes][width] = g^T x, or [width][classes] = x^T g
+      p.M = (int)(c.trans_w ? n : c.width);
+      p.N = (int)(c.trans_w ? c.width : n);
+      p.K = (int)c.rows;
+      p.splits = 1;
+      p.out = static_cast<char*>(dW) + (c.trans_w ? c0 * lddw : c0) * es;
+      p.ldo = lddw;
+      p.out_bf16 = !c.f32();
+      p.accumulate = (accumulate & TL_ACC_DW) != 0;
+      memset(&o, 0, sizeof(o));
+      p.tma_out = !p.accumulate && (lddw * es) % 16 == 0 && aligned_to(p.out, 16) &&
+                  make_map3(&o, p.out, c.f32(), 1, p.M, p.N, lddw, c.f32() ? 32 : 64, 32);
+      const Planes& A = c.trans_w ? g : x;
+      const Planes& B = c.trans_w ? x : g;
+      if (!mn_major(&a, A) || !mn_major(&b, B)) return TL_ERR_UNSUPPORTED;
+      TL_TRY((launch_tiles<1, 0, kOut>(a, b, o, p, c.st)));
+    }
+    if (dbias) {
+      dbias_kernel<<<(unsigned)((n + 31) / 32), 256, 0, c.st>>>(
+          colsum, up_to(c.rows, 32) / 32, n, scale, dbias + c0, accumulate & TL_ACC_DBIAS);
+      TL_TRY(after_launch());
+    }
+  }
+  if (dx) {
+    const int64_t blocks = std::min<int64_t>((c.rows * c.width + 255) / 256, 16LL * sm_count());
+    if (c.f32())
+      dx_kernel<float><<<(unsigned)blocks, 256, 0, c.st>>>(sums, q.splits, c.rows, c.width, sums_ld, scale,
+                                                           static_cast<float*>(dx), lddx,
+                                                           accumulate & TL_ACC_DX);
+    else
+      dx_kernel<__nv_bfloat16><<<(unsigned)blocks, 256, 0, c.st>>>(
+          sums, q.splits, c.rows, c.width, sums_ld, scale, static_cast<__nv_bfloat16*>(dx), lddx,
+          accumulate & TL_ACC_DX);
+    TL_TRY(after_launch());
+  }
+  return TL_OK;
+}
+
+int check(const Call& c, size_t scratch_bytes, bool backward) {
+  if (!dtype_ok(c.dtype) || !index_ok(c.index_type)) return TL_ERR_INVALID_ARG;
+  if (c.trans_w != 0 && c.trans_w != 1) return TL_ERR_INVALID_ARG;
+  if (c.rows < 0 || c.classes <= 0 || c.width <= 0) return TL_ERR_INVALID_ARG;
+  if (c.rows > INT32_MAX / 2 || c.classes > INT32_MAX / 2 || c.width > INT32_MAX / 2)
+    return TL_ERR_UNSUPPORTED;
+  if (c.rows > 0 && (!c.x || !c.w || !c.target)) return TL_ERR_INVALID_ARG;
+  if (c.ldx < c.width || c.ldw < (c.trans_w ? c.width : c.classes)) return TL_ERR_INVALID_ARG;
+  if (!(c.divisor >= 0.f)) return TL_ERR_INVALID_ARG;
+  if (!c.scratch || !aligned_to(c.scratch, 16) ||
+      scratch_bytes < tl_linear_ce_scratch_bytes(c.dtype, c.trans_w, c.rows, c.classes, c.width, backward))
+    return TL_ERR_INVALID_ARG;
+  return TL_OK;
+}
+
+}  // namespace
+
+int linear_ce_device_error(int* code, int reset) { return read_device_error(code, reset); }
+
+}  // namespace tl
+
+extern "C" {
+
+size_t tl_linear_ce_scratch_bytes(int dtype, int trans_w, int64_t rows, int64_t classes, int64_t width,
+                                  int backward) {
+  if (!tl::dtype_ok(dtype) || rows < 0 || classes <= 0 || width <= 0) return 0;
+  return (size_t)tl::make_plan(dtype, trans_w, std::max<int64_t>(rows, 1), classes, width, backward != 0)
+      .total;
+}
+
+int tl_linear_ce(int dtype, int trans_w, int64_t rows, int64_t classes, int64_t width, const void* x,
+                 int64_t ldx, const void* W, int64_t ldw, const float* bias, const void* target,
+                 int index_type, float divisor, float* loss, float* row_loss, float* lse, void* scratch,
+                 size_t scratch_bytes, void* stream) {
+  tl::Call c{dtype, trans_w, index_type, rows, classes, width, x, ldx, W, ldw, bias, target, divisor,
+             static_cast<char*>(scratch), nullptr};
+  TL_TRY(tl::check(c, scratch_bytes, false));
+  if (!loss && !row_loss && !lse) return TL_ERR_INVALID_ARG;
+  c.st = tl::stream_or_default(stream);
+  if (rows == 0) {
+    if (loss) TL_CUDA_TRY(cudaMemsetAsync(loss, 0, sizeof(float), c.st));
+    return TL_OK;
+  }
+  return tl::forward(c, tl::make_plan(dtype, trans_w, rows, classes, width, false), loss, row_loss, lse);
+}
+
+int tl_linear_ce_backward(int dtype, int trans_w, int64_t rows, int64_t classes, int64_t width,
+                          const void* x, int64_t ldx, const void* W, int64_t ldw, const float* bias,
+                          const void* target, int index_type, float divisor, const float* lse,
+                          const float* upstream, void* dx, int64_t lddx, void* dW, int64_t lddw,
+                          float* dbias, int accumulate, void* scratch, size_t scratch_bytes,
+                          void* stream) {
+  tl::Call c{dtype, trans_w, index_type, rows, classes, width, x, ldx, W, ldw, bias, target, divisor,
+             static_cast<char*>(scratch), nullptr};
+  TL_TRY(tl::check(c, scratch_bytes, true));
+  if ((rows > 0 && !lse) || (!dx && !dW && !dbias)) return TL_ERR_INVALID_ARG;
+  if (accumulate & ~(TL_ACC_DX | TL_ACC_DW | TL_ACC_DBIAS)) return TL_ERR_INVALID_ARG;
+  if ((dx && lddx < width) || (dW && lddw < (trans_w ? width : classes))) return TL_ERR_INVALID_ARG;
+  // the gradients are written piece by piece, while x and W are still read
+  if ((dx && (dx == x || dx == W)) || (dW && (dW == W || dW == x)) || (dx && dx == dW))
+    return TL_ERR_INVALID_ARG;
+  c.st = tl::stream_or_default(stream);
+  if (rows == 0) {  // sums over no rows
+    const size_t es = tl::elem_bytes(dtype);
+    if (dW && !(accumulate & TL_ACC_DW))
+      TL_CUDA_TRY(cudaMemset2DAsync(dW, lddw * es, 0, (trans_w ? width : classes) * es,
+                                    trans_w ? classes : width, c.st));
+    if (dbias && !(accumulate & TL_ACC_DBIAS))
+      TL_CUDA_TRY(cudaMemsetAsync(dbias, 0, classes * sizeof(float), c.st));
+    return TL_OK;
+  }
+  return tl::backward(c, tl::make_plan(dtype, trans_w, rows, classes, width, true), lse, upstream, dx, lddx,
+                      dW, lddw, dbias, accumulate);
+}
+
+}  // extern "C"

@@ -39,6 +39,7 @@ IDX_F32, IDX_I32, IDX_I64 = 0, 1, 2    # class-index types
 NORM_LAYER, NORM_RMS = 0, 1
 GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_FULL = 0, 1, 2, 3
 ACC_DX, ACC_DU, ACC_DGATE, ACC_DW_POST, ACC_DW_PRE = 1, 2, 4, 8, 16
+ACC_DW, ACC_DBIAS = 2, 4
 
 
 class TLCudaError(RuntimeError):
@@ -153,6 +154,14 @@ _SIGS = [
                                 c_int64, c_void_p, c_int64, c_int, c_float, c_float, c_void_p,
                                 c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p,
                                 c_size_t, c_void_p]),
+    ("tl_linear_ce_scratch_bytes", c_size_t, [c_int, c_int, c_int64, c_int64, c_int64, c_int]),
+    ("tl_linear_ce", c_int, [c_int, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+                             c_int64, c_void_p, c_void_p, c_int, c_float, c_void_p, c_void_p,
+                             c_void_p, c_void_p, c_size_t, c_void_p]),
+    ("tl_linear_ce_backward", c_int, [c_int, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64,
+                                      c_void_p, c_int64, c_void_p, c_void_p, c_int, c_float,
+                                      c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
+                                      c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
     ("tl_device_error", c_int, [ctypes.POINTER(c_int), c_int]),
     ("tl_nccl_unique_id", c_int, [ctypes.c_char_p]),
     ("tl_nccl_comm_init", c_int, [ctypes.POINTER(c_void_p), c_int, ctypes.c_char_p, c_int, c_int]),

@@ -1,0 +1,244 @@
+"""tl_linear_ce and its gradients against the definition in float64.
+
+Tolerances, with S = |x| |W| (the magnitudes a logit sums): a product's terms
+are exact (bf16) or miss less than 3 * 2^-24 of themselves (float32 as three
+bf16 terms, six products); the tensor core's accumulator drops up to 2^-23 of
+the running sum at each of the additions of full-size terms in a chunk of K
+(1024 / 16 = 64 bf16, 256 / 16 = 16 float32), and chunks add in float32:
+  e = 1.2e-5 (bf16) or 4e-6 (float32) of the magnitudes summed, for logits and
+  for the gradients' products.
+A logit off by d changes p by the factor 1 + d, lse by at most d; exp, log and
+the sums of exponentials add 4e-6.  g is held as bf16 for bf16 operands (half a
+step of each element, p - 1 at the target included), as three terms for float32.  Outputs in bf16 add half a step of their own.
+"""
+import numpy as np
+import pytest
+
+from conftest import REPO  # noqa: F401
+from lm_util import BF16_STEP, CODE, Dev, rounded, rt
+from oracle import lm_ops
+
+pytestmark = pytest.mark.gpu
+
+IDX = {"f32": (rt.IDX_F32, np.float32), "i32": (rt.IDX_I32, np.int32), "i64": (rt.IDX_I64, np.int64)}
+GRADS = ("dx", "dw", "dbias")
+
+
+def inputs(rows, classes, width, dtype, bias=True, seed=0, ignored=True):
+    rng = np.random.default_rng(seed + 101 * rows + classes + width)
+    x = rounded(rng.standard_normal((rows, width)), dtype)
+    w = rounded(rng.standard_normal((width, classes)) * 1.5 / np.sqrt(width), dtype)
+    b = rounded(rng.standard_normal(classes) * 0.5, "f32") if bias else None
+    t = rng.integers(0, classes, rows)
+    if ignored and rows > 4:
+        t[rng.integers(0, rows, max(1, rows // 20))] = -100
+    return x, w, b, t
+
+
+def run(x, w, b, t, dtype, trans=0, idx="i64", divisor=0.0, up=None, pad=0, lead=0, want=GRADS, start=None,
+        calls=1, fwd=("loss", "row_loss", "lse")):
+    rows, width = x.shape
+    classes = w.shape[1]
+    code, ity = IDX[idx]
+    with Dev() as D:
+        L = rt.lib()
+        px, ldx = D.rows(x, dtype, width + pad, lead)
+        wm = w.T if trans else w
+        pw, ldw = D.rows(wm, dtype, wm.shape[1] + pad, lead)
+        pb = D.put(b, "f32")
+        pt = D.put(t.astype(ity))
+        nb = L.tl_linear_ce_scratch_bytes(CODE[dtype], trans, rows, classes, width, 1)
+        scratch = D.zeros(nb)
+        o = {k: D.new(1 if k == "loss" else rows) for k in set(fwd) | {"lse"}}
+        out = {}
+        base = (CODE[dtype], trans, rows, classes, width, px, ldx, pw, ldw, pb, pt, code, divisor)
+        pu = None if up is None else D.put(np.float32([up]))
+        start = start or {}
+        acc = sum({"dx": rt.ACC_DX, "dw": rt.ACC_DW, "dbias": rt.ACC_DBIAS}[k] for k in start)
+        g = {}
+        if "dx" in want:
+            g["dx"] = D.rows(start.get("dx", np.full(x.shape, 7.0)), dtype, ldx, lead)[0]
+        if "dw" in want:
+            s = start.get("dw", np.full(w.shape, 7.0))
+            g["dw"] = D.rows(s.T if trans else s, dtype, ldw, lead)[0]
+        if "dbias" in want and b is not None:
+            g["dbias"] = D.put(start.get("dbias", np.full(classes, 7.0)), "f32")
+        for _ in range(calls):
+            rt.check(L.tl_linear_ce(*base, o.get("loss"), o.get("row_loss"), o["lse"], scratch, nb, D.stream),
+                     "forward")
+            if g:
+                rt.check(L.tl_linear_ce_backward(*base, o["lse"], pu, g.get("dx"), ldx, g.get("dw"), ldw,
+                                                 g.get("dbias"), acc, scratch, nb, D.stream), "backward")
+        for k, p in o.items():
+            out[k] = D.get(p, (1,) if k == "loss" else (rows,))
+        if "dx" in g:
+            out["dx"], rest = D.get_rows(g["dx"], rows, width, ldx, dtype, lead)
+            assert np.all(rest == 7.0), "dx: written between rows"
+        if "dw" in g:
+            m, rest = D.get_rows(g["dw"], *wm.shape, ldw, dtype, lead)
+            out["dw"] = m.T if trans else m
+            assert np.all(rest == 7.0), "dw: written between rows"
+        if "dbias" in g:
+            out["dbias"] = D.get(g["dbias"], (classes,))
+        code = np.zeros(1, np.int32)
+        rt.check(L.tl_device_error(code.ctypes.data_as(__import__("ctypes").POINTER(rt.c_int)), 1))
+        assert code[0] == 0, "a bounded wait gave up"
+    return out
+
+
+def within(got, ref, tol, name):
+    got = np.asarray(got, np.float64)
+    assert got.shape == ref.shape, name
+    fin = np.isfinite(ref)
+    np.testing.assert_array_equal(got[~fin], ref[~fin], err_msg=name)
+    tol = np.broadcast_to(tol, ref.shape)
+    bad = fin & ~(np.abs(got - ref) <= tol)
+    if bad.any():
+        i = np.unravel_index(np.argmax(np.where(bad, np.abs(got - ref) / tol, -1)), ref.shape)
+        raise AssertionError(f"{name}: {int(bad.sum())} of {ref.size} off; worst at {i}: got {got[i]!r}, "
+                             f"want {ref[i]!r}, allowed {tol[i]:.3g}")
+
+
+def compare(out, x, w, b, t, dtype, divisor=0.0, up=1.0, start=None):
+    ref = lm_ops.linear_ce(x, w, t, b, divisor, up)
+    e, half = (1.2e-5, BF16_STEP) if dtype == "bf16" else (4e-6, 0.0)
+    ax, aw = np.abs(x), np.abs(w)
+    size = ax @ aw + (0.0 if b is None else np.where(np.isfinite(b), np.abs(b), 0.0))
+    ez = e * size.max(axis=1) + 4e-6          # of a logit, and so of lse
+    lse = np.where(np.isfinite(ref["lse"]), np.abs(ref["lse"]), 0.0)
+    ez = ez + 2.0 ** -23 * lse                # lse is stored in float32
+    if "lse" in out:
+        within(out["lse"], ref["lse"], ez, "lse")
+    if "row_loss" in out:
+        within(out["row_loss"], ref["row_loss"], 2 * ez + 2.0 ** -23 * lse, "row_loss")
+    if "loss" in out:
+        within(out["loss"], np.array([ref["loss"]]), 2 * ez.mean() + 1e-6 * np.abs(lse).mean() + 1e-6, "loss")
+    g = np.abs(ref["g"])
+    ok = (t >= 0) & (t < w.shape[1])
+    div = divisor if divisor > 0 else max(1, int(ok.sum()))
+    p = g.copy()
+    r = np.nonzero(ok)[0]
+    p[r, t[r]] = np.abs(ref["g"][r, t[r]] + up / div)
+    eg = p * (2 * ez + 4e-6)[:, None]                          # g before it is rounded
+    eg8 = eg + half * g
+    start = start or {}
+
+    def grad(name, err, size):
+        want = ref[name] + start.get(name, 0.0)
+        tol = err + e * size + 2e-6 * (np.abs(ref[name]) + np.abs(start.get(name, 0.0)))
+        if dtype == "bf16" and name != "dbias":
+            tol = tol + half * (np.abs(want) + tol)
+        within(out[name], want, tol + 1e-30, name)
+
+    if "dx" in out:
+        grad("dx", eg8 @ aw.T, g @ aw.T)
+    if "dw" in out:
+        grad("dw", ax.T @ eg8, ax.T @ g)
+    if "dbias" in out:
+        grad("dbias", eg.sum(axis=0), g.sum(axis=0))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("trans", [0, 1])
+@pytest.mark.parametrize("rows,classes,width", [
+    (1, 1, 1), (1, 2, 3), (3, 17, 5), (5, 300, 64), (130, 257, 65), (257, 1000, 72), (300, 515, 200),
+    (64, 20011, 100), (520, 3001, 1000), (1, 16384, 256), (1025, 2048, 1288), (2000, 40, 333)])
+def test_sizes(dtype, trans, rows, classes, width):
+    a = inputs(rows, classes, width, dtype)
+    compare(run(*a, dtype, trans), *a, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("pad,lead", [(8, 0), (3, 0), (0, 1), (5, 3)])
+@pytest.mark.parametrize("trans", [0, 1])
+def test_strides_and_offsets(dtype, pad, lead, trans):
+    a = inputs(70, 392, 136, dtype, seed=1)
+    compare(run(*a, dtype, trans, pad=pad, lead=lead), *a, dtype)
+
+
+@pytest.mark.parametrize("idx", ["f32", "i32", "i64"])
+@pytest.mark.parametrize("divisor,up", [(0.0, None), (0.0, 0.25), (512.0, 2.0)])
+def test_targets_and_scales(idx, divisor, up):
+    a = inputs(90, 700, 96, "bf16", seed=2)
+    a[3][:3] = [700, -1, 2 ** 24 + 1]      # out of range; the last also as a float
+    compare(run(*a, "bf16", 1, idx=idx, divisor=divisor, up=up), *a, "bf16", divisor, up or 1.0)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_parts_and_accumulate(dtype):
+    a = inputs(150, 600, 100, dtype, seed=3)
+    x, w, b, t = a
+    for want in (("dx",), ("dw",), ("dbias",), ()):
+        compare(run(*a, dtype, want=want), *a, dtype)
+    out = run(*a, dtype, want=(), fwd=("loss",))
+    compare({"loss": out["loss"]}, *a, dtype)
+    rng = np.random.default_rng(5)
+    for trans in (0, 1):
+        start = {"dx": rounded(rng.standard_normal(x.shape) * 0.01, dtype),
+                 "dw": rounded(rng.standard_normal(w.shape) * 0.01, dtype),
+                 "dbias": rounded(rng.standard_normal(b.shape) * 0.01, "f32")}
+        compare(run(*a, dtype, trans, start=start), *a, dtype, start=start)
+    compare(run(*a, dtype, calls=3), *a, dtype)
+
+
+def test_masked_classes_and_rows_without_target():
+    """bias -inf and the type's lowest value mask classes; a row may lose every
+    class, its target, or all rows their targets."""
+    x, w, b, t = inputs(40, 300, 64, "f32", seed=4, ignored=False)
+    b[100:200] = -np.inf
+    b[250:] = np.finfo(np.float32).min
+    t[:] = np.arange(40)
+    t[3] = 150                              # a masked target: loss +inf
+    with np.errstate(invalid="ignore"):
+        out, ref = run(x, w, b, t, "f32"), lm_ops.linear_ce(x, w, t, b)
+    assert np.isposinf(out["row_loss"][3]) and np.isposinf(out["loss"][0])
+    good = np.arange(40) != 3
+    within(out["row_loss"][good], ref["row_loss"][good], 1e-3, "row_loss")
+    compare({k: out[k] for k in ("lse", "dx", "dw", "dbias")}, x, w, b, t, "f32")
+    everything = np.full(300, -np.inf)
+    out = run(x, w, everything, t, "f32")
+    assert np.isneginf(out["lse"]).all() and np.isposinf(out["loss"][0])
+    assert np.isfinite(out["dx"]).all() and np.isfinite(out["dw"]).all()
+    none = np.full(40, -100)
+    out = run(x, w, None, none, "f32")
+    assert out["loss"][0] == 0 and not out["row_loss"].any() and not out["dx"].any() and not out["dw"].any()
+
+
+def test_nan_rows_stay_their_own():
+    x, w, b, t = inputs(20, 500, 64, "bf16", seed=6, ignored=False)
+    x[7, 3] = np.nan
+    out = run(x, w, b, t, "bf16", divisor=20.0)
+    keep = np.arange(20) != 7
+    ref = lm_ops.linear_ce(x[keep], w, t[keep], b, 20.0)
+    assert np.isnan(out["row_loss"][7]) and np.isnan(out["dx"][7]).all()
+    within(out["row_loss"][keep], ref["row_loss"], 1e-3, "row_loss")
+    assert np.isfinite(out["dx"][keep]).all()
+
+
+def test_pieces_of_the_vocabulary():
+    """A width whose weights' terms make the vocabulary two pieces, in both
+    directions (512 MB of terms: 10752 classes of 8192 floats)."""
+    a = inputs(5, 11800, 8192, "f32", seed=7)
+    compare(run(*a, "f32", 1), *a, "f32")
+
+
+def test_two_runs_agree():
+    a = inputs(700, 2500, 520, "bf16", seed=8)
+    p, q = run(*a, "bf16", 1), run(*a, "bf16", 1)
+    for k in p:
+        np.testing.assert_array_equal(p[k], q[k])
+
+
+def test_no_rows():
+    with Dev() as D:
+        L = rt.lib()
+        nb = L.tl_linear_ce_scratch_bytes(0, 0, 0, 12, 8, 1)
+        s, w, loss = D.zeros(nb), D.new(96), D.new(1)
+        dw, db = D.new(8 * 13, fill=7.0), D.new(12)
+        rt.check(L.tl_linear_ce(0, 0, 0, 12, 8, None, 8, w, 12, None, None, 2, 0.0, loss, None, None, s, nb,
+                                D.stream))
+        rt.check(L.tl_linear_ce_backward(0, 0, 0, 12, 8, None, 8, w, 12, None, None, 2, 0.0, None, None,
+                                         None, 8, dw, 13, db, 0, s, nb, D.stream))
+        assert D.get(loss, (1,))[0] == 0
+        m, rest = D.get_rows(dw, 8, 12, 13, "f32")
+        assert not m.any() and np.all(rest == 7.0) and not D.get(db, (12,)).any()

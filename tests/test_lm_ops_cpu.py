@@ -121,3 +121,32 @@ def test_linear_ce_gradients_against_differences():
                        ("dbias", b, lambda v: lm_ops.linear_ce(x, w, t, v)["loss"])):
         for at in np.ndindex(*a.shape):
             assert abs(ref[name][at] - _difference(f, a, at)) < 1e-8, (name, at)
+
+
+CE = ["dtype", "trans", "rows", "classes", "width", "x", "ldx", "w", "ldw", "bias", "target", "it", "div"]
+CE_GOOD = {"dtype": 1, "trans": 0, "rows": 4, "classes": 100, "width": 16, "x": P, "ldx": 16, "w": 2 * P,
+           "ldw": 100, "bias": None, "target": 3 * P, "it": 2, "div": 0.0, "scratch": 16 * P, "stream": None}
+CE_BAD = [({"dtype": 2}, BAD), ({"trans": 2}, BAD), ({"trans": 1, "ldw": 15}, BAD), ({"rows": -1}, BAD),
+          ({"classes": 0}, BAD), ({"width": 0}, BAD), ({"rows": 1 << 31}, UNSUP), ({"x": None}, BAD),
+          ({"w": None}, BAD), ({"target": None}, BAD), ({"ldx": 15}, BAD), ({"ldw": 99}, BAD),
+          ({"it": 3}, BAD), ({"div": -1.0}, BAD), ({"div": float("nan")}, BAD), ({"scratch": None}, BAD),
+          ({"scratch": 16 * P + 8}, BAD)]
+
+
+def test_linear_ce_refuses():
+    nb = rt.load_library().tl_linear_ce_scratch_bytes(1, 0, 4, 100, 16, 0)
+    good = dict(CE_GOOD, loss=4 * P, row_loss=None, lse=None, nb=nb)
+    refused("tl_linear_ce", good, CE + ["loss", "row_loss", "lse", "scratch", "nb", "stream"], CE_BAD + [
+        ({"loss": None}, BAD), ({"nb": nb - 1}, BAD)])
+
+
+def test_linear_ce_backward_refuses():
+    L = rt.load_library()
+    nb = L.tl_linear_ce_scratch_bytes(1, 0, 4, 100, 16, 1)
+    assert nb >= L.tl_linear_ce_scratch_bytes(1, 0, 4, 100, 16, 0)
+    good = dict(CE_GOOD, lse=5 * P, up=None, dx=6 * P, lddx=16, dw=7 * P, lddw=100, dbias=8 * P, acc=0, nb=nb)
+    order = CE + ["lse", "up", "dx", "lddx", "dw", "lddw", "dbias", "acc", "scratch", "nb", "stream"]
+    refused("tl_linear_ce_backward", good, order, CE_BAD + [
+        ({"lse": None}, BAD), ({"dx": None, "dw": None, "dbias": None}, BAD), ({"lddx": 15}, BAD),
+        ({"lddw": 99}, BAD), ({"acc": 8}, BAD), ({"dx": P}, BAD), ({"dw": 2 * P}, BAD), ({"dw": P}, BAD),
+        ({"dx": 7 * P}, BAD), ({"nb": nb - 1}, BAD)])
