@@ -60,7 +60,7 @@ struct NormArgs {
   float* part;  // [grid][3][cols]: sums of dw_post, dw_pre, dgate (channel)
 };
 
-// Sums of a row's threads (NT threads; one warp, or the whole block).
+// Sums over a row's threads (the whole block).
 template <int NT, int K>
 __device__ __forceinline__ void row_sum(float (&v)[K], float* sh) {
 #pragma unroll
@@ -152,6 +152,77 @@ struct RowIo {
   }
 };
 
+// A thread's elements of the rows it will work on, brought into shared memory
+// ahead of time by asynchronous copies (each thread copies and reads only its
+// own elements, so its own wait is enough): `depth` slots of NA arrays.  Element
+// types or alignments that have no asynchronous copy (2 bytes) load directly.
+template <typename T, int NT, int VEC, int NV, int NA>
+struct Ahead {
+  using Io = RowIo<T, NT, VEC, NV>;
+  static constexpr bool kStaged = VEC * sizeof(T) >= 4;
+  static constexpr int kBytes = VEC * sizeof(T);
+  static constexpr int kArray = NT * NV * kBytes;  // bytes of one array of one row
+  const void* p[NA];
+  int64_t ld[NA];
+  unsigned char* buf;  // [depth][NA][NV][NT] vectors
+  int depth;
+
+  __device__ __forceinline__ void fetch(const Io& io, int64_t r, int64_t rows, int slot) const {
+    if constexpr (kStaged) {
+      if (r < rows) {
+#pragma unroll
+        for (int q = 0; q < NA; ++q) {
+          if (!p[q]) continue;
+          const T* src = static_cast<const T*>(p[q]) + r * ld[q];
+          unsigned char* dst = buf + (slot * NA + q) * kArray + io.t * kBytes;
+#pragma unroll
+          for (int j = 0; j < NV; ++j) {
+            if (io.at(j) >= io.cols) continue;
+            const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst + j * NT * kBytes);
+            if constexpr (kBytes == 16)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src + io.at(j))
+                           : "memory");
+            else
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d), "l"(src + io.at(j))
+                           : "memory");
+          }
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");  // an empty group past the last row
+    }
+  }
+  // the oldest of `depth` outstanding rows has arrived
+  __device__ __forceinline__ void wait() const {
+    if constexpr (kStaged) {
+      if (depth >= 4)
+        asm volatile("cp.async.wait_group 3;" ::: "memory");
+      else if (depth == 3)
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+      else if (depth == 2)
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+      else
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+  }
+  __device__ __forceinline__ void load(const Io& io, int q, int64_t r, int slot,
+                                       float (&v)[Io::E]) const {
+    if constexpr (kStaged) {
+      const unsigned char* src = buf + (slot * NA + q) * kArray + io.t * kBytes;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        float e[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) e[i] = 0.f;
+        if (io.at(j) < io.cols) ld_vec<VEC>(reinterpret_cast<const T*>(src + j * NT * kBytes), e);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[j * VEC + i] = e[i];
+      }
+    } else {
+      io.load(static_cast<const T*>(p[q]) + r * ld[q], v);
+    }
+  }
+};
+
 // v *= gate, for row r
 template <typename T, typename Io, int E>
 __device__ __forceinline__ void apply_gate(const NormArgs& a, const Io& io, int64_t r,
@@ -168,86 +239,96 @@ __device__ __forceinline__ void apply_gate(const NormArgs& a, const Io& io, int6
   }
 }
 
-constexpr int threads_of(int nt) { return nt == 32 ? 256 : nt; }
-
+// One row after another per block (b, b + grid, ...), the next rows of x and u
+// on their way while a row is worked on.
 template <typename T, int NT, int VEC, int NV, bool LAYER>
-__global__ void __launch_bounds__(threads_of(NT)) residual_norm_kernel(NormArgs a) {
+__global__ void __launch_bounds__(NT, NT <= 512 ? 1024 / NT : 1)
+    residual_norm_kernel(NormArgs a, int depth) {
   using Io = RowIo<T, NT, VEC, NV>;
   constexpr int E = Io::E;
+  extern __shared__ __align__(16) unsigned char ahead_buf[];
   __shared__ float sh[32];
-  const Io io{a.cols, (int)(threadIdx.x % NT)};
-  const int64_t r = (int64_t)blockIdx.x * (threads_of(NT) / NT) + threadIdx.x / NT;
-  if (r >= a.rows) return;  // NT > 32: the whole block; NT == 32: a warp, and no block barrier follows
-  const float inv_c = 1.f / (float)a.cols;
+  const Io io{a.cols, (int)threadIdx.x};
+  const Ahead<T, NT, VEC, NV, 2> rows{{a.x, a.u}, {a.ldx, a.ldu}, ahead_buf, depth};
+  const float inv_c = 1.f / (float)a.cols, cols_f = (float)a.cols;
   auto in = [&](int i) { return io.in(i); };
-  float y[E];
-  io.load(static_cast<const T*>(a.x) + r * a.ldx, y);
-  if (a.u) {
-    float v[E];
-    io.load(static_cast<const T*>(a.u) + r * a.ldu, v);
-    normalise<NT, E, LAYER>(v, (float)a.cols, inv_c, a.eps, sh, in);
-    io.scale(static_cast<const T*>(a.w_post), v);
-    apply_gate<T>(a, io, r, v);
+  for (int k = 0; k + 1 < depth; ++k) rows.fetch(io, blockIdx.x + (int64_t)k * gridDim.x, a.rows, k);
+  int slot = 0;
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x, slot = slot + 1 == depth ? 0 : slot + 1) {
+    rows.fetch(io, r + (int64_t)(depth - 1) * gridDim.x, a.rows, slot == 0 ? depth - 1 : slot - 1);
+    rows.wait();
+    float y[E];
+    rows.load(io, 0, r, slot, y);
+    if (a.u) {
+      float v[E];
+      rows.load(io, 1, r, slot, v);
+      normalise<NT, E, LAYER>(v, cols_f, inv_c, a.eps, sh, in);
+      io.scale(static_cast<const T*>(a.w_post), v);
+      apply_gate<T>(a, io, r, v);
 #pragma unroll
-    for (int i = 0; i < E; ++i) y[i] = fmaf(a.alpha, y[i], v[i]);
-  } else {
+      for (int i = 0; i < E; ++i) y[i] = fmaf(a.alpha, y[i], v[i]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < E; ++i) y[i] *= a.alpha;
-  }
-  if (a.y) io.store(static_cast<T*>(a.y) + r * a.ldy, y, false);
-  if (a.n) {
-    normalise<NT, E, LAYER>(y, (float)a.cols, inv_c, a.eps, sh, in);
-    io.scale(static_cast<const T*>(a.w_pre), y);
-    io.store(static_cast<T*>(a.n) + r * a.ldn, y, false);
+      for (int i = 0; i < E; ++i) y[i] *= a.alpha;
+    }
+    if (a.y) io.store(static_cast<T*>(a.y) + r * a.ldy, y, false);
+    if (a.n) {
+      normalise<NT, E, LAYER>(y, cols_f, inv_c, a.eps, sh, in);
+      io.scale(static_cast<const T*>(a.w_pre), y);
+      io.store(static_cast<T*>(a.n) + r * a.ldn, y, false);
+    }
   }
 }
 
 // Block b takes rows b, b + grid, ...: the column sums stay in its threads'
 // registers and leave as one row of partials, which norm_sums_kernel adds in
 // block order (no atomics: results do not depend on the order blocks end).
+// x, u, dy and dn of the next rows are on their way while a row is worked on;
+// dn and dy are read from shared memory where they are used, so that only
+// hat(u), hat(y) and G are held beside the sums.
 template <typename T, int NT, int VEC, int NV, bool LAYER>
-__global__ void __launch_bounds__(NT) residual_norm_bwd_kernel(NormArgs a) {
+__global__ void __launch_bounds__(NT, NT <= 256 ? 512 / NT : 1)
+    residual_norm_bwd_kernel(NormArgs a, int depth) {
   using Io = RowIo<T, NT, VEC, NV>;
   constexpr int E = Io::E;
+  extern __shared__ __align__(16) unsigned char ahead_buf[];
   __shared__ float sh[3 * 32];
   const Io io{a.cols, (int)threadIdx.x};
-  const float inv_c = 1.f / (float)a.cols;
+  const Ahead<T, NT, VEC, NV, 4> rows{{a.u, a.x, a.dn, a.dy}, {a.ldu, a.ldx, a.lddn, a.lddy}, ahead_buf, depth};
+  const float inv_c = 1.f / (float)a.cols, cols_f = (float)a.cols;
   auto in = [&](int i) { return io.in(i); };
   float s_post[E], s_pre[E], s_gate[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) s_post[i] = s_pre[i] = s_gate[i] = 0.f;
   const T* w_post = static_cast<const T*>(a.w_post);
   const T* w_pre = static_cast<const T*>(a.w_pre);
-  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    float y[E], hu[E], G[E];
-    io.load(static_cast<const T*>(a.x) + r * a.ldx, y);
+  for (int k = 0; k + 1 < depth; ++k) rows.fetch(io, blockIdx.x + (int64_t)k * gridDim.x, a.rows, k);
+  int slot = 0;
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x, slot = slot + 1 == depth ? 0 : slot + 1) {
+    rows.fetch(io, r + (int64_t)(depth - 1) * gridDim.x, a.rows, slot == 0 ? depth - 1 : slot - 1);
+    rows.wait();
+    float hu[E], G[E];
     float ru = 0.f;
     if (a.u) {
-      io.load(static_cast<const T*>(a.u) + r * a.ldu, hu);
-    } else {
-#pragma unroll
-      for (int i = 0; i < E; ++i) hu[i] = 0.f;
+      rows.load(io, 0, r, slot, hu);
+      ru = normalise<NT, E, LAYER>(hu, cols_f, inv_c, a.eps, sh, in);
     }
-    if (a.dy) {
-      io.load(static_cast<const T*>(a.dy) + r * a.lddy, G);
-    } else {
-#pragma unroll
-      for (int i = 0; i < E; ++i) G[i] = 0.f;
-    }
-    if (a.u) ru = normalise<NT, E, LAYER>(hu, (float)a.cols, inv_c, a.eps, sh, in);
     if (a.dn) {
-      float d[E];
-      io.load(static_cast<const T*>(a.dn) + r * a.lddn, d);
-      {
-        float v[E];
+      float y[E], d[E];
+      rows.load(io, 1, r, slot, y);
+      if (a.u) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) v[i] = hu[i];
-        io.scale(w_post, v);
-        apply_gate<T>(a, io, r, v);
+        for (int i = 0; i < E; ++i) d[i] = hu[i];
+        io.scale(w_post, d);
+        apply_gate<T>(a, io, r, d);
 #pragma unroll
-        for (int i = 0; i < E; ++i) y[i] = a.u ? fmaf(a.alpha, y[i], v[i]) : a.alpha * y[i];
+        for (int i = 0; i < E; ++i) y[i] = fmaf(a.alpha, y[i], d[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) y[i] *= a.alpha;
       }
-      const float ry = normalise<NT, E, LAYER>(y, (float)a.cols, inv_c, a.eps, sh, in);  // y: hat(y)
+      const float ry = normalise<NT, E, LAYER>(y, cols_f, inv_c, a.eps, sh, in);  // y: hat(y)
+      rows.load(io, 2, r, slot, d);
 #pragma unroll
       for (int i = 0; i < E; ++i) s_pre[i] = fmaf(d[i], y[i], s_pre[i]);
       io.scale(w_pre, d);
@@ -257,10 +338,19 @@ __global__ void __launch_bounds__(NT) residual_norm_bwd_kernel(NormArgs a) {
         c[0] = fmaf(d[i], y[i], c[0]);
         c[1] += d[i];
       }
-      row_sum<NT, 2>(c, sh);
+      row_sum<NT, LAYER ? 2 : 1>(reinterpret_cast<float (&)[LAYER ? 2 : 1]>(c), sh);
       const float m1 = c[0] * inv_c, m0 = LAYER ? c[1] * inv_c : 0.f;
 #pragma unroll
-      for (int i = 0; i < E; ++i) G[i] = fmaf(ry, d[i] - m0 - y[i] * m1, G[i]);
+      for (int i = 0; i < E; ++i) G[i] = ry * (d[i] - m0 - y[i] * m1);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) G[i] = 0.f;
+    }
+    if (a.dy) {
+      float d[E];
+      rows.load(io, 3, r, slot, d);
+#pragma unroll
+      for (int i = 0; i < E; ++i) G[i] += d[i];
     }
     if (a.dx) {
       float v[E];
@@ -269,6 +359,7 @@ __global__ void __launch_bounds__(NT) residual_norm_bwd_kernel(NormArgs a) {
       io.store(static_cast<T*>(a.dx) + r * a.lddx, v, a.accumulate & TL_ACC_DX);
     }
     if (!a.u) continue;
+    float c[3] = {0.f, 0.f, 0.f};
     if (a.dgate) {
       float v[E];
 #pragma unroll
@@ -278,31 +369,29 @@ __global__ void __launch_bounds__(NT) residual_norm_bwd_kernel(NormArgs a) {
 #pragma unroll
         for (int i = 0; i < E; ++i) s_gate[i] += v[i];
       } else if (a.gate_mode == TL_GATE_FULL) {
-        // the gate is read below: a full gate's gradient may not overwrite it
         io.store(static_cast<T*>(a.dgate) + r * a.lddg, v, a.accumulate & TL_ACC_DGATE);
       } else {
-        float s[1] = {0.f};
 #pragma unroll
-        for (int i = 0; i < E; ++i) s[0] += v[i];
-        row_sum<NT, 1>(s, sh);
-        if (threadIdx.x == 0) {
-          T* p = static_cast<T*>(a.dgate) + r;
-          from_f32(p, (a.accumulate & TL_ACC_DGATE) ? to_f32(*p) + s[0] : s[0]);
-        }
+        for (int i = 0; i < E; ++i) c[2] += v[i];
       }
     }
     apply_gate<T>(a, io, r, G);  // P
 #pragma unroll
     for (int i = 0; i < E; ++i) s_post[i] = fmaf(G[i], hu[i], s_post[i]);
-    if (a.du) {
-      io.scale(w_post, G);
-      float c[2] = {0.f, 0.f};
+    const bool token = a.dgate && a.gate_mode == TL_GATE_TOKEN;
+    if (!a.du && !token) continue;
+    io.scale(w_post, G);
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        c[0] = fmaf(G[i], hu[i], c[0]);
-        c[1] += G[i];
-      }
-      row_sum<NT, 2>(c, sh);
+    for (int i = 0; i < E; ++i) {
+      c[0] = fmaf(G[i], hu[i], c[0]);
+      c[1] += G[i];
+    }
+    row_sum<NT, 3>(c, sh);
+    if (token && threadIdx.x == 0) {
+      T* p = static_cast<T*>(a.dgate) + r;
+      from_f32(p, (a.accumulate & TL_ACC_DGATE) ? to_f32(*p) + c[2] : c[2]);
+    }
+    if (a.du) {
       const float m1 = c[0] * inv_c, m0 = LAYER ? c[1] * inv_c : 0.f;
 #pragma unroll
       for (int i = 0; i < E; ++i) G[i] = ru * (G[i] - m0 - hu[i] * m1);
@@ -321,24 +410,26 @@ __global__ void __launch_bounds__(NT) residual_norm_bwd_kernel(NormArgs a) {
 }
 
 // Adds the partials of `blocks` blocks: 32 columns of one of the three sums
-// per block; warp w adds partial rows w, w + 8, ... in turn, then the warps
+// per block; warp w adds partial rows w, w + 32, ... in turn, then the warps
 // in order.
 template <typename T>
-__global__ void __launch_bounds__(256) norm_sums_kernel(NormArgs a, int64_t blocks) {
-  __shared__ float sh[8][33];
+__global__ void __launch_bounds__(1024) norm_sums_kernel(NormArgs a, int64_t blocks) {
+  __shared__ float sh[32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, which = blockIdx.y;
   T* out = static_cast<T*>(which == 0 ? a.dw_post : which == 1 ? a.dw_pre : a.dgate);
   if (!out || (which == 2 && a.gate_mode != TL_GATE_CHANNEL)) return;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
   float s = 0.f;
-  if (c < a.cols)
-    for (int64_t b = w; b < blocks; b += 8) s += a.part[(b * 3 + which) * a.cols + c];
+  if (c < a.cols) {
+#pragma unroll 4
+    for (int64_t b = w; b < blocks; b += 32) s += a.part[(b * 3 + which) * a.cols + c];
+  }
   sh[w][lane] = s;
   __syncthreads();
   if (w == 0 && c < a.cols) {
     float t = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) t += sh[k][lane];
+    for (int k = 0; k < 32; ++k) t += sh[k][lane];
     const int flag = which == 0 ? TL_ACC_DW_POST : which == 1 ? TL_ACC_DW_PRE : TL_ACC_DGATE;
     from_f32(out + c, (a.accumulate & flag) ? to_f32(out[c]) + t : t);
   }
@@ -474,56 +565,68 @@ __global__ void __launch_bounds__(kLong) residual_norm_bwd_long_kernel(NormArgs 
 }
 
 // ------------------------------------------------------------- host side ---
-// Blocks of the backward (and rows of its partials): two per SM.
-int64_t bwd_blocks(int64_t rows) { return std::max<int64_t>(1, std::min<int64_t>(rows, 2LL * sm_count())); }
-
-// The register kernels hold a row in NT threads x VEC * NV elements.
+// The register kernels hold a row in NT threads x 16 elements (or fewer).
 constexpr int64_t kMaxCols = 8192;
+constexpr int64_t kSmem = 216 << 10;  // of an SM, for rows on their way
+
+// Blocks of the backward (and rows of its partials): 512 threads an SM while
+// rows are short, at most eight blocks of them.
+int64_t bwd_blocks(int64_t rows, int64_t cols) {
+  const int64_t per_sm = cols > 4096 ? 1 : cols > 2048 ? 2 : cols > 1024 ? 4 : 8;
+  return std::max<int64_t>(1, std::min<int64_t>(rows, per_sm * sm_count()));
+}
+
+// Rows on their way per block: what fits beside the SM's other blocks, at
+// least the row itself and at most four, and no more than a block has.
+int ahead_depth(int64_t row_bytes, int64_t per_sm, int64_t rows, int64_t grid) {
+  const int64_t fit = kSmem / per_sm / std::max<int64_t>(1, row_bytes);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({fit, 4, (rows + grid - 1) / grid}));
+}
+
+template <typename K>
+int launch_rows(K kern, const NormArgs& a, int64_t grid, int nt, int64_t row_bytes, int64_t per_sm,
+                cudaStream_t st) {
+  const int depth = ahead_depth(row_bytes, per_sm, a.rows, grid);
+  const size_t smem = (size_t)(depth * row_bytes);
+  TL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  kern<<<(unsigned)grid, nt, smem, st>>>(a, depth);
+  return after_launch();
+}
 
 template <typename T, int VEC, int NT, int NV>
 int launch_fwd(const NormArgs& a, int kind, cudaStream_t st) {
-  constexpr int per = threads_of(NT) / NT;
-  const unsigned grid = (unsigned)((a.rows + per - 1) / per);
-  if (kind == TL_NORM_LAYER)
-    residual_norm_kernel<T, NT, VEC, NV, true><<<grid, threads_of(NT), 0, st>>>(a);
-  else
-    residual_norm_kernel<T, NT, VEC, NV, false><<<grid, threads_of(NT), 0, st>>>(a);
-  return after_launch();
+  constexpr int64_t row = 2 * Ahead<T, NT, VEC, NV, 2>::kArray, per_sm = NT <= 512 ? 1024 / NT : 1;
+  const int64_t grid = std::min<int64_t>(a.rows, per_sm * sm_count());
+  return kind == TL_NORM_LAYER
+             ? launch_rows(residual_norm_kernel<T, NT, VEC, NV, true>, a, grid, NT, row, per_sm, st)
+             : launch_rows(residual_norm_kernel<T, NT, VEC, NV, false>, a, grid, NT, row, per_sm, st);
 }
 
 template <typename T, int VEC>
 int forward(const NormArgs& a, int kind, cudaStream_t st) {
-  constexpr int E = VEC == 1 ? 4 : VEC;  // elements of a thread with the fewest
-  constexpr int N1 = E / VEC;
   const int64_t c = a.cols;
-  if (c <= 32 * E) return launch_fwd<T, VEC, 32, N1>(a, kind, st);
-  if (c <= 64 * E) return launch_fwd<T, VEC, 64, N1>(a, kind, st);
-  if (c <= 128 * E) return launch_fwd<T, VEC, 128, N1>(a, kind, st);
-  if (c <= 256 * E) return launch_fwd<T, VEC, 256, N1>(a, kind, st);
-  if (c <= 512 * E) return launch_fwd<T, VEC, 512, N1>(a, kind, st);
-  return launch_fwd<T, VEC, 512, kMaxCols / 512 / VEC>(a, kind, st);
+  if (c <= 1024) return launch_fwd<T, VEC, 64, 16 / VEC>(a, kind, st);
+  if (c <= 2048) return launch_fwd<T, VEC, 128, 16 / VEC>(a, kind, st);
+  if (c <= 4096) return launch_fwd<T, VEC, 256, 16 / VEC>(a, kind, st);
+  return launch_fwd<T, VEC, 512, 16 / VEC>(a, kind, st);
 }
 
 template <typename T, int VEC, int NT, int NV>
 int launch_bwd(const NormArgs& a, int kind, cudaStream_t st) {
-  const unsigned grid = (unsigned)bwd_blocks(a.rows);
-  if (kind == TL_NORM_LAYER)
-    residual_norm_bwd_kernel<T, NT, VEC, NV, true><<<grid, NT, 0, st>>>(a);
-  else
-    residual_norm_bwd_kernel<T, NT, VEC, NV, false><<<grid, NT, 0, st>>>(a);
-  return after_launch();
+  constexpr int64_t row = 4 * Ahead<T, NT, VEC, NV, 4>::kArray, per_sm = NT <= 256 ? 512 / NT : 1;
+  const int64_t grid = bwd_blocks(a.rows, a.cols);
+  return kind == TL_NORM_LAYER
+             ? launch_rows(residual_norm_bwd_kernel<T, NT, VEC, NV, true>, a, grid, NT, row, per_sm, st)
+             : launch_rows(residual_norm_bwd_kernel<T, NT, VEC, NV, false>, a, grid, NT, row, per_sm, st);
 }
 
 template <typename T, int VEC>
 int backward(const NormArgs& a, int kind, cudaStream_t st) {
-  constexpr int E = VEC == 1 ? 4 : VEC;
-  constexpr int N1 = E / VEC;
   const int64_t c = a.cols;
-  if (c <= 64 * E) return launch_bwd<T, VEC, 64, N1>(a, kind, st);
-  if (c <= 128 * E) return launch_bwd<T, VEC, 128, N1>(a, kind, st);
-  if (c <= 256 * E) return launch_bwd<T, VEC, 256, N1>(a, kind, st);
-  if (c <= 512 * E) return launch_bwd<T, VEC, 512, N1>(a, kind, st);
-  return launch_bwd<T, VEC, 512, kMaxCols / 512 / VEC>(a, kind, st);
+  if (c <= 1024) return launch_bwd<T, VEC, 64, 16 / VEC>(a, kind, st);
+  if (c <= 2048) return launch_bwd<T, VEC, 128, 16 / VEC>(a, kind, st);
+  if (c <= 4096) return launch_bwd<T, VEC, 256, 16 / VEC>(a, kind, st);
+  return launch_bwd<T, VEC, 512, 16 / VEC>(a, kind, st);
 }
 
 // Whether rows of p (leading dimension ld) take 128-bit accesses.
@@ -561,7 +664,7 @@ int run_backward(const NormArgs& a, int kind, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   if (a.rows > 0) {
     if (a.cols > kMaxCols) {
-      const unsigned grid = (unsigned)bwd_blocks(a.rows);
+      const unsigned grid = (unsigned)bwd_blocks(a.rows, a.cols);
       if (kind == TL_NORM_LAYER)
         residual_norm_bwd_long_kernel<T, true><<<grid, kLong, 0, st>>>(a);
       else
@@ -572,8 +675,8 @@ int run_backward(const NormArgs& a, int kind, cudaStream_t st) {
     }
   }
   if (a.dw_post || a.dw_pre || (a.dgate && a.gate_mode == TL_GATE_CHANNEL)) {
-    norm_sums_kernel<T><<<dim3((unsigned)((a.cols + 31) / 32), 3), 256, 0, st>>>(
-        a, a.rows > 0 ? bwd_blocks(a.rows) : 0);
+    norm_sums_kernel<T><<<dim3((unsigned)((a.cols + 31) / 32), 3), 1024, 0, st>>>(
+        a, a.rows > 0 ? bwd_blocks(a.rows, a.cols) : 0);
     TL_TRY(after_launch());
   }
   return TL_OK;
@@ -621,7 +724,7 @@ int tl_residual_norm(int dtype, int kind, int64_t rows, int64_t cols, const void
 
 size_t tl_residual_norm_scratch_bytes(int64_t rows, int64_t cols) {
   if (rows < 0 || cols <= 0) return 0;
-  return (size_t)tl::bwd_blocks(rows) * 3 * (size_t)cols * sizeof(float);
+  return (size_t)tl::bwd_blocks(rows, cols) * 3 * (size_t)cols * sizeof(float);
 }
 
 int tl_residual_norm_backward(int dtype, int kind, int64_t rows, int64_t cols, const void* x,
