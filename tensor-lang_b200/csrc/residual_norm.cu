@@ -57,105 +57,111 @@ struct NormArgs {
   void* dw_post;
   void* dw_pre;
   int accumulate;
-  float* part;  // [grid][3][cols]: sums of dw_post, dw_pre, dgate (channel)
+  float* part;  // [grid][2][cols]: sums over rows of G gate hat(u) (a gate per channel left out) and dn hat(y)
 };
+
+// Two float32 operations in one instruction (sm_100): the row kernels hold
+// their elements in pairs, since single operations, at 92 instructions per
+// element, bounded the backward by instruction issue and not by memory.
+__device__ __forceinline__ float2 pair(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float hsum(float2 a) { return a.x + a.y; }
 
 // Sums over a row's threads (the whole block).
 template <int NT, int K>
 __device__ __forceinline__ void row_sum(float (&v)[K], float* sh) {
+  constexpr int NW = NT / 32;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
 #pragma unroll
   for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
-  if constexpr (NT > 32) {
-    constexpr int NW = NT / 32;
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    __syncthreads();  // the previous sum's readers are done
-    if (lane == 0) {
+  __syncthreads();  // the previous sum's readers are done
+  if (lane == 0) {
 #pragma unroll
-      for (int k = 0; k < K; ++k) sh[k * NW + w] = v[k];
-    }
-    __syncthreads();
+    for (int k = 0; k < K; ++k) sh[k * NW + w] = v[k];
+  }
+  __syncthreads();
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const float t = lane < NW ? sh[k * NW + lane] : 0.f;
-      v[k] = warp_sum(t);
-    }
+  for (int k = 0; k < K; ++k) {
+    float t = lane < NW ? sh[k * NW + lane] : 0.f;
+#pragma unroll
+    for (int o = NW < 32 ? NW / 2 : 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    v[k] = __shfl_sync(0xffffffffu, t, 0);
   }
 }
 
-// v becomes hat(v) for the elements a thread holds; returns 1 / scale.  Lanes
-// past the row hold zeros and must stay out of the centred sum (`in`).
-template <int NT, int E, bool LAYER, typename In>
-__device__ __forceinline__ float normalise(float (&v)[E], float cols, float inv_c, float eps, float* sh,
-                                           In in) {
-  float s[1];
-  if constexpr (LAYER) {
-    s[0] = 0.f;
-#pragma unroll
-    for (int i = 0; i < E; ++i) s[0] += v[i];
-    row_sum<NT, 1>(s, sh);
-    const float mean = s[0] / cols;  // divided: the mean of a constant row is that constant
-#pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = in(i) ? v[i] - mean : 0.f;
-  }
-  s[0] = 0.f;
-#pragma unroll
-  for (int i = 0; i < E; ++i) s[0] = fmaf(v[i], v[i], s[0]);
-  row_sum<NT, 1>(s, sh);
-  const float r = 1.f / sqrtf(s[0] * inv_c + eps);
-#pragma unroll
-  for (int i = 0; i < E; ++i) v[i] *= r;
-  return r;
-}
-
-// A thread's elements of a row: vector j of VEC elements at (j * NT + t) * VEC.
+// A thread's elements of a row, in pairs: vector j of VEC elements at
+// (j * NT + t) * VEC.
 template <typename T, int NT, int VEC, int NV>
 struct RowIo {
-  static constexpr int E = VEC * NV;
+  static constexpr int E = VEC * NV, H = E / 2;
   int64_t cols;
   int t;
   __device__ __forceinline__ int64_t at(int j) const { return ((int64_t)j * NT + t) * VEC; }
   __device__ __forceinline__ bool in(int i) const { return at(i / VEC) < cols; }
-  __device__ __forceinline__ void load(const T* p, float (&v)[E]) const {
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      float q[VEC];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) q[i] = 0.f;
-      if (at(j) < cols) ld_vec<VEC>(p + at(j), q);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[j * VEC + i] = q[i];
-    }
-  }
-  __device__ __forceinline__ void store(T* p, const float (&v)[E], bool add) const {
+  __device__ __forceinline__ bool full() const { return at(NV - 1) < cols; }
+  __device__ __forceinline__ void store(T* p, const float2 (&v)[H], bool add) const {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       if (at(j) >= cols) continue;
       float q[VEC];
-      if (add) {
-        ld_vec<VEC>(p + at(j), q);
-      } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) q[i] = 0.f;
+      for (int i = 0; i < VEC; ++i) {
+        const int e = j * VEC + i;
+        q[i] = e & 1 ? v[e / 2].y : v[e / 2].x;
       }
+      if (add) {
+        float o[VEC];
+        ld_vec<VEC>(p + at(j), o);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) q[i] += v[j * VEC + i];
+        for (int i = 0; i < VEC; ++i) q[i] += o[i];
+      }
       st_vec<VEC>(p + at(j), q);
     }
   }
-  // v *= p (a weight or gate; null is 1)
-  __device__ __forceinline__ void scale(const T* p, float (&v)[E]) const {
-    if (!p) return;
-    float q[E];
-    load(p, q);
-#pragma unroll
-    for (int i = 0; i < E; ++i) v[i] *= q[i];
-  }
 };
+
+// v becomes hat(v) for the elements a thread holds; returns 1 / scale.
+// Elements past the row are zero and stay out of the centred sum.
+template <bool LAYER, typename T, int NT, int VEC, int NV, int H>
+__device__ __forceinline__ float normalise(const RowIo<T, NT, VEC, NV>& io, float2 (&v)[H], float eps,
+                                           float* sh) {
+  const float cols = (float)io.cols;
+  float s[1];
+  float2 q = pair(0.f);
+  if constexpr (LAYER) {
+#pragma unroll
+    for (int i = 0; i < H; ++i) q = add2(q, v[i]);
+    s[0] = hsum(q);
+    row_sum<NT, 1>(s, sh);
+    const float2 mean = pair(-(s[0] / cols));  // divided: the mean of a constant row is that constant
+#pragma unroll
+    for (int i = 0; i < H; ++i) v[i] = add2(v[i], mean);
+    if (!io.full()) {
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        if (!io.in(2 * i)) v[i].x = 0.f;
+        if (!io.in(2 * i + 1)) v[i].y = 0.f;
+      }
+    }
+    q = pair(0.f);
+  }
+#pragma unroll
+  for (int i = 0; i < H; ++i) q = fma2(v[i], v[i], q);
+  s[0] = hsum(q);
+  row_sum<NT, 1>(s, sh);
+  const float r = 1.f / sqrtf(s[0] / cols + eps);
+#pragma unroll
+  for (int i = 0; i < H; ++i) v[i] = mul2(v[i], pair(r));
+  return r;
+}
 
 // A thread's elements of the rows it will work on, brought into shared memory
 // ahead of time by asynchronous copies (each thread copies and reads only its
-// own elements, so its own wait is enough): `depth` slots of NA arrays.  Element
-// types or alignments that have no asynchronous copy (2 bytes) load directly.
+// own elements, so its own wait is enough): `depth` slots of `na` arrays.
+// Element types or alignments that have no asynchronous copy (2 bytes) load
+// directly.
 template <typename T, int NT, int VEC, int NV, int NA>
 struct Ahead {
   using Io = RowIo<T, NT, VEC, NV>;
@@ -164,8 +170,8 @@ struct Ahead {
   static constexpr int kArray = NT * NV * kBytes;  // bytes of one array of one row
   const void* p[NA];
   int64_t ld[NA];
-  unsigned char* buf;  // [depth][NA][NV][NT] vectors
-  int depth;
+  unsigned char* buf;  // [depth][na][NV][NT] vectors
+  int depth, na;
 
   __device__ __forceinline__ void fetch(const Io& io, int64_t r, int64_t rows, int slot) const {
     if constexpr (kStaged) {
@@ -174,7 +180,7 @@ struct Ahead {
         for (int q = 0; q < NA; ++q) {
           if (!p[q]) continue;
           const T* src = static_cast<const T*>(p[q]) + r * ld[q];
-          unsigned char* dst = buf + (slot * NA + q) * kArray + io.t * kBytes;
+          unsigned char* dst = buf + (slot * na + q) * kArray + io.t * kBytes;
 #pragma unroll
           for (int j = 0; j < NV; ++j) {
             if (io.at(j) >= io.cols) continue;
@@ -205,76 +211,108 @@ struct Ahead {
     }
   }
   __device__ __forceinline__ void load(const Io& io, int q, int64_t r, int slot,
-                                       float (&v)[Io::E]) const {
-    if constexpr (kStaged) {
-      const unsigned char* src = buf + (slot * NA + q) * kArray + io.t * kBytes;
+                                       float2 (&v)[Io::H]) const {
+    const T* src = kStaged ? reinterpret_cast<const T*>(buf + (slot * na + q) * kArray + io.t * kBytes)
+                           : static_cast<const T*>(p[q]) + r * ld[q];
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        float e[VEC];
+    for (int j = 0; j < NV; ++j) {
+      float e[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) e[i] = 0.f;
-        if (io.at(j) < io.cols) ld_vec<VEC>(reinterpret_cast<const T*>(src + j * NT * kBytes), e);
+      for (int i = 0; i < VEC; ++i) e[i] = 0.f;
+      if (io.at(j) < io.cols) ld_vec<VEC>(kStaged ? src + j * NT * VEC : src + io.at(j), e);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[j * VEC + i] = e[i];
+      for (int i = 0; i < VEC; ++i) {
+        const int k = j * VEC + i;
+        (k & 1 ? v[k / 2].y : v[k / 2].x) = e[i];
       }
-    } else {
-      io.load(static_cast<const T*>(p[q]) + r * ld[q], v);
     }
   }
 };
 
-// v *= gate, for row r
-template <typename T, typename Io, int E>
-__device__ __forceinline__ void apply_gate(const NormArgs& a, const Io& io, int64_t r,
-                                           float (&v)[E]) {
-  const T* g = static_cast<const T*>(a.gate);
-  if (a.gate_mode == TL_GATE_CHANNEL) {
-    io.scale(g, v);
-  } else if (a.gate_mode == TL_GATE_FULL) {
-    io.scale(g + r * a.ldg, v);
-  } else if (a.gate_mode == TL_GATE_TOKEN) {
-    const float q = to_f32(g[r]);
+// A thread's elements of a weight vector, in shared memory as float32; only
+// that thread writes and reads them.
+template <typename T, int NT, int VEC, int NV>
+struct RowWeights {
+  using Io = RowIo<T, NT, VEC, NV>;
+  static constexpr int H = Io::H;
+  static constexpr int kBytes = NT * Io::E * 4;
+  float4* p;  // [H / 2][NT]
+  // w * g (either may be null: 1)
+  __device__ __forceinline__ void fill(const Io& io, const T* w, const T* g) const {
 #pragma unroll
-    for (int i = 0; i < E; ++i) v[i] *= q;
+    for (int i = 0; i < H / 2; ++i) {
+      float e[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int64_t c = io.at((4 * i + k) / VEC) + (4 * i + k) % VEC;
+        e[k] = c < io.cols ? (w ? to_f32(w[c]) : 1.f) * (g ? to_f32(g[c]) : 1.f) : 0.f;
+      }
+      p[i * NT + io.t] = make_float4(e[0], e[1], e[2], e[3]);
+    }
   }
-}
+  __device__ __forceinline__ void load(const Io& io, float2 (&v)[H]) const {
+#pragma unroll
+    for (int i = 0; i < H / 2; ++i) {
+      const float4 q = p[i * NT + io.t];
+      v[2 * i] = make_float2(q.x, q.y);
+      v[2 * i + 1] = make_float2(q.z, q.w);
+    }
+  }
+};
 
 // One row after another per block (b, b + grid, ...), the next rows of x and u
 // on their way while a row is worked on.
 template <typename T, int NT, int VEC, int NV, bool LAYER>
-__global__ void __launch_bounds__(NT, NT <= 512 ? 1024 / NT : 1)
-    residual_norm_kernel(NormArgs a, int depth) {
+__global__ void __launch_bounds__(NT, 1024 / NT) residual_norm_kernel(NormArgs a, int depth) {
   using Io = RowIo<T, NT, VEC, NV>;
-  constexpr int E = Io::E;
-  extern __shared__ __align__(16) unsigned char ahead_buf[];
+  using W = RowWeights<T, NT, VEC, NV>;
+  constexpr int H = Io::H;
+  extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ float sh[32];
   const Io io{a.cols, (int)threadIdx.x};
-  const Ahead<T, NT, VEC, NV, 2> rows{{a.x, a.u}, {a.ldx, a.ldu}, ahead_buf, depth};
-  const float inv_c = 1.f / (float)a.cols, cols_f = (float)a.cols;
-  auto in = [&](int i) { return io.in(i); };
+  const bool full_gate = a.gate_mode == TL_GATE_FULL;
+  const Ahead<T, NT, VEC, NV, 3> rows{{a.x, a.u, full_gate ? a.gate : nullptr}, {a.ldx, a.ldu, a.ldg},
+                                      dyn + 2 * W::kBytes, depth, full_gate ? 3 : 2};
   for (int k = 0; k + 1 < depth; ++k) rows.fetch(io, blockIdx.x + (int64_t)k * gridDim.x, a.rows, k);
+  const W w_post{reinterpret_cast<float4*>(dyn)}, w_pre{reinterpret_cast<float4*>(dyn + W::kBytes)};
   int slot = 0;
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x, slot = slot + 1 == depth ? 0 : slot + 1) {
     rows.fetch(io, r + (int64_t)(depth - 1) * gridDim.x, a.rows, slot == 0 ? depth - 1 : slot - 1);
+    if (r == blockIdx.x) {  // while the first row is on its way
+      w_post.fill(io, static_cast<const T*>(a.w_post),
+                  a.gate_mode == TL_GATE_CHANNEL ? static_cast<const T*>(a.gate) : nullptr);
+      w_pre.fill(io, static_cast<const T*>(a.w_pre), nullptr);
+    }
     rows.wait();
-    float y[E];
+    float2 y[H];
     rows.load(io, 0, r, slot, y);
+#pragma unroll
+    for (int i = 0; i < H; ++i) y[i] = mul2(y[i], pair(a.alpha));
     if (a.u) {
-      float v[E];
+      float2 v[H], w[H];
       rows.load(io, 1, r, slot, v);
-      normalise<NT, E, LAYER>(v, cols_f, inv_c, a.eps, sh, in);
-      io.scale(static_cast<const T*>(a.w_post), v);
-      apply_gate<T>(a, io, r, v);
+      normalise<LAYER>(io, v, a.eps, sh);
+      w_post.load(io, w);
+      if (full_gate) {
+        float2 g[H];
+        rows.load(io, 2, r, slot, g);
 #pragma unroll
-      for (int i = 0; i < E; ++i) y[i] = fmaf(a.alpha, y[i], v[i]);
-    } else {
+        for (int i = 0; i < H; ++i) w[i] = mul2(w[i], g[i]);
+      } else if (a.gate_mode == TL_GATE_TOKEN) {
+        const float g = to_f32(static_cast<const T*>(a.gate)[r]);
 #pragma unroll
-      for (int i = 0; i < E; ++i) y[i] *= a.alpha;
+        for (int i = 0; i < H; ++i) w[i] = mul2(w[i], pair(g));
+      }
+#pragma unroll
+      for (int i = 0; i < H; ++i) y[i] = fma2(v[i], w[i], y[i]);
     }
     if (a.y) io.store(static_cast<T*>(a.y) + r * a.ldy, y, false);
     if (a.n) {
-      normalise<NT, E, LAYER>(y, cols_f, inv_c, a.eps, sh, in);
-      io.scale(static_cast<const T*>(a.w_pre), y);
+      normalise<LAYER>(io, y, a.eps, sh);
+      float2 w[H];
+      w_pre.load(io, w);
+#pragma unroll
+      for (int i = 0; i < H; ++i) y[i] = mul2(y[i], w[i]);
       io.store(static_cast<T*>(a.n) + r * a.ldn, y, false);
     }
   }
@@ -285,144 +323,201 @@ __global__ void __launch_bounds__(NT, NT <= 512 ? 1024 / NT : 1)
 // block order (no atomics: results do not depend on the order blocks end).
 // x, u, dy and dn of the next rows are on their way while a row is worked on;
 // dn and dy are read from shared memory where they are used, so that only
-// hat(u), hat(y) and G are held beside the sums.
+// hat(u), hat(y) and G are held beside the sums.  A gate per channel needs no
+// sum of its own: with S = sum_rows G hat(u), dw_post = gate S and
+// dgate = w_post S.
 template <typename T, int NT, int VEC, int NV, bool LAYER>
 __global__ void __launch_bounds__(NT, NT <= 256 ? 512 / NT : 1)
     residual_norm_bwd_kernel(NormArgs a, int depth) {
   using Io = RowIo<T, NT, VEC, NV>;
-  constexpr int E = Io::E;
-  extern __shared__ __align__(16) unsigned char ahead_buf[];
+  using W = RowWeights<T, NT, VEC, NV>;
+  constexpr int H = Io::H;
+  extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ float sh[3 * 32];
   const Io io{a.cols, (int)threadIdx.x};
-  const Ahead<T, NT, VEC, NV, 4> rows{{a.u, a.x, a.dn, a.dy}, {a.ldu, a.ldx, a.lddn, a.lddy}, ahead_buf, depth};
-  const float inv_c = 1.f / (float)a.cols, cols_f = (float)a.cols;
-  auto in = [&](int i) { return io.in(i); };
-  float s_post[E], s_pre[E], s_gate[E];
-#pragma unroll
-  for (int i = 0; i < E; ++i) s_post[i] = s_pre[i] = s_gate[i] = 0.f;
-  const T* w_post = static_cast<const T*>(a.w_post);
-  const T* w_pre = static_cast<const T*>(a.w_pre);
+  const bool full_gate = a.gate_mode == TL_GATE_FULL, token_gate = a.gate_mode == TL_GATE_TOKEN;
+  const Ahead<T, NT, VEC, NV, 5> rows{{a.u, a.x, a.dn, a.dy, full_gate ? a.gate : nullptr},
+                                      {a.ldu, a.ldx, a.lddn, a.lddy, a.ldg},
+                                      dyn + 2 * W::kBytes, depth, full_gate ? 5 : 4};
+  const float inv_c = 1.f / (float)a.cols;
   for (int k = 0; k + 1 < depth; ++k) rows.fetch(io, blockIdx.x + (int64_t)k * gridDim.x, a.rows, k);
+  const W w_post{reinterpret_cast<float4*>(dyn)}, w_pre{reinterpret_cast<float4*>(dyn + W::kBytes)};
+  float2 s_post[H], s_pre[H];
+#pragma unroll
+  for (int i = 0; i < H; ++i) s_post[i] = s_pre[i] = pair(0.f);
   int slot = 0;
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x, slot = slot + 1 == depth ? 0 : slot + 1) {
     rows.fetch(io, r + (int64_t)(depth - 1) * gridDim.x, a.rows, slot == 0 ? depth - 1 : slot - 1);
+    if (r == blockIdx.x) {  // while the first row is on its way
+      w_post.fill(io, static_cast<const T*>(a.w_post),
+                  a.gate_mode == TL_GATE_CHANNEL ? static_cast<const T*>(a.gate) : nullptr);
+      w_pre.fill(io, static_cast<const T*>(a.w_pre), nullptr);
+    }
     rows.wait();
-    float hu[E], G[E];
+    const float gate_r = token_gate ? to_f32(static_cast<const T*>(a.gate)[r]) : 1.f;
+    // what hat(u) is multiplied by on its way to y: w_post * gate
+    auto branch_weight = [&](float2(&w)[H]) {
+      w_post.load(io, w);
+      if (full_gate) {
+        float2 g[H];
+        rows.load(io, 4, r, slot, g);
+#pragma unroll
+        for (int i = 0; i < H; ++i) w[i] = mul2(w[i], g[i]);
+      } else if (token_gate) {
+#pragma unroll
+        for (int i = 0; i < H; ++i) w[i] = mul2(w[i], pair(gate_r));
+      }
+    };
+    float2 hu[H], G[H];
     float ru = 0.f;
     if (a.u) {
       rows.load(io, 0, r, slot, hu);
-      ru = normalise<NT, E, LAYER>(hu, cols_f, inv_c, a.eps, sh, in);
+      ru = normalise<LAYER>(io, hu, a.eps, sh);
     }
     if (a.dn) {
-      float y[E], d[E];
+      float2 y[H], d[H];
       rows.load(io, 1, r, slot, y);
+#pragma unroll
+      for (int i = 0; i < H; ++i) y[i] = mul2(y[i], pair(a.alpha));
       if (a.u) {
+        branch_weight(d);
 #pragma unroll
-        for (int i = 0; i < E; ++i) d[i] = hu[i];
-        io.scale(w_post, d);
-        apply_gate<T>(a, io, r, d);
+        for (int i = 0; i < H; ++i) y[i] = fma2(hu[i], d[i], y[i]);
+      }
+      const float ry = normalise<LAYER>(io, y, a.eps, sh);  // y: hat(y)
+      rows.load(io, 2, r, slot, d);
+      float2 c0 = pair(0.f), c1 = pair(0.f);
+      w_pre.load(io, G);
 #pragma unroll
-        for (int i = 0; i < E; ++i) y[i] = fmaf(a.alpha, y[i], d[i]);
+      for (int i = 0; i < H; ++i) {
+        s_pre[i] = fma2(d[i], y[i], s_pre[i]);
+        d[i] = mul2(d[i], G[i]);
+        c0 = fma2(d[i], y[i], c0);
+        if (LAYER) c1 = add2(c1, d[i]);
+      }
+      float m[LAYER ? 2 : 1];
+      m[0] = hsum(c0);
+      if constexpr (LAYER) m[1] = hsum(c1);
+      row_sum<NT, LAYER ? 2 : 1>(m, sh);
+      const float2 m1 = pair(-m[0] * inv_c);
+#pragma unroll
+      for (int i = 0; i < H; ++i) G[i] = fma2(y[i], m1, d[i]);
+      if constexpr (LAYER) {
+        const float2 m0 = pair(-m[1] * inv_c);
+#pragma unroll
+        for (int i = 0; i < H; ++i) G[i] = add2(G[i], m0);
+      }
+      if (a.dy) {
+        rows.load(io, 3, r, slot, d);
+#pragma unroll
+        for (int i = 0; i < H; ++i) G[i] = fma2(G[i], pair(ry), d[i]);
       } else {
 #pragma unroll
-        for (int i = 0; i < E; ++i) y[i] *= a.alpha;
+        for (int i = 0; i < H; ++i) G[i] = mul2(G[i], pair(ry));
       }
-      const float ry = normalise<NT, E, LAYER>(y, cols_f, inv_c, a.eps, sh, in);  // y: hat(y)
-      rows.load(io, 2, r, slot, d);
-#pragma unroll
-      for (int i = 0; i < E; ++i) s_pre[i] = fmaf(d[i], y[i], s_pre[i]);
-      io.scale(w_pre, d);
-      float c[2] = {0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        c[0] = fmaf(d[i], y[i], c[0]);
-        c[1] += d[i];
-      }
-      row_sum<NT, LAYER ? 2 : 1>(reinterpret_cast<float (&)[LAYER ? 2 : 1]>(c), sh);
-      const float m1 = c[0] * inv_c, m0 = LAYER ? c[1] * inv_c : 0.f;
-#pragma unroll
-      for (int i = 0; i < E; ++i) G[i] = ry * (d[i] - m0 - y[i] * m1);
+    } else if (a.dy) {
+      rows.load(io, 3, r, slot, G);
     } else {
 #pragma unroll
-      for (int i = 0; i < E; ++i) G[i] = 0.f;
-    }
-    if (a.dy) {
-      float d[E];
-      rows.load(io, 3, r, slot, d);
-#pragma unroll
-      for (int i = 0; i < E; ++i) G[i] += d[i];
+      for (int i = 0; i < H; ++i) G[i] = pair(0.f);
     }
     if (a.dx) {
-      float v[E];
+      float2 v[H];
 #pragma unroll
-      for (int i = 0; i < E; ++i) v[i] = a.alpha * G[i];
+      for (int i = 0; i < H; ++i) v[i] = mul2(G[i], pair(a.alpha));
       io.store(static_cast<T*>(a.dx) + r * a.lddx, v, a.accumulate & TL_ACC_DX);
     }
     if (!a.u) continue;
     float c[3] = {0.f, 0.f, 0.f};
-    if (a.dgate) {
-      float v[E];
+    if (full_gate || token_gate) {
+      float2 v[H], w[H], t = pair(0.f);
+      w_post.load(io, w);
 #pragma unroll
-      for (int i = 0; i < E; ++i) v[i] = G[i] * hu[i];
-      io.scale(w_post, v);
-      if (a.gate_mode == TL_GATE_CHANNEL) {
+      for (int i = 0; i < H; ++i) {
+        v[i] = mul2(G[i], hu[i]);
+        w[i] = mul2(v[i], w[i]);
+        t = add2(t, w[i]);
+      }
+      c[2] = hsum(t);
+      if (full_gate && a.dgate)
+        io.store(static_cast<T*>(a.dgate) + r * a.lddg, w, a.accumulate & TL_ACC_DGATE);
+      if (full_gate) {
+        rows.load(io, 4, r, slot, w);
 #pragma unroll
-        for (int i = 0; i < E; ++i) s_gate[i] += v[i];
-      } else if (a.gate_mode == TL_GATE_FULL) {
-        io.store(static_cast<T*>(a.dgate) + r * a.lddg, v, a.accumulate & TL_ACC_DGATE);
+        for (int i = 0; i < H; ++i) s_post[i] = fma2(v[i], w[i], s_post[i]);
       } else {
 #pragma unroll
-        for (int i = 0; i < E; ++i) c[2] += v[i];
+        for (int i = 0; i < H; ++i) s_post[i] = fma2(v[i], pair(gate_r), s_post[i]);
       }
-    }
-    apply_gate<T>(a, io, r, G);  // P
+    } else {
 #pragma unroll
-    for (int i = 0; i < E; ++i) s_post[i] = fmaf(G[i], hu[i], s_post[i]);
-    const bool token = a.dgate && a.gate_mode == TL_GATE_TOKEN;
+      for (int i = 0; i < H; ++i) s_post[i] = fma2(G[i], hu[i], s_post[i]);
+    }
+    const bool token = token_gate && a.dgate;
     if (!a.du && !token) continue;
-    io.scale(w_post, G);
+    {
+      float2 w[H], c0 = pair(0.f), c1 = pair(0.f);
+      branch_weight(w);
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      c[0] = fmaf(G[i], hu[i], c[0]);
-      c[1] += G[i];
+      for (int i = 0; i < H; ++i) {
+        G[i] = mul2(G[i], w[i]);
+        c0 = fma2(G[i], hu[i], c0);
+        if (LAYER) c1 = add2(c1, G[i]);
+      }
+      c[0] = hsum(c0);
+      c[1] = hsum(c1);
     }
-    row_sum<NT, 3>(c, sh);
-    if (token && threadIdx.x == 0) {
-      T* p = static_cast<T*>(a.dgate) + r;
-      from_f32(p, (a.accumulate & TL_ACC_DGATE) ? to_f32(*p) + c[2] : c[2]);
+    if (token) {
+      row_sum<NT, 3>(c, sh);
+      if (threadIdx.x == 0) {
+        T* p = static_cast<T*>(a.dgate) + r;
+        from_f32(p, (a.accumulate & TL_ACC_DGATE) ? to_f32(*p) + c[2] : c[2]);
+      }
+    } else {
+      float m[LAYER ? 2 : 1];
+      m[0] = c[0];
+      if constexpr (LAYER) m[1] = c[1];
+      row_sum<NT, LAYER ? 2 : 1>(m, sh);
+      c[0] = m[0];
+      if constexpr (LAYER) c[1] = m[1];
     }
     if (a.du) {
-      const float m1 = c[0] * inv_c, m0 = LAYER ? c[1] * inv_c : 0.f;
+      const float2 m1 = pair(-c[0] * inv_c), m0 = pair(-c[1] * inv_c);
 #pragma unroll
-      for (int i = 0; i < E; ++i) G[i] = ru * (G[i] - m0 - hu[i] * m1);
+      for (int i = 0; i < H; ++i) {
+        G[i] = fma2(hu[i], m1, G[i]);
+        if (LAYER) G[i] = add2(G[i], m0);
+        G[i] = mul2(G[i], pair(ru));
+      }
       io.store(static_cast<T*>(a.du) + r * a.lddu, G, a.accumulate & TL_ACC_DU);
     }
   }
-  float* part = a.part + (int64_t)blockIdx.x * 3 * a.cols;
+  float* part = a.part + (int64_t)blockIdx.x * 2 * a.cols;
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
+  for (int i = 0; i < Io::E; ++i) {
     const int64_t c = io.at(i / VEC) + i % VEC;
     if (c >= a.cols) continue;
-    if (a.dw_post) part[c] = s_post[i];
-    if (a.dw_pre) part[a.cols + c] = s_pre[i];
-    if (a.dgate && a.gate_mode == TL_GATE_CHANNEL) part[2 * a.cols + c] = s_gate[i];
+    part[c] = i & 1 ? s_post[i / 2].y : s_post[i / 2].x;
+    part[a.cols + c] = i & 1 ? s_pre[i / 2].y : s_pre[i / 2].x;
   }
 }
 
-// Adds the partials of `blocks` blocks: 32 columns of one of the three sums
-// per block; warp w adds partial rows w, w + 32, ... in turn, then the warps
-// in order.
+// Adds the partials of `blocks` blocks: 32 columns of one of the outputs per
+// block (0 dw_post, 1 dw_pre, 2 dgate of a gate per channel); warp w adds
+// partial rows w, w + 32, ... in turn, then the warps in order.
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_sums_kernel(NormArgs a, int64_t blocks) {
   __shared__ float sh[32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, which = blockIdx.y;
+  const bool channel = a.gate_mode == TL_GATE_CHANNEL;
   T* out = static_cast<T*>(which == 0 ? a.dw_post : which == 1 ? a.dw_pre : a.dgate);
-  if (!out || (which == 2 && a.gate_mode != TL_GATE_CHANNEL)) return;
+  if (!out || (which == 2 && !channel)) return;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  const float* part = a.part + (which == 1 ? a.cols : 0);
   float s = 0.f;
   if (c < a.cols) {
 #pragma unroll 4
-    for (int64_t b = w; b < blocks; b += 32) s += a.part[(b * 3 + which) * a.cols + c];
+    for (int64_t b = w; b < blocks; b += 32) s += part[b * 2 * a.cols + c];
   }
   sh[w][lane] = s;
   __syncthreads();
@@ -430,6 +525,8 @@ __global__ void __launch_bounds__(1024) norm_sums_kernel(NormArgs a, int64_t blo
     float t = 0.f;
 #pragma unroll
     for (int k = 0; k < 32; ++k) t += sh[k][lane];
+    if (which == 0 && channel) t *= to_f32(static_cast<const T*>(a.gate)[c]);
+    if (which == 2 && a.w_post) t *= to_f32(static_cast<const T*>(a.w_post)[c]);
     const int flag = which == 0 ? TL_ACC_DW_POST : which == 1 ? TL_ACC_DW_PRE : TL_ACC_DGATE;
     from_f32(out + c, (a.accumulate & flag) ? to_f32(out[c]) + t : t);
   }
@@ -500,8 +597,8 @@ template <typename T, bool LAYER>
 __global__ void __launch_bounds__(kLong) residual_norm_bwd_long_kernel(NormArgs a) {
   __shared__ float sh[32];
   const float inv_c = 1.f / (float)a.cols;
-  float* part = a.part + (int64_t)blockIdx.x * 3 * a.cols;
-  for (int64_t c = threadIdx.x; c < 3 * a.cols; c += kLong) part[c] = 0.f;
+  float* part = a.part + (int64_t)blockIdx.x * 2 * a.cols;
+  for (int64_t c = threadIdx.x; c < 2 * a.cols; c += kLong) part[c] = 0.f;
   __syncthreads();  // column c's partials belong to thread c % kLong below
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const LongRow<T, LAYER> R{a, r, sh, inv_c};
@@ -543,9 +640,8 @@ __global__ void __launch_bounds__(kLong) residual_norm_bwd_long_kernel(NormArgs 
       float du = 0.f, dg = 0.f;
       if (a.u) {
         const float p = g * R.gate(c), h = hat_u(c);
-        part[c] += p * h;
+        part[c] += (a.gate_mode == TL_GATE_CHANNEL ? g : p) * h;
         dg = g * h * R.w_post(c);
-        if (a.gate_mode == TL_GATE_CHANNEL) part[2 * a.cols + c] += dg;
         du = su.y * (p * R.w_post(c) - e0 - h * e1);
       }
       if (a.dx) {
@@ -576,18 +672,14 @@ int64_t bwd_blocks(int64_t rows, int64_t cols) {
   return std::max<int64_t>(1, std::min<int64_t>(rows, per_sm * sm_count()));
 }
 
-// Rows on their way per block: what fits beside the SM's other blocks, at
-// least the row itself and at most four, and no more than a block has.
-int ahead_depth(int64_t row_bytes, int64_t per_sm, int64_t rows, int64_t grid) {
-  const int64_t fit = kSmem / per_sm / std::max<int64_t>(1, row_bytes);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({fit, 4, (rows + grid - 1) / grid}));
-}
-
+// Rows on their way per block: what fits beside the weights and the SM's other
+// blocks, at least the row itself and at most four, and no more than a block has.
 template <typename K>
-int launch_rows(K kern, const NormArgs& a, int64_t grid, int nt, int64_t row_bytes, int64_t per_sm,
-                cudaStream_t st) {
-  const int depth = ahead_depth(row_bytes, per_sm, a.rows, grid);
-  const size_t smem = (size_t)(depth * row_bytes);
+int launch_rows(K kern, const NormArgs& a, int64_t grid, int nt, int64_t row_bytes, int64_t weight_bytes,
+                int64_t per_sm, cudaStream_t st) {
+  const int64_t fit = (kSmem / per_sm - weight_bytes) / row_bytes;
+  const int depth = (int)std::max<int64_t>(1, std::min<int64_t>({fit, 4, (a.rows + grid - 1) / grid}));
+  const size_t smem = (size_t)(weight_bytes + depth * row_bytes);
   TL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   kern<<<(unsigned)grid, nt, smem, st>>>(a, depth);
   return after_launch();
@@ -595,11 +687,13 @@ int launch_rows(K kern, const NormArgs& a, int64_t grid, int nt, int64_t row_byt
 
 template <typename T, int VEC, int NT, int NV>
 int launch_fwd(const NormArgs& a, int kind, cudaStream_t st) {
-  constexpr int64_t row = 2 * Ahead<T, NT, VEC, NV, 2>::kArray, per_sm = NT <= 512 ? 1024 / NT : 1;
+  constexpr int64_t per_sm = 1024 / NT, w = 2 * RowWeights<T, NT, VEC, NV>::kBytes;
+  using A = Ahead<T, NT, VEC, NV, 3>;
+  const int64_t row = A::kStaged ? (a.gate_mode == TL_GATE_FULL ? 3 : 2) * A::kArray : 16;
   const int64_t grid = std::min<int64_t>(a.rows, per_sm * sm_count());
   return kind == TL_NORM_LAYER
-             ? launch_rows(residual_norm_kernel<T, NT, VEC, NV, true>, a, grid, NT, row, per_sm, st)
-             : launch_rows(residual_norm_kernel<T, NT, VEC, NV, false>, a, grid, NT, row, per_sm, st);
+             ? launch_rows(residual_norm_kernel<T, NT, VEC, NV, true>, a, grid, NT, row, w, per_sm, st)
+             : launch_rows(residual_norm_kernel<T, NT, VEC, NV, false>, a, grid, NT, row, w, per_sm, st);
 }
 
 template <typename T, int VEC>
@@ -613,11 +707,13 @@ int forward(const NormArgs& a, int kind, cudaStream_t st) {
 
 template <typename T, int VEC, int NT, int NV>
 int launch_bwd(const NormArgs& a, int kind, cudaStream_t st) {
-  constexpr int64_t row = 4 * Ahead<T, NT, VEC, NV, 4>::kArray, per_sm = NT <= 256 ? 512 / NT : 1;
+  constexpr int64_t per_sm = NT <= 256 ? 512 / NT : 1, w = 2 * RowWeights<T, NT, VEC, NV>::kBytes;
+  using A = Ahead<T, NT, VEC, NV, 5>;
+  const int64_t row = A::kStaged ? (a.gate_mode == TL_GATE_FULL ? 5 : 4) * A::kArray : 16;
   const int64_t grid = bwd_blocks(a.rows, a.cols);
   return kind == TL_NORM_LAYER
-             ? launch_rows(residual_norm_bwd_kernel<T, NT, VEC, NV, true>, a, grid, NT, row, per_sm, st)
-             : launch_rows(residual_norm_bwd_kernel<T, NT, VEC, NV, false>, a, grid, NT, row, per_sm, st);
+             ? launch_rows(residual_norm_bwd_kernel<T, NT, VEC, NV, true>, a, grid, NT, row, w, per_sm, st)
+             : launch_rows(residual_norm_bwd_kernel<T, NT, VEC, NV, false>, a, grid, NT, row, w, per_sm, st);
 }
 
 template <typename T, int VEC>
@@ -724,7 +820,7 @@ int tl_residual_norm(int dtype, int kind, int64_t rows, int64_t cols, const void
 
 size_t tl_residual_norm_scratch_bytes(int64_t rows, int64_t cols) {
   if (rows < 0 || cols <= 0) return 0;
-  return (size_t)tl::bwd_blocks(rows, cols) * 3 * (size_t)cols * sizeof(float);
+  return (size_t)tl::bwd_blocks(rows, cols) * 2 * (size_t)cols * sizeof(float);
 }
 
 int tl_residual_norm_backward(int dtype, int kind, int64_t rows, int64_t cols, const void* x,
