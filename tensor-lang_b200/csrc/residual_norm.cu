@@ -69,36 +69,49 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a
 __device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
 __device__ __forceinline__ float hsum(float2 a) { return a.x + a.y; }
 
-// Sums over a row's threads (the whole block).
-template <int NT, int K>
-__device__ __forceinline__ void row_sum(float (&v)[K], float* sh) {
-  constexpr int NW = NT / 32;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+// Sums over a row's threads (the whole block), a float each in two buffers
+// used in turn: a sum's writes cannot meet the last one's reads, which every
+// thread ended before the barrier between them.
+template <int NT>
+struct RowSum {
+  static constexpr int NW = NT / 32, kMost = 3;
+  float* sh;  // [2][kMost][NW]
+  int turn = 0;
+  template <int K>
+  __device__ __forceinline__ void operator()(float (&v)[K]) {
+    static_assert(K <= kMost, "buffer");
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    float* b = sh + turn * kMost * NW;
+    turn ^= 1;
 #pragma unroll
-  for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
-  __syncthreads();  // the previous sum's readers are done
-  if (lane == 0) {
+    for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
+    if (lane == 0) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) sh[k * NW + w] = v[k];
+      for (int k = 0; k < K; ++k) b[k * NW + w] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if constexpr (NW <= 8) {
+        v[k] = b[k * NW];
+#pragma unroll
+        for (int i = 1; i < NW; ++i) v[k] += b[k * NW + i];
+      } else {
+        float t = lane < NW ? b[k * NW + lane] : 0.f;
+        v[k] = warp_sum(t);
+      }
+    }
   }
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    float t = lane < NW ? sh[k * NW + lane] : 0.f;
-#pragma unroll
-    for (int o = NW < 32 ? NW / 2 : 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    v[k] = __shfl_sync(0xffffffffu, t, 0);
-  }
-}
+};
 
 // A thread's elements of a row, in pairs: vector j of VEC elements at
 // (j * NT + t) * VEC.
 template <typename T, int NT, int VEC, int NV>
 struct RowIo {
   static constexpr int E = VEC * NV, H = E / 2;
-  int64_t cols;
+  int cols;  // at most 16 * NT
   int t;
-  __device__ __forceinline__ int64_t at(int j) const { return ((int64_t)j * NT + t) * VEC; }
+  __device__ __forceinline__ int at(int j) const { return (j * NT + t) * VEC; }
   __device__ __forceinline__ bool in(int i) const { return at(i / VEC) < cols; }
   __device__ __forceinline__ bool full() const { return at(NV - 1) < cols; }
   __device__ __forceinline__ void store(T* p, const float2 (&v)[H], bool add) const {
@@ -125,19 +138,21 @@ struct RowIo {
 // v becomes hat(v) for the elements a thread holds; returns 1 / scale.
 // Elements past the row are zero and stay out of the centred sum.
 template <bool LAYER, typename T, int NT, int VEC, int NV, int H>
-__device__ __forceinline__ float normalise(const RowIo<T, NT, VEC, NV>& io, float2 (&v)[H], float eps,
-                                           float* sh) {
-  const float cols = (float)io.cols;
+__device__ __forceinline__ float normalise(const RowIo<T, NT, VEC, NV>& io, float2 (&v)[H], float inv_c,
+                                           float eps, RowSum<NT>& sum) {
   float s[1];
   float2 q = pair(0.f);
   if constexpr (LAYER) {
 #pragma unroll
     for (int i = 0; i < H; ++i) q = add2(q, v[i]);
     s[0] = hsum(q);
-    row_sum<NT, 1>(s, sh);
-    const float2 mean = pair(-(s[0] / cols));  // divided: the mean of a constant row is that constant
+    sum(s);
+    // s / cols, by one correction of s * inv_c: the mean of a constant row is
+    // that constant where its sum is exact
+    float m = s[0] * inv_c;
+    m = fmaf(fmaf(-m, (float)io.cols, s[0]), inv_c, m);
 #pragma unroll
-    for (int i = 0; i < H; ++i) v[i] = add2(v[i], mean);
+    for (int i = 0; i < H; ++i) v[i] = add2(v[i], pair(-m));
     if (!io.full()) {
 #pragma unroll
       for (int i = 0; i < H; ++i) {
@@ -150,8 +165,8 @@ __device__ __forceinline__ float normalise(const RowIo<T, NT, VEC, NV>& io, floa
 #pragma unroll
   for (int i = 0; i < H; ++i) q = fma2(v[i], v[i], q);
   s[0] = hsum(q);
-  row_sum<NT, 1>(s, sh);
-  const float r = 1.f / sqrtf(s[0] / cols + eps);
+  sum(s);
+  const float r = rsqrtf(fmaf(s[0], inv_c, eps));  // within 2 ulp
 #pragma unroll
   for (int i = 0; i < H; ++i) v[i] = mul2(v[i], pair(r));
   return r;
@@ -244,7 +259,7 @@ struct RowWeights {
       float e[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int64_t c = io.at((4 * i + k) / VEC) + (4 * i + k) % VEC;
+        const int c = io.at((4 * i + k) / VEC) + (4 * i + k) % VEC;
         e[k] = c < io.cols ? (w ? to_f32(w[c]) : 1.f) * (g ? to_f32(g[c]) : 1.f) : 0.f;
       }
       p[i * NT + io.t] = make_float4(e[0], e[1], e[2], e[3]);
@@ -268,8 +283,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) residual_norm_kernel(NormArgs a
   using W = RowWeights<T, NT, VEC, NV>;
   constexpr int H = Io::H;
   extern __shared__ __align__(16) unsigned char dyn[];
-  __shared__ float sh[32];
-  const Io io{a.cols, (int)threadIdx.x};
+  __shared__ float sh[2 * 3 * (NT / 32)];
+  RowSum<NT> sum{sh};
+  const Io io{(int)a.cols, (int)threadIdx.x};
+  const float inv_c = 1.f / (float)a.cols;
   const bool full_gate = a.gate_mode == TL_GATE_FULL;
   const Ahead<T, NT, VEC, NV, 3> rows{{a.x, a.u, full_gate ? a.gate : nullptr}, {a.ldx, a.ldu, a.ldg},
                                       dyn + 2 * W::kBytes, depth, full_gate ? 3 : 2};
@@ -291,7 +308,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) residual_norm_kernel(NormArgs a
     if (a.u) {
       float2 v[H], w[H];
       rows.load(io, 1, r, slot, v);
-      normalise<LAYER>(io, v, a.eps, sh);
+      normalise<LAYER>(io, v, inv_c, a.eps, sum);
       w_post.load(io, w);
       if (full_gate) {
         float2 g[H];
@@ -308,7 +325,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) residual_norm_kernel(NormArgs a
     }
     if (a.y) io.store(static_cast<T*>(a.y) + r * a.ldy, y, false);
     if (a.n) {
-      normalise<LAYER>(io, y, a.eps, sh);
+      normalise<LAYER>(io, y, inv_c, a.eps, sum);
       float2 w[H];
       w_pre.load(io, w);
 #pragma unroll
@@ -333,8 +350,9 @@ __global__ void __launch_bounds__(NT, NT <= 256 ? 512 / NT : 1)
   using W = RowWeights<T, NT, VEC, NV>;
   constexpr int H = Io::H;
   extern __shared__ __align__(16) unsigned char dyn[];
-  __shared__ float sh[3 * 32];
-  const Io io{a.cols, (int)threadIdx.x};
+  __shared__ float sh[2 * 3 * (NT / 32)];
+  RowSum<NT> sum{sh};
+  const Io io{(int)a.cols, (int)threadIdx.x};
   const bool full_gate = a.gate_mode == TL_GATE_FULL, token_gate = a.gate_mode == TL_GATE_TOKEN;
   const Ahead<T, NT, VEC, NV, 5> rows{{a.u, a.x, a.dn, a.dy, full_gate ? a.gate : nullptr},
                                       {a.ldu, a.ldx, a.lddn, a.lddy, a.ldg},
@@ -372,7 +390,7 @@ __global__ void __launch_bounds__(NT, NT <= 256 ? 512 / NT : 1)
     float ru = 0.f;
     if (a.u) {
       rows.load(io, 0, r, slot, hu);
-      ru = normalise<LAYER>(io, hu, a.eps, sh);
+      ru = normalise<LAYER>(io, hu, inv_c, a.eps, sum);
     }
     if (a.dn) {
       float2 y[H], d[H];
@@ -384,7 +402,7 @@ __global__ void __launch_bounds__(NT, NT <= 256 ? 512 / NT : 1)
 #pragma unroll
         for (int i = 0; i < H; ++i) y[i] = fma2(hu[i], d[i], y[i]);
       }
-      const float ry = normalise<LAYER>(io, y, a.eps, sh);  // y: hat(y)
+      const float ry = normalise<LAYER>(io, y, inv_c, a.eps, sum);  // y: hat(y)
       rows.load(io, 2, r, slot, d);
       float2 c0 = pair(0.f), c1 = pair(0.f);
       w_pre.load(io, G);
@@ -398,7 +416,7 @@ __global__ void __launch_bounds__(NT, NT <= 256 ? 512 / NT : 1)
       float m[LAYER ? 2 : 1];
       m[0] = hsum(c0);
       if constexpr (LAYER) m[1] = hsum(c1);
-      row_sum<NT, LAYER ? 2 : 1>(m, sh);
+      sum(m);
       const float2 m1 = pair(-m[0] * inv_c);
 #pragma unroll
       for (int i = 0; i < H; ++i) G[i] = fma2(y[i], m1, d[i]);
@@ -468,7 +486,7 @@ __global__ void __launch_bounds__(NT, NT <= 256 ? 512 / NT : 1)
       c[1] = hsum(c1);
     }
     if (token) {
-      row_sum<NT, 3>(c, sh);
+      sum(c);
       if (threadIdx.x == 0) {
         T* p = static_cast<T*>(a.dgate) + r;
         from_f32(p, (a.accumulate & TL_ACC_DGATE) ? to_f32(*p) + c[2] : c[2]);
@@ -477,7 +495,7 @@ __global__ void __launch_bounds__(NT, NT <= 256 ? 512 / NT : 1)
       float m[LAYER ? 2 : 1];
       m[0] = c[0];
       if constexpr (LAYER) m[1] = c[1];
-      row_sum<NT, LAYER ? 2 : 1>(m, sh);
+      sum(m);
       c[0] = m[0];
       if constexpr (LAYER) c[1] = m[1];
     }
@@ -543,9 +561,12 @@ struct LongRow {
   float* sh;
   float inv_c;
   __device__ float sum(float v) const {
-    float s[1] = {v};
-    row_sum<kLong, 1>(s, sh);
-    return s[0];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    v = warp_sum(v);
+    __syncthreads();  // the previous sum's readers are done
+    if (lane == 0) sh[w] = v;
+    __syncthreads();
+    return warp_sum(sh[lane]);
   }
   template <typename F>
   __device__ float total(F f) const {
