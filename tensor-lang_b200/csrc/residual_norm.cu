@@ -19,6 +19,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "lm_common.cuh"
 
@@ -682,68 +683,92 @@ __global__ void __launch_bounds__(kLong) residual_norm_bwd_long_kernel(NormArgs 
 }
 
 // ------------------------------------------------------------- host side ---
-// The register kernels hold a row in NT threads x 16 elements (or fewer).
-constexpr int64_t kMaxCols = 8192;
-constexpr int64_t kSmem = 216 << 10;  // of an SM, for rows on their way
+constexpr int64_t kMaxCols = 8192;    // of the register kernels
+constexpr int64_t kSmem = 216 << 10;  // of an SM, for weights and rows on their way
 
-// Blocks of the backward (and rows of its partials): 512 threads an SM while
-// rows are short, at most eight blocks of them.
+// Elements a thread holds: 16 bf16, or 8 float32, whose rows and weights on
+// their way take 384 bytes a thread in the backward (16 would leave 288 threads
+// an SM).  The longest bf16 rows of a forward take 8 as well: one block of 1024
+// threads has room for two rows on their way beside the weights.
+template <typename T>
+constexpr int kElems = sizeof(T) == 4 ? 8 : 16;
+
+// Threads per row, so that a row fits: 64 to 1024.
+template <int E, typename F>
+int by_width(int64_t cols, F f) {
+  if (cols <= 64 * E) return f(std::integral_constant<int, 64>{});
+  if (cols <= 128 * E) return f(std::integral_constant<int, 128>{});
+  if (cols <= 256 * E) return f(std::integral_constant<int, 256>{});
+  if constexpr (512 * E < kMaxCols) {
+    if (cols <= 512 * E) return f(std::integral_constant<int, 512>{});
+    return f(std::integral_constant<int, kMaxCols / E>{});
+  } else {
+    return f(std::integral_constant<int, 512>{});
+  }
+}
+
+// Blocks of the backward at most (rows of its partials): 512 threads an SM.
 int64_t bwd_blocks(int64_t rows, int64_t cols) {
   const int64_t per_sm = cols > 4096 ? 1 : cols > 2048 ? 2 : cols > 1024 ? 4 : 8;
   return std::max<int64_t>(1, std::min<int64_t>(rows, per_sm * sm_count()));
 }
 
-// Rows on their way per block: what fits beside the weights and the SM's other
-// blocks, at least the row itself and at most four, and no more than a block has.
+// Blocks an SM holds and rows each has on its way: two rows (the one worked on
+// and the next) where that leaves at least 256 threads an SM, else one; at most
+// four rows.
+struct Shape {
+  int64_t grid;
+  int depth;
+};
+Shape launch_shape(int64_t rows, int nt, int64_t most_threads, int64_t row_bytes, int64_t weight_bytes,
+                   int64_t most_blocks) {
+  int64_t per_sm = std::max<int64_t>(1, most_threads / nt);
+  auto fit = [&](int64_t blocks) { return (kSmem / blocks - weight_bytes - 1024) / row_bytes; };
+  while (per_sm > 1 && (fit(per_sm) < 1 || (fit(per_sm) < 2 && (per_sm - 1) * nt >= 256 && nt <= 256))) --per_sm;
+  Shape q;
+  q.grid = std::min<int64_t>({rows, per_sm * sm_count(), most_blocks});
+  q.depth = (int)std::max<int64_t>(1, std::min<int64_t>({fit(per_sm), 4, (rows + q.grid - 1) / q.grid}));
+  return q;
+}
+
 template <typename K>
-int launch_rows(K kern, const NormArgs& a, int64_t grid, int nt, int64_t row_bytes, int64_t weight_bytes,
-                int64_t per_sm, cudaStream_t st) {
-  const int64_t fit = (kSmem / per_sm - weight_bytes) / row_bytes;
-  const int depth = (int)std::max<int64_t>(1, std::min<int64_t>({fit, 4, (a.rows + grid - 1) / grid}));
-  const size_t smem = (size_t)(weight_bytes + depth * row_bytes);
+int launch_rows(K kern, const NormArgs& a, Shape q, int nt, int64_t row_bytes, int64_t weight_bytes,
+                cudaStream_t st) {
+  const size_t smem = (size_t)(weight_bytes + q.depth * row_bytes);
   TL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  kern<<<(unsigned)grid, nt, smem, st>>>(a, depth);
+  kern<<<(unsigned)q.grid, nt, smem, st>>>(a, q.depth);
   return after_launch();
 }
 
-template <typename T, int VEC, int NT, int NV>
-int launch_fwd(const NormArgs& a, int kind, cudaStream_t st) {
-  constexpr int64_t per_sm = 1024 / NT, w = 2 * RowWeights<T, NT, VEC, NV>::kBytes;
-  using A = Ahead<T, NT, VEC, NV, 3>;
-  const int64_t row = A::kStaged ? (a.gate_mode == TL_GATE_FULL ? 3 : 2) * A::kArray : 16;
-  const int64_t grid = std::min<int64_t>(a.rows, per_sm * sm_count());
-  return kind == TL_NORM_LAYER
-             ? launch_rows(residual_norm_kernel<T, NT, VEC, NV, true>, a, grid, NT, row, w, per_sm, st)
-             : launch_rows(residual_norm_kernel<T, NT, VEC, NV, false>, a, grid, NT, row, w, per_sm, st);
-}
-
-template <typename T, int VEC>
+template <typename T, int VEC, int E>
 int forward(const NormArgs& a, int kind, cudaStream_t st) {
-  const int64_t c = a.cols;
-  if (c <= 1024) return launch_fwd<T, VEC, 64, 16 / VEC>(a, kind, st);
-  if (c <= 2048) return launch_fwd<T, VEC, 128, 16 / VEC>(a, kind, st);
-  if (c <= 4096) return launch_fwd<T, VEC, 256, 16 / VEC>(a, kind, st);
-  return launch_fwd<T, VEC, 512, 16 / VEC>(a, kind, st);
+  return by_width<E>(a.cols, [&](auto threads) {
+    constexpr int NT = decltype(threads)::value, NV = E / VEC;
+    using A = Ahead<T, NT, VEC, NV, 3>;
+    const int64_t w = 2 * RowWeights<T, NT, VEC, NV>::kBytes;
+    const int64_t row = A::kStaged ? (a.gate_mode == TL_GATE_FULL ? 3 : 2) * A::kArray : 16;
+    const Shape q = launch_shape(a.rows, NT, 1024, row, w, INT32_MAX);
+    return kind == TL_NORM_LAYER
+               ? launch_rows(residual_norm_kernel<T, NT, VEC, NV, true>, a, q, NT, row, w, st)
+               : launch_rows(residual_norm_kernel<T, NT, VEC, NV, false>, a, q, NT, row, w, st);
+  });
 }
 
-template <typename T, int VEC, int NT, int NV>
-int launch_bwd(const NormArgs& a, int kind, cudaStream_t st) {
-  constexpr int64_t per_sm = NT <= 256 ? 512 / NT : 1, w = 2 * RowWeights<T, NT, VEC, NV>::kBytes;
-  using A = Ahead<T, NT, VEC, NV, 5>;
-  const int64_t row = A::kStaged ? (a.gate_mode == TL_GATE_FULL ? 5 : 4) * A::kArray : 16;
-  const int64_t grid = bwd_blocks(a.rows, a.cols);
-  return kind == TL_NORM_LAYER
-             ? launch_rows(residual_norm_bwd_kernel<T, NT, VEC, NV, true>, a, grid, NT, row, w, per_sm, st)
-             : launch_rows(residual_norm_bwd_kernel<T, NT, VEC, NV, false>, a, grid, NT, row, w, per_sm, st);
-}
-
+// grid: the partials' rows
 template <typename T, int VEC>
-int backward(const NormArgs& a, int kind, cudaStream_t st) {
-  const int64_t c = a.cols;
-  if (c <= 1024) return launch_bwd<T, VEC, 64, 16 / VEC>(a, kind, st);
-  if (c <= 2048) return launch_bwd<T, VEC, 128, 16 / VEC>(a, kind, st);
-  if (c <= 4096) return launch_bwd<T, VEC, 256, 16 / VEC>(a, kind, st);
-  return launch_bwd<T, VEC, 512, 16 / VEC>(a, kind, st);
+int backward(const NormArgs& a, int kind, cudaStream_t st, int64_t* grid) {
+  constexpr int E = kElems<T>;
+  return by_width<E>(a.cols, [&](auto threads) {
+    constexpr int NT = decltype(threads)::value, NV = E / VEC;
+    using A = Ahead<T, NT, VEC, NV, 5>;
+    const int64_t w = 2 * RowWeights<T, NT, VEC, NV>::kBytes;
+    const int64_t row = A::kStaged ? (a.gate_mode == TL_GATE_FULL ? 5 : 4) * A::kArray : 16;
+    const Shape q = launch_shape(a.rows, NT, 512, row, w, bwd_blocks(a.rows, a.cols));
+    *grid = q.grid;
+    return kind == TL_NORM_LAYER
+               ? launch_rows(residual_norm_bwd_kernel<T, NT, VEC, NV, true>, a, q, NT, row, w, st)
+               : launch_rows(residual_norm_bwd_kernel<T, NT, VEC, NV, false>, a, q, NT, row, w, st);
+  });
 }
 
 // Whether rows of p (leading dimension ld) take 128-bit accesses.
@@ -773,27 +798,32 @@ int run_forward(const NormArgs& a, int kind, cudaStream_t st) {
       residual_norm_long_kernel<T, false><<<grid, kLong, 0, st>>>(a);
     return after_launch();
   }
-  return vec_ok(a, V) ? forward<T, V>(a, kind, st) : forward<T, 1>(a, kind, st);
+  constexpr int E = kElems<T>;
+  if (vec_ok(a, V))
+    return a.cols > 4096 ? forward<T, V, 8>(a, kind, st) : forward<T, V, E>(a, kind, st);
+  return a.cols > 4096 ? forward<T, 1, 8>(a, kind, st) : forward<T, 1, E>(a, kind, st);
 }
 
 template <typename T>
 int run_backward(const NormArgs& a, int kind, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
+  int64_t blocks = 0;
   if (a.rows > 0) {
     if (a.cols > kMaxCols) {
-      const unsigned grid = (unsigned)bwd_blocks(a.rows, a.cols);
+      blocks = bwd_blocks(a.rows, a.cols);
+      const unsigned grid = (unsigned)blocks;
       if (kind == TL_NORM_LAYER)
         residual_norm_bwd_long_kernel<T, true><<<grid, kLong, 0, st>>>(a);
       else
         residual_norm_bwd_long_kernel<T, false><<<grid, kLong, 0, st>>>(a);
       TL_TRY(after_launch());
     } else {
-      TL_TRY((vec_ok(a, V) ? backward<T, V>(a, kind, st) : backward<T, 1>(a, kind, st)));
+      TL_TRY((vec_ok(a, V) ? backward<T, V>(a, kind, st, &blocks) : backward<T, 1>(a, kind, st, &blocks)));
     }
   }
   if (a.dw_post || a.dw_pre || (a.dgate && a.gate_mode == TL_GATE_CHANNEL)) {
     norm_sums_kernel<T><<<dim3((unsigned)((a.cols + 31) / 32), 3), 1024, 0, st>>>(
-        a, a.rows > 0 ? bwd_blocks(a.rows, a.cols) : 0);
+        a, blocks);
     TL_TRY(after_launch());
   }
   return TL_OK;
