@@ -20,8 +20,8 @@
 //
 // Listed classes: the gradient there is p - q with the q of equal indices
 // added, rounded once.  Their cells in shared memory are replaced by the
-// number of the list entry that came first, and a bit per cell says so; the
-// store pass looks the entry up.  (No atomics on values: sums are in list
+// number of the list entry that came first, and a mark says so; the store
+// pass looks the entry up.  (No atomics on values: sums are in list
 // order.)
 #include <math.h>
 
@@ -36,6 +36,7 @@ constexpr int kMaxTop = 1024;
 constexpr int64_t kSegTarget = 32 << 10;    // bytes of a row a CTA aims at
 constexpr int64_t kSegMax = 192 << 10;      // and the most it takes
 constexpr int kMaxCluster = 8;
+constexpr int kSmemMost = 226 << 10;        // dynamic, beside a few hundred bytes
 
 struct DistillArgs {
   int64_t rows, classes;
@@ -55,7 +56,7 @@ struct DistillArgs {
   void* dz;
   int64_t lddz;
   int accumulate;
-  unsigned* counters;   // [0] rows that count, [1] rows done
+  unsigned* counters;   // [0] rows that count, 0 between calls
   int64_t seg;          // classes per CTA
 };
 
@@ -91,14 +92,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// (m, s) <- the maximum and the sum of exp(k (v - m)) of both parts
-__device__ __forceinline__ void merge(float& m, float& s, float m2, float s2, float k) {
-  const float M = fmaxf(m, m2);
-  const float base = M == -INFINITY ? 0.f : M;  // both empty: 0 + 0
-  s = s * exp2_fast((m - base) * k) + s2 * exp2_fast((m2 - base) * k);
-  m = M;
-}
-
 // Entry k of row r: its class in [0, classes) with a teacher logit above -inf
 // (t), or -1.
 template <typename T>
@@ -107,6 +100,10 @@ __device__ __forceinline__ int entry(const DistillArgs& a, int64_t r, int k, flo
   const int64_t c = class_index(a.index, a.index_type, r * a.ldi + k, a.classes);
   return t == -INFINITY ? -1 : (int)c;
 }
+
+// Words of the marks of a segment: a byte per vector, one before the middle and
+// one behind it besides.
+__host__ __device__ constexpr int mark_words(int64_t seg, int vec) { return (int)((seg / vec + 2 + 3) / 4); }
 
 // Rows with a valid entry, one warp per row.
 template <typename T>
@@ -128,18 +125,19 @@ template <typename T, int NT>
 __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   constexpr int V = 16 / sizeof(T), NW = NT / 32;
   extern __shared__ __align__(16) unsigned char smem[];
-  // [list: class, q, first entry's q sum, its z] [bits of the listed cells] [segment]
+  // [list: class, q, first entry's q sum, its z] [marks of the listed cells] [segment]
   int* li = reinterpret_cast<int*>(smem);
   float* lq = reinterpret_cast<float*>(li + a.top);
   float* lsum = lq + a.top;
   float* lz = lsum + a.top;
-  uint32_t* bits = reinterpret_cast<uint32_t*>(lz + a.top);
-  const int nbits = (int)((a.seg + 31) / 32);
+  // per vector of V cells a byte with the listed ones' bits; the vectors are
+  // those of the middle (below), the cells before it are vector 0
+  uint32_t* marks = reinterpret_cast<uint32_t*>(lz + a.top);
+  const int nmarks = mark_words(a.seg, V);
   unsigned char* cells = reinterpret_cast<unsigned char*>(
-      ((uintptr_t)(bits + nbits) + 15) & ~(uintptr_t)15);
+      ((uintptr_t)(marks + nmarks) + 15) & ~(uintptr_t)15);
   __shared__ float peer[4][kMaxCluster];
-  __shared__ float sh[4][NW];
-  __shared__ unsigned ticket;
+  __shared__ float sh[3][NW];
 
   const uint32_t rank = cluster_rank(), size = cluster_size();
   const int64_t r = blockIdx.x / size;
@@ -154,20 +152,24 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   const int head = min(n, phase ? V - phase : 0), mid = (n - head) / V * V;
   if (size > 1) cluster_arrive();  // every CTA of the cluster runs: waited for before the exchange
 
-  // each thread brings in the vectors it reads in the first pass, so waiting
-  // for its own copies is enough
+  // each thread brings in what it reads in the first pass, so waiting for its
+  // own copies is enough; the row's ends, outside the 16-byte copies, are one
+  // element for each of the first threads (fewer than 2 V)
   for (int i = head + tid * V; i < head + mid; i += NT * V)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(saddr(cell + i)), "l"(src + i)
                  : "memory");
   asm volatile("cp.async.commit_group;" ::: "memory");
-  // the row's ends, outside the 16-byte copies
-  for (int i = tid; i < n - mid; i += NT) {
-    const int c = i < head ? i : mid + i;
-    cell[c] = src[c];
+  const int end = tid < n - mid ? (tid < head ? tid : mid + tid) : -1;
+  float end_z = -INFINITY;
+  if (end >= 0) {
+    cell[end] = src[end];
+    end_z = to_f32(cell[end]);
   }
-  for (int i = tid; i < nbits; i += NT) bits[i] = 0u;
+  for (int i = tid; i < nmarks; i += NT) marks[i] = 0u;
+  const float up = a.upstream ? *a.upstream : 1.f;
+  const float div = a.divisor > 0.f ? a.divisor : fmaxf(1.f, (float)a.counters[0]);
 
-  // the teacher's list: q = softmax(t / tau)
+  // while they are on their way, the teacher's list: q = softmax(t / tau)
   const float k2 = 1.4426950408889634f / a.temperature;  // exp(v / tau) = 2^(v k2)
   const float inv_tau = 1.f / a.temperature;
   float tm = -INFINITY;
@@ -189,10 +191,14 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   for (int i = 1; i < NW; ++i) tm = fmaxf(tm, sh[0][i]);
   float tsum = 0.f, tdot = 0.f;
   for (int k = tid; k < a.top; k += NT) {
-    if (li[k] < 0) continue;
-    const float d = (lq[k] - tm) * inv_tau, e = expf(d);
-    tsum += e;
-    tdot += e > 0.f ? e * d : 0.f;
+    float e = 0.f;
+    if (li[k] >= 0) {
+      const float d = (lq[k] - tm) * inv_tau;
+      e = expf(d);
+      tsum += e;
+      tdot += e > 0.f ? e * d : 0.f;
+    }
+    lq[k] = e;  // q times the sum
   }
   tsum = warp_sum(tsum);
   tdot = warp_sum(tdot);
@@ -208,207 +214,193 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
     tdot += sh[2][i];
   }
   const float inv_t = some ? 1.f / tsum : 0.f;
-  // sum q log q = sum e d / S - log S
-  const float qlogq = some ? tdot * inv_t - logf(tsum) : 0.f;
-  for (int k = tid; k < a.top; k += NT)
-    lq[k] = li[k] >= 0 ? expf((lq[k] - tm) * inv_tau) * inv_t : 0.f;
+  // the q of equal classes added, for the first of them (the others: -1)
+  for (int k = tid; k < a.top; k += NT) {
+    const int c = li[k];
+    if (c < c0 || c >= c0 + n) continue;
+    float sum = 0.f;
+    bool first = true;
+    for (int j = 0; j < a.top; ++j)
+      if (li[j] == c) {
+        first = first && j >= k;
+        sum += lq[j];
+      }
+    lsum[k] = first ? sum * inv_t : -1.f;
+  }
 
-  // the segment is here: its maximum and sum of exponentials
+  // the segment: each thread's maximum and sum of exponentials, then the warp's
   asm volatile("cp.async.wait_group 0;" ::: "memory");
-  __syncthreads();
-  float m = -INFINITY, s = 0.f;
+  float m = end_z, s;
   for (int i = head + tid * V; i < head + mid; i += NT * V) {
     float v[V];
     ld_vec<V>(cell + i, v);
-    float mm = m;
 #pragma unroll
-    for (int j = 0; j < V; ++j) mm = fmaxf(mm, v[j]);
-    const float base = mm == -INFINITY ? 0.f : mm;
-    s *= exp2_fast((m - base) * k2);
+    for (int j = 0; j < V; ++j) m = fmaxf(m, v[j]);
+  }
+  {
+    const float base = m == -INFINITY ? 0.f : m;
+    const float2 nb = make_float2(-base, -base), kk = make_float2(k2, k2);
+    float2 t = make_float2(end >= 0 ? exp2_fast((end_z - base) * k2) : 0.f, 0.f);
+    for (int i = head + tid * V; i < head + mid; i += NT * V) {
+      float v[V];
+      ld_vec<V>(cell + i, v);
 #pragma unroll
-    for (int j = 0; j < V; ++j) s += exp2_fast((v[j] - base) * k2);
-    m = mm;
+      for (int j = 0; j < V; j += 2) {
+        const float2 x = __fmul2_rn(__fadd2_rn(make_float2(v[j], v[j + 1]), nb), kk);
+        t = __fadd2_rn(t, make_float2(exp2_fast(x.x), exp2_fast(x.y)));
+      }
+    }
+    s = t.x + t.y;
+    const float wm = warp_max(m), wbase = wm == -INFINITY ? 0.f : wm;
+    s = warp_sum(s * exp2_fast((m - wbase) * k2));
+    m = wm;
   }
-  for (int i = tid; i < n - mid; i += NT) {
-    const float v = to_f32(cell[i < head ? i : mid + i]);
-    merge(m, s, v, v == -INFINITY ? 0.f : 1.f, k2);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-    merge(m, s, m2, s2, k2);
-  }
-  __syncthreads();  // sh's earlier readers are done
+  __syncthreads();  // sh's readers are done; every cell, mark and list entry is there
   if (lane == 0) {
     sh[0][w] = m;
     sh[1][w] = s;
   }
   __syncthreads();
-  m = sh[0][0];
-  s = sh[1][0];
-#pragma unroll
-  for (int i = 1; i < NW; ++i) merge(m, s, sh[0][i], sh[1][i], k2);
-  // the list's entries in this segment: the sums of q and of q (z - m) / tau
-  // (differences to the maximum: logits of the type's lowest value cancel
-  // exactly); equal classes are handled by the first of them
-  float dot = 0.f, qs = 0.f;
-  {
-    const float base = m == -INFINITY ? 0.f : m;
-    for (int k = tid; k < a.top; k += NT) {
+  if (w == 0) {
+    m = lane < NW ? sh[0][lane] : -INFINITY;
+    s = lane < NW ? sh[1][lane] : 0.f;
+    const float sm = warp_max(m), base = sm == -INFINITY ? 0.f : sm;
+    s = warp_sum(s * exp2_fast((m - base) * k2));
+    // the list's entries in this segment: the sums of q and of q (z - m) / tau
+    // (differences to the maximum: logits of the type's lowest value cancel
+    // exactly); their cells make way for the entry's number
+    float dot = 0.f, qs = 0.f;
+    for (int k = lane; k < a.top; k += 32) {
       const int c = li[k];
       if (c < c0 || c >= c0 + n) continue;
-      const float zc = to_f32(cell[c - c0]);
-      if (lq[k] > 0.f || lq[k] != lq[k]) {
-        dot += lq[k] * ((zc - base) * inv_tau);
-        qs += lq[k];
+      const float q = lq[k] * inv_t, z = to_f32(cell[c - c0]);
+      lz[k] = z;
+      if (q > 0.f || q != q) {
+        dot += q * ((z - base) * inv_tau);
+        qs += q;
       }
-      float sum = 0.f;
-      bool first = true;
-      for (int j = 0; j < a.top; ++j)
-        if (li[j] == c) {
-          first = first && j >= k;
-          sum += lq[j];
-        }
-      lz[k] = zc;
-      lsum[k] = first ? sum : -1.f;
     }
-  }
-  dot = warp_sum(dot);
-  qs = warp_sum(qs);
-  if (lane == 0) {
-    sh[2][w] = dot;
-    sh[3][w] = qs;
-  }
-  __syncthreads();
-  for (int k = tid; k < a.top; k += NT) {
-    const int c = li[k] - (int)c0;
-    if (li[k] < 0 || c < 0 || c >= n || lsum[k] < 0.f) continue;
-    atomicOr(&bits[c >> 5], 1u << (c & 31));
-    if constexpr (sizeof(T) == 2)
-      reinterpret_cast<uint16_t*>(cell)[c] = (uint16_t)k;
-    else
-      reinterpret_cast<uint32_t*>(cell)[c] = (uint32_t)k;
-  }
-  dot = sh[2][0];
-  qs = sh[3][0];
-#pragma unroll
-  for (int i = 1; i < NW; ++i) {
-    dot += sh[2][i];
-    qs += sh[3][i];
-  }
-  if (size > 1) {
-    cluster_wait();
-    if (tid < (int)size) {
-      st_peer(&peer[0][rank], tid, m);
-      st_peer(&peer[1][rank], tid, s);
-      st_peer(&peer[2][rank], tid, dot);
-      st_peer(&peer[3][rank], tid, qs);
+    dot = warp_sum(dot);  // every lane has read its cells
+    qs = warp_sum(qs);
+    for (int k = lane; k < a.top; k += 32) {
+      const int c = li[k] - (int)c0;
+      if (li[k] < 0 || c < 0 || c >= n || lsum[k] < 0.f) continue;
+      const int at = c - head + V;  // byte at / V, bit at % V
+      atomicOr(&marks[at / V >> 2], 1u << (8 * (at / V & 3) + at % V));
+      if constexpr (sizeof(T) == 2)
+        reinterpret_cast<uint16_t*>(cell)[c] = (uint16_t)k;
+      else
+        reinterpret_cast<uint32_t*>(cell)[c] = (uint32_t)k;
+    }
+    if (size > 1) cluster_wait();
+    if (lane < (int)size) {
+      st_peer(&peer[0][rank], lane, sm);
+      st_peer(&peer[1][rank], lane, s);
+      st_peer(&peer[2][rank], lane, dot);
+      st_peer(&peer[3][rank], lane, qs);
     }
     __syncwarp();
+  } else if (size > 1) {
+    cluster_wait();
+  }
+  if (size > 1) {
     cluster_arrive();
     cluster_wait();
-    m = peer[0][0];
-    s = peer[1][0];
-    for (uint32_t i = 1; i < size; ++i) merge(m, s, peer[0][i], peer[1][i], k2);
-    const float base = m == -INFINITY ? 0.f : m;
-    dot = 0.f;
-    for (uint32_t i = 0; i < size; ++i) {
-      const float mi = peer[0][i] == -INFINITY ? 0.f : peer[0][i];
-      dot += peer[3][i] == 0.f ? 0.f : peer[2][i] + peer[3][i] * ((mi - base) * inv_tau);
-    }
   } else {
-    __syncthreads();  // the marked cells are seen by all
+    __syncthreads();
+  }
+  m = peer[0][0];
+  for (uint32_t i = 1; i < size; ++i) m = fmaxf(m, peer[0][i]);
+  const float base = m == -INFINITY ? 0.f : m;
+  float dot = 0.f;
+  s = 0.f;
+  for (uint32_t i = 0; i < size; ++i) {
+    const float mi = peer[0][i] == -INFINITY ? 0.f : peer[0][i];
+    s += peer[1][i] == 0.f ? 0.f : peer[1][i] * exp2_fast((mi - base) * k2);
+    dot += peer[3][i] == 0.f ? 0.f : peer[2][i] + peer[3][i] * ((mi - base) * inv_tau);
   }
   if (rank == 0 && tid == 0) {
     const float log_s = logf(s);  // a row of -inf: -inf
     if (a.lse) a.lse[r] = m * inv_tau + log_s;
     float l = 0.f;
-    if (some)
+    if (some) {
+      // sum q log q = sum e d / S - log S
+      const float qlogq = tdot * inv_t - logf(tsum);
       l = dot == -INFINITY ? INFINITY : a.temperature * a.temperature * (qlogq + (log_s - dot));
-    a.row_loss[r] = l;
+    }
+    if (a.row_loss) a.row_loss[r] = l;
   }
-  const unsigned counted = a.counters[0];
-  const float div = a.divisor > 0.f ? a.divisor : fmaxf(1.f, (float)counted);
-  if (a.dz) {
-    const float up = a.upstream ? *a.upstream : 1.f;
-    const float cf = some ? a.temperature * up / div : 0.f;
-    // p = exp((z - m) / tau) / s: nearer than exp(z / tau - lse), whose lse is rounded
-    const float inv_s = s > 0.f || s != s ? 1.f / s : 0.f;
-    const float base = m == -INFINITY ? 0.f : m;
-    auto grad = [&](int c) {  // of cell c
-      float z = to_f32(cell[c]), q = 0.f;
-      if (bits[c >> 5] >> (c & 31) & 1u) {
-        const int k = sizeof(T) == 2 ? (int)reinterpret_cast<const uint16_t*>(cell)[c]
-                                     : (int)reinterpret_cast<const uint32_t*>(cell)[c];
-        z = lz[k];
-        q = lsum[k];
-      }
-      return cf * (exp2_fast((z - base) * k2) * inv_s - q);
-    };
-    T* dst = static_cast<T*>(a.dz) + r * a.lddz + c0;
-    const bool add_to = a.accumulate != 0;
-    const bool vec = ((uintptr_t)(dst + head) & 15) == 0;
-    if (!some && !add_to) {
+  if (!a.dz) return;
+  const float cf = some ? a.temperature * up / div : 0.f;
+  // p = exp((z - m) / tau) / s: nearer than exp(z / tau - lse), whose lse is rounded
+  const float inv_s = s > 0.f || s != s ? 1.f / s : 0.f;
+  auto grad = [&](int c) {  // of cell c
+    const int at = c - head + V;
+    float z = to_f32(cell[c]), q = 0.f;
+    if (marks[at / V >> 2] >> (8 * (at / V & 3) + at % V) & 1u) {
+      const int k = sizeof(T) == 2 ? (int)reinterpret_cast<const uint16_t*>(cell)[c]
+                                   : (int)reinterpret_cast<const uint32_t*>(cell)[c];
+      z = lz[k];
+      q = lsum[k];
+    }
+    return cf * (exp2_fast((z - base) * k2) * inv_s - q);
+  };
+  T* dst = static_cast<T*>(a.dz) + r * a.lddz + c0;
+  const bool add_to = a.accumulate != 0;
+  if (!some) {
+    if (!add_to)
       for (int i = tid; i < n; i += NT) from_f32(dst + i, 0.f);
-    } else if (some) {
-      if (vec) {
-        for (int i = head + tid * V; i < head + mid; i += NT * V) {
-          float v[V], o[V];
-          ld_vec<V>(cell + i, v);
-          uint32_t b = 0;
-          // V cells' bits may lie in two words
-          const int w0 = i >> 5, w1 = (i + V - 1) >> 5, sft = i & 31;
-          b = bits[w0] >> sft;
-          if (w1 != w0) b |= bits[w1] << (32 - sft);
-          b &= (1u << V) - 1u;
+    return;
+  }
+  if (((uintptr_t)(dst + head) & 15) != 0) {
+    for (int c = tid; c < n; c += NT) from_f32(dst + c, (add_to ? to_f32(dst[c]) : 0.f) + grad(c));
+    return;
+  }
+  const float2 nb = make_float2(-base, -base), kk = make_float2(k2, k2);
+  const float2 cs = make_float2(cf * inv_s, cf * inv_s);
+  const unsigned char* mark_of = reinterpret_cast<const unsigned char*>(marks);
+  for (int i = head + tid * V; i < head + mid; i += NT * V) {
+    float v[V], o[V];
+    ld_vec<V>(cell + i, v);
 #pragma unroll
-          for (int j = 0; j < V; ++j) o[j] = cf * (exp2_fast((v[j] - base) * k2) * inv_s);
-          if (b) {
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-              if (b >> j & 1u) o[j] = grad(i + j);
-          }
-          if (add_to) {
-            ld_vec<V>(dst + i, v);
-#pragma unroll
-            for (int j = 0; j < V; ++j) o[j] += v[j];
-          }
-          st_vec<V>(dst + i, o);
-        }
-        for (int i = tid; i < n - mid; i += NT) {
-          const int c = i < head ? i : mid + i;
-          from_f32(dst + c, (add_to ? to_f32(dst[c]) : 0.f) + grad(c));
-        }
-      } else {
-        for (int c = tid; c < n; c += NT)
-          from_f32(dst + c, (add_to ? to_f32(dst[c]) : 0.f) + grad(c));
-      }
+    for (int j = 0; j < V; j += 2) {
+      const float2 x = __fmul2_rn(__fadd2_rn(make_float2(v[j], v[j + 1]), nb), kk);
+      const float2 y = __fmul2_rn(make_float2(exp2_fast(x.x), exp2_fast(x.y)), cs);
+      o[j] = y.x;
+      o[j + 1] = y.y;
     }
-  }
-  // the last row's cluster to finish writes the mean and clears the counters
-  if (rank == 0 && tid == 0) {
-    __threadfence();
-    ticket = atomicAdd(&a.counters[1], 1u);
-  }
-  if (rank != 0) return;
-  __syncthreads();
-  if (ticket != (unsigned)(a.rows - 1)) return;
-  if (a.loss) {
-    __threadfence();
-    double t = 0.0;
-    for (int64_t i = tid; i < a.rows; i += NT) t += (double)__ldcg(a.row_loss + i);
-    t = warp_sum(t);
-    __shared__ double shd[NW];
-    if (lane == 0) shd[w] = t;
-    __syncthreads();
-    if (tid == 0) {
-      t = 0.0;
-      for (int i = 0; i < NW; ++i) t += shd[i];
-      a.loss[0] = (float)(t / (double)div);
+    if (const unsigned listed = mark_of[(i - head) / V + 1]) {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (listed >> j & 1u) o[j] = grad(i + j);
     }
+    if (add_to) {
+      ld_vec<V>(dst + i, v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) o[j] += v[j];
+    }
+    st_vec<V>(dst + i, o);
   }
+  if (end >= 0) from_f32(dst + end, (add_to ? to_f32(dst[end]) : 0.f) + grad(end));
+}
+
+// The mean, in double, and the counter cleared for the next call.
+__global__ void __launch_bounds__(1024) distill_mean_kernel(DistillArgs a) {
+  __shared__ double sh[32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  double t = 0.0;
+  if (a.loss)
+    for (int64_t i = threadIdx.x; i < a.rows; i += 1024) t += (double)a.row_loss[i];
+  t = warp_sum(t);
+  if (lane == 0) sh[w] = t;
   __syncthreads();
-  if (tid == 0) a.counters[0] = a.counters[1] = 0u;
+  if (threadIdx.x == 0) {
+    t = 0.0;
+    for (int i = 0; i < 32; ++i) t += sh[i];
+    const float div = a.divisor > 0.f ? a.divisor : fmaxf(1.f, (float)a.counters[0]);
+    if (a.loss) a.loss[0] = (float)(t / (double)div);
+    a.counters[0] = 0u;
+  }
 }
 
 // ------------------------------------------------------------- host side ---
@@ -420,10 +412,10 @@ int cluster_for(int64_t row_bytes) {
 
 template <typename T, int NT>
 int launch(const DistillArgs& a, int cluster, cudaStream_t st) {
-  const size_t smem = (size_t)a.top * 16 + (size_t)((a.seg + 31) / 32) * 4 + 16 +
+  const size_t smem = (size_t)a.top * 16 + (size_t)mark_words(a.seg, 16 / sizeof(T)) * 4 + 16 +
                       (size_t)a.seg * sizeof(T) + 16;
-  auto kern = distill_kernel<T, NT>;
-  TL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  constexpr auto kern = distill_kernel<T, NT>;
+  TL_TRY((allow_smem<kern, kSmemMost>()));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.rows * cluster));
   cfg.blockDim = dim3(NT);
@@ -451,8 +443,15 @@ int run(DistillArgs a, cudaStream_t st) {
   // segments start at multiples of 32 classes: 16-byte aligned in an aligned row
   a.seg = ((a.classes + cluster - 1) / cluster + 31) / 32 * 32;
   static_assert(32 % V == 0, "aligned segments");
-  if (a.seg <= 2048) return launch<T, 128>(a, cluster, st);
-  return launch<T, 256>(a, cluster, st);
+  if (a.seg <= 2048)
+    TL_TRY((launch<T, 128>(a, cluster, st)));
+  else
+    TL_TRY((launch<T, 256>(a, cluster, st)));
+  if (a.loss || a.divisor == 0.f) {
+    distill_mean_kernel<<<1, 1024, 0, st>>>(a);
+    TL_TRY(after_launch());
+  }
+  return TL_OK;
 }
 
 int check(int dtype, const DistillArgs& a, int64_t top) {

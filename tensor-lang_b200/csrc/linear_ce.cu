@@ -718,8 +718,8 @@ bool mn_major(CUtensorMap* m, const Planes& x) {
 template <int TA, int TB, int EPI>
 int launch_tiles(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c, const TileParams& p,
                  cudaStream_t st) {
-  auto kern = vocab_tile_kernel<TA, TB, EPI>;
-  TL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
+  constexpr auto kern = vocab_tile_kernel<TA, TB, EPI>;
+  TL_TRY((allow_smem<kern, SMEM_BYTES>()));
   const int64_t tiles = (int64_t)p.splits * ((p.M + 255) / 256) * ((p.N + 255) / 256);
   if (tiles > INT32_MAX / 2) return TL_ERR_UNSUPPORTED;
   const int64_t clusters = std::min<int64_t>(tiles, std::max(1, sm_count() / 2));

@@ -4,6 +4,8 @@
 
 #include <cuda_bf16.h>
 
+#include <atomic>
+
 #include "tl_common.cuh"
 
 namespace tl {
@@ -77,6 +79,19 @@ __device__ __forceinline__ int64_t class_index(const void* p, int type, int64_t 
   return (v >= 0 && v < n) ? v : -1;
 }
 
+// Lets a kernel be launched with up to `bytes` of dynamic shared memory on the
+// current device: once per kernel and device, since the call costs as much as a
+// launch.  (A race of two first calls sets the same value twice.)
+template <auto Kern, int Bytes>
+int allow_smem() {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  TL_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return TL_OK;
+  TL_CUDA_TRY(cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Bytes));
+  if (dev < 64) done.fetch_or(1ull << dev);
+  return TL_OK;
+}
 inline bool aligned_to(const void* p, size_t n) { return ((uintptr_t)p % n) == 0; }
 inline size_t elem_bytes(int dtype) { return dtype == TL_BF16 ? 2 : 4; }
 inline bool dtype_ok(int dtype) { return dtype == TL_F32 || dtype == TL_BF16; }

@@ -684,6 +684,7 @@ __global__ void __launch_bounds__(kLong) residual_norm_bwd_long_kernel(NormArgs 
 
 // ------------------------------------------------------------- host side ---
 constexpr int64_t kMaxCols = 8192;    // of the register kernels
+constexpr int kSmemMost = 226 << 10;  // dynamic, beside the sums' few hundred bytes
 constexpr int64_t kSmem = 216 << 10;  // of an SM, for weights and rows on their way
 
 // Elements a thread holds: 16 bf16, or 8 float32, whose rows and weights on
@@ -731,12 +732,13 @@ Shape launch_shape(int64_t rows, int nt, int64_t most_threads, int64_t row_bytes
   return q;
 }
 
-template <typename K>
-int launch_rows(K kern, const NormArgs& a, Shape q, int nt, int64_t row_bytes, int64_t weight_bytes,
+template <auto Kern>
+int launch_rows(const NormArgs& a, Shape q, int nt, int64_t row_bytes, int64_t weight_bytes,
                 cudaStream_t st) {
   const size_t smem = (size_t)(weight_bytes + q.depth * row_bytes);
-  TL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  kern<<<(unsigned)q.grid, nt, smem, st>>>(a, q.depth);
+  if (smem > kSmemMost) return TL_ERR_UNSUPPORTED;
+  TL_TRY((allow_smem<Kern, kSmemMost>()));
+  Kern<<<(unsigned)q.grid, nt, smem, st>>>(a, q.depth);
   return after_launch();
 }
 
@@ -749,8 +751,8 @@ int forward(const NormArgs& a, int kind, cudaStream_t st) {
     const int64_t row = A::kStaged ? (a.gate_mode == TL_GATE_FULL ? 3 : 2) * A::kArray : 16;
     const Shape q = launch_shape(a.rows, NT, 1024, row, w, INT32_MAX);
     return kind == TL_NORM_LAYER
-               ? launch_rows(residual_norm_kernel<T, NT, VEC, NV, true>, a, q, NT, row, w, st)
-               : launch_rows(residual_norm_kernel<T, NT, VEC, NV, false>, a, q, NT, row, w, st);
+               ? launch_rows<residual_norm_kernel<T, NT, VEC, NV, true>>(a, q, NT, row, w, st)
+               : launch_rows<residual_norm_kernel<T, NT, VEC, NV, false>>(a, q, NT, row, w, st);
   });
 }
 
@@ -766,8 +768,8 @@ int backward(const NormArgs& a, int kind, cudaStream_t st, int64_t* grid) {
     const Shape q = launch_shape(a.rows, NT, 512, row, w, bwd_blocks(a.rows, a.cols));
     *grid = q.grid;
     return kind == TL_NORM_LAYER
-               ? launch_rows(residual_norm_bwd_kernel<T, NT, VEC, NV, true>, a, q, NT, row, w, st)
-               : launch_rows(residual_norm_bwd_kernel<T, NT, VEC, NV, false>, a, q, NT, row, w, st);
+               ? launch_rows<residual_norm_bwd_kernel<T, NT, VEC, NV, true>>(a, q, NT, row, w, st)
+               : launch_rows<residual_norm_bwd_kernel<T, NT, VEC, NV, false>>(a, q, NT, row, w, st);
   });
 }
 
