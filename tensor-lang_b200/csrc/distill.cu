@@ -101,9 +101,34 @@ __device__ __forceinline__ int entry(const DistillArgs& a, int64_t r, int k, flo
   return t == -INFINITY ? -1 : (int)c;
 }
 
+// the larger of m and 16 bytes of elements
+__device__ __forceinline__ float max_vec(const float* p, float m) {
+  const float4 q = *reinterpret_cast<const float4*>(p);
+  return fmaxf(fmaxf(fmaxf(m, q.x), fmaxf(q.y, q.z)), q.w);
+}
+__device__ __forceinline__ float max_vec(const __nv_bfloat16* p, float m) {
+  const uint4 q = *reinterpret_cast<const uint4*>(p);
+  auto b2 = [](const uint32_t& w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+  const __nv_bfloat162 a = __hmax2(__hmax2(b2(q.x), b2(q.y)), __hmax2(b2(q.z), b2(q.w)));
+  return fmaxf(fmaxf(m, __low2float(a)), __high2float(a));
+}
+// sum and maximum of the first N lanes' values, in every lane
+template <int N>
+__device__ __forceinline__ float few_sum(float v) {
+#pragma unroll
+  for (int o = N / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return __shfl_sync(0xffffffffu, v, 0);
+}
+template <int N>
+__device__ __forceinline__ float few_max(float v) {
+#pragma unroll
+  for (int o = N / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return __shfl_sync(0xffffffffu, v, 0);
+}
+
 // Words of the marks of a segment: a byte per vector, one before the middle and
 // one behind it besides.
-__host__ __device__ constexpr int mark_words(int64_t seg, int vec) { return (int)((seg / vec + 2 + 3) / 4); }
+__host__ __device__ constexpr int mark_words(int seg, int vec) { return (seg / vec + 2 + 3) / 4; }
 
 // Rows with a valid entry, one warp per row.
 template <typename T>
@@ -126,16 +151,18 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   constexpr int V = 16 / sizeof(T), NW = NT / 32;
   extern __shared__ __align__(16) unsigned char smem[];
   // [list: class, q, first entry's q sum, its z] [marks of the listed cells] [segment]
+  // (offsets from the array, not pointer casts: the compiler keeps to shared
+  // memory instructions)
   int* li = reinterpret_cast<int*>(smem);
-  float* lq = reinterpret_cast<float*>(li + a.top);
-  float* lsum = lq + a.top;
-  float* lz = lsum + a.top;
+  float* lq = reinterpret_cast<float*>(smem + 4 * a.top);
+  float* lsum = reinterpret_cast<float*>(smem + 8 * a.top);
+  float* lz = reinterpret_cast<float*>(smem + 12 * a.top);
   // per vector of V cells a byte with the listed ones' bits; the vectors are
   // those of the middle (below), the cells before it are vector 0
-  uint32_t* marks = reinterpret_cast<uint32_t*>(lz + a.top);
-  const int nmarks = mark_words(a.seg, V);
-  unsigned char* cells = reinterpret_cast<unsigned char*>(
-      ((uintptr_t)(marks + nmarks) + 15) & ~(uintptr_t)15);
+  unsigned char* mark_of = smem + 16 * a.top;
+  uint32_t* marks = reinterpret_cast<uint32_t*>(mark_of);
+  const int nmarks = mark_words((int)a.seg, V);
+  T* cells = reinterpret_cast<T*>(smem + ((16 * a.top + 4 * nmarks + 15) & ~15));
   __shared__ float peer[4][kMaxCluster];
   __shared__ float sh[3][NW];
 
@@ -148,7 +175,7 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   // the segment sits in shared memory at the offset within 16 bytes that it
   // has in memory, so that its middle is copied 16 bytes at a time
   const int phase = (int)(((uintptr_t)src & 15) / sizeof(T));
-  T* cell = reinterpret_cast<T*>(cells) + phase;
+  T* cell = cells + phase;
   const int head = min(n, phase ? V - phase : 0), mid = (n - head) / V * V;
   if (size > 1) cluster_arrive();  // every CTA of the cluster runs: waited for before the exchange
 
@@ -186,9 +213,7 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   tm = warp_max(tm);
   if (lane == 0) sh[0][w] = tm;
   const bool some = __syncthreads_or(tm > -INFINITY || tnan);
-  tm = sh[0][0];
-#pragma unroll
-  for (int i = 1; i < NW; ++i) tm = fmaxf(tm, sh[0][i]);
+  tm = few_max<NW>(lane < NW ? sh[0][lane] : -INFINITY);
   float tsum = 0.f, tdot = 0.f;
   for (int k = tid; k < a.top; k += NT) {
     float e = 0.f;
@@ -207,40 +232,45 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
     sh[2][w] = tdot;
   }
   __syncthreads();
-  tsum = tdot = 0.f;
-#pragma unroll
-  for (int i = 0; i < NW; ++i) {
-    tsum += sh[1][i];
-    tdot += sh[2][i];
-  }
+  tsum = few_sum<NW>(lane < NW ? sh[1][lane] : 0.f);
   const float inv_t = some ? 1.f / tsum : 0.f;
-  // the q of equal classes added, for the first of them (the others: -1)
+  // listed cells are marked; where a class is met again (its bit is there
+  // already), the q of equal classes are added, in list order, for the first
+  // of them (the others: -1)
+  bool again = false;
   for (int k = tid; k < a.top; k += NT) {
     const int c = li[k];
     if (c < c0 || c >= c0 + n) continue;
-    float sum = 0.f;
-    bool first = true;
-    for (int j = 0; j < a.top; ++j)
-      if (li[j] == c) {
-        first = first && j >= k;
-        sum += lq[j];
-      }
-    lsum[k] = first ? sum * inv_t : -1.f;
+    const int at = c - (int)c0 - head + V;  // byte at / V, bit at % V
+    const uint32_t bit = 1u << (8 * (at / V & 3) + at % V);
+    again |= (atomicOr(&marks[at / V >> 2], bit) & bit) != 0;
+    lsum[k] = lq[k] * inv_t;
+  }
+  if (__syncthreads_or(again)) {
+    for (int k = tid; k < a.top; k += NT) {
+      const int c = li[k];
+      if (c < c0 || c >= c0 + n) continue;
+      float sum = 0.f;
+      bool first = true;
+      for (int j = 0; j < a.top; ++j)
+        if (li[j] == c) {
+          first = first && j >= k;
+          sum += lq[j];
+        }
+      lsum[k] = first ? sum * inv_t : -1.f;
+    }
   }
 
   // the segment: each thread's maximum and sum of exponentials, then the warp's
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   float m = end_z, s;
-  for (int i = head + tid * V; i < head + mid; i += NT * V) {
-    float v[V];
-    ld_vec<V>(cell + i, v);
-#pragma unroll
-    for (int j = 0; j < V; ++j) m = fmaxf(m, v[j]);
-  }
+#pragma unroll 4
+  for (int i = head + tid * V; i < head + mid; i += NT * V) m = max_vec(cell + i, m);
   {
     const float base = m == -INFINITY ? 0.f : m;
     const float2 nb = make_float2(-base, -base), kk = make_float2(k2, k2);
     float2 t = make_float2(end >= 0 ? exp2_fast((end_z - base) * k2) : 0.f, 0.f);
+#pragma unroll 2
     for (int i = head + tid * V; i < head + mid; i += NT * V) {
       float v[V];
       ld_vec<V>(cell + i, v);
@@ -255,8 +285,7 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
     s = warp_sum(s * exp2_fast((m - wbase) * k2));
     m = wm;
   }
-  __syncthreads();  // sh's readers are done; every cell, mark and list entry is there
-  if (lane == 0) {
+  if (lane == 0) {  // sh's readers are past the last barrier
     sh[0][w] = m;
     sh[1][w] = s;
   }
@@ -264,8 +293,8 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   if (w == 0) {
     m = lane < NW ? sh[0][lane] : -INFINITY;
     s = lane < NW ? sh[1][lane] : 0.f;
-    const float sm = warp_max(m), base = sm == -INFINITY ? 0.f : sm;
-    s = warp_sum(s * exp2_fast((m - base) * k2));
+    const float sm = few_max<NW>(m), base = sm == -INFINITY ? 0.f : sm;
+    s = few_sum<NW>(s * exp2_fast((m - base) * k2));
     // the list's entries in this segment: the sums of q and of q (z - m) / tau
     // (differences to the maximum: logits of the type's lowest value cancel
     // exactly); their cells make way for the entry's number
@@ -285,8 +314,6 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
     for (int k = lane; k < a.top; k += 32) {
       const int c = li[k] - (int)c0;
       if (li[k] < 0 || c < 0 || c >= n || lsum[k] < 0.f) continue;
-      const int at = c - head + V;  // byte at / V, bit at % V
-      atomicOr(&marks[at / V >> 2], 1u << (8 * (at / V & 3) + at % V));
       if constexpr (sizeof(T) == 2)
         reinterpret_cast<uint16_t*>(cell)[c] = (uint16_t)k;
       else
@@ -309,15 +336,16 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   } else {
     __syncthreads();
   }
-  m = peer[0][0];
-  for (uint32_t i = 1; i < size; ++i) m = fmaxf(m, peer[0][i]);
-  const float base = m == -INFINITY ? 0.f : m;
+  const bool there = lane < (int)size;
+  const float pm = there ? peer[0][lane] : -INFINITY, ps = there ? peer[1][lane] : 0.f;
+  m = few_max<kMaxCluster>(pm);
+  const float base = m == -INFINITY ? 0.f : m, pb = pm == -INFINITY ? 0.f : pm;
+  s = few_sum<kMaxCluster>(ps == 0.f ? 0.f : ps * exp2_fast((pb - base) * k2));
   float dot = 0.f;
-  s = 0.f;
-  for (uint32_t i = 0; i < size; ++i) {
-    const float mi = peer[0][i] == -INFINITY ? 0.f : peer[0][i];
-    s += peer[1][i] == 0.f ? 0.f : peer[1][i] * exp2_fast((mi - base) * k2);
-    dot += peer[3][i] == 0.f ? 0.f : peer[2][i] + peer[3][i] * ((mi - base) * inv_tau);
+  if (rank == 0 && w == 0) {
+    const float pq = there ? peer[3][lane] : 0.f;
+    dot = few_sum<kMaxCluster>(pq == 0.f ? 0.f : peer[2][lane] + pq * ((pb - base) * inv_tau));
+    tdot = few_sum<NW>(lane < NW ? sh[2][lane] : 0.f);
   }
   if (rank == 0 && tid == 0) {
     const float log_s = logf(s);  // a row of -inf: -inf
@@ -358,7 +386,6 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   }
   const float2 nb = make_float2(-base, -base), kk = make_float2(k2, k2);
   const float2 cs = make_float2(cf * inv_s, cf * inv_s);
-  const unsigned char* mark_of = reinterpret_cast<const unsigned char*>(marks);
   for (int i = head + tid * V; i < head + mid; i += NT * V) {
     float v[V], o[V];
     ld_vec<V>(cell + i, v);
@@ -412,7 +439,7 @@ int cluster_for(int64_t row_bytes) {
 
 template <typename T, int NT>
 int launch(const DistillArgs& a, int cluster, cudaStream_t st) {
-  const size_t smem = (size_t)a.top * 16 + (size_t)mark_words(a.seg, 16 / sizeof(T)) * 4 + 16 +
+  const size_t smem = (size_t)a.top * 16 + (size_t)mark_words((int)a.seg, 16 / sizeof(T)) * 4 + 16 +
                       (size_t)a.seg * sizeof(T) + 16;
   constexpr auto kern = distill_kernel<T, NT>;
   TL_TRY((allow_smem<kern, kSmemMost>()));
