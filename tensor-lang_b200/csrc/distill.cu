@@ -14,8 +14,8 @@
 // segment in with asynchronous copies, takes the segment's maximum and sum of
 // exponentials from shared memory, exchanges four numbers (maximum, sum,
 // the list's sums of q and q z) with the other CTAs through distributed shared memory,
-// and writes its segment's gradient from the same copy.  Segments are about
-// 32 KB, so several CTAs share an SM and one's copy overlaps another's
+// and writes its segment's gradient from the same copy.  Segments are 32 to
+// 64 KB, so several CTAs share an SM and one's copy overlaps another's
 // exponentials and stores.
 //
 // Listed classes: the gradient there is p - q with the q of equal indices
@@ -33,7 +33,7 @@ namespace tl {
 namespace {
 
 constexpr int kMaxTop = 1024;
-constexpr int64_t kSegTarget = 32 << 10;    // bytes of a row a CTA aims at
+constexpr int64_t kSegTarget = 16384;       // classes of a row a CTA aims at
 constexpr int64_t kSegMax = 192 << 10;      // and the most it takes
 constexpr int kMaxCluster = 8;
 constexpr int kSmemMost = 226 << 10;        // dynamic, beside a few hundred bytes
@@ -49,6 +49,7 @@ struct DistillArgs {
   int64_t ldi;
   int index_type;
   float temperature, divisor;
+  float k2, inv_tau;    // exp(v / temperature) = 2^(v k2); 1 / temperature
   const float* upstream;
   float* loss;
   float* row_loss;      // the caller's, or scratch when only the mean is wanted
@@ -56,7 +57,7 @@ struct DistillArgs {
   void* dz;
   int64_t lddz;
   int accumulate;
-  unsigned* counters;   // [0] rows that count, 0 between calls
+  unsigned* counters;   // [0] rows that count, [1] rows done; 0 between calls
   int64_t seg;          // classes per CTA
 };
 
@@ -75,6 +76,9 @@ __device__ __forceinline__ uint32_t saddr(const void* p) {
 }
 __device__ __forceinline__ void cluster_arrive() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -130,23 +134,30 @@ __device__ __forceinline__ float few_max(float v) {
 // one behind it besides.
 __host__ __device__ constexpr int mark_words(int seg, int vec) { return (seg / vec + 2 + 3) / 4; }
 
+// Whether row r has a valid entry (asked by a whole warp).
+template <typename T>
+__device__ __forceinline__ bool row_counts(const DistillArgs& a, int64_t r) {
+  const int lane = threadIdx.x & 31;
+  bool any = false;
+  for (int k0 = 0; k0 < a.top && !any; k0 += 32) {
+    float t;
+    any = __any_sync(0xffffffffu, k0 + lane < a.top && entry<T>(a, r, k0 + lane, t) >= 0);
+  }
+  return any;
+}
+
 // Rows with a valid entry, one warp per row.
 template <typename T>
 __global__ void __launch_bounds__(256) distill_count_kernel(DistillArgs a) {
   const int lane = threadIdx.x & 31;
   unsigned n = 0;
-  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < a.rows; r += 8LL * gridDim.x) {
-    bool any = false;
-    for (int k0 = 0; k0 < a.top && !any; k0 += 32) {
-      float t;
-      any = __any_sync(0xffffffffu, k0 + lane < a.top && entry<T>(a, r, k0 + lane, t) >= 0);
-    }
-    n += any;
-  }
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < a.rows; r += 8LL * gridDim.x)
+    n += row_counts<T>(a, r);
   if (lane == 0 && n) atomicAdd(&a.counters[0], n);  // a whole number: any order
 }
 
-template <typename T, int NT>
+// ALONE: few rows; every CTA counts them itself and the last row's adds up.
+template <typename T, int NT, bool ALONE>
 __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   constexpr int V = 16 / sizeof(T), NW = NT / 32;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -164,7 +175,8 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   const int nmarks = mark_words((int)a.seg, V);
   T* cells = reinterpret_cast<T*>(smem + ((16 * a.top + 4 * nmarks + 15) & ~15));
   __shared__ float peer[4][kMaxCluster];
-  __shared__ float sh[3][NW];
+  __shared__ float sh[2][NW], lsh[5][NW], list[3];
+  __shared__ int few[NW];
 
   const uint32_t rank = cluster_rank(), size = cluster_size();
   const int64_t r = blockIdx.x / size;
@@ -177,7 +189,7 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   const int phase = (int)(((uintptr_t)src & 15) / sizeof(T));
   T* cell = cells + phase;
   const int head = min(n, phase ? V - phase : 0), mid = (n - head) / V * V;
-  if (size > 1) cluster_arrive();  // every CTA of the cluster runs: waited for before the exchange
+  if (size > 1) cluster_arrive_relaxed();  // every CTA of the cluster runs: waited for before the exchange
 
   // each thread brings in what it reads in the first pass, so waiting for its
   // own copies is enough; the row's ends, outside the 16-byte copies, are one
@@ -194,70 +206,101 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   }
   for (int i = tid; i < nmarks; i += NT) marks[i] = 0u;
   const float up = a.upstream ? *a.upstream : 1.f;
-  const float div = a.divisor > 0.f ? a.divisor : fmaxf(1.f, (float)a.counters[0]);
+  const float k2 = a.k2, inv_tau = a.inv_tau;
+  float div = a.divisor;
+  if (ALONE && a.divisor == 0.f) {
+    int counted = 0;
+    for (int64_t i = w; i < a.rows; i += NW) counted += row_counts<T>(a, i);
+    if (lane == 0) few[w] = counted;
+    __syncthreads();
+    counted = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) counted += few[i];
+    div = fmaxf(1.f, (float)counted);
+  } else {
+    if (a.divisor == 0.f) div = fmaxf(1.f, (float)a.counters[0]);
+    __syncthreads();
+  }
 
-  // while they are on their way, the teacher's list: q = softmax(t / tau)
-  const float k2 = 1.4426950408889634f / a.temperature;  // exp(v / tau) = 2^(v k2)
-  const float inv_tau = 1.f / a.temperature;
-  float tm = -INFINITY;
-  bool tnan = false;
-  for (int k = tid; k < a.top; k += NT) {
-    float t;
-    li[k] = entry<T>(a, r, k, t);
-    lq[k] = t;
-    if (li[k] >= 0) {
-      tm = fmaxf(tm, t);
-      tnan |= t != t;
+  // while they are on their way (and while the other warps work on the
+  // segment), the first warps prepare the teacher's list: q = softmax(t / tau)
+  const int list_warps = min(NW, (a.top + 31) / 32), LT = 32 * list_warps;
+  if (w < list_warps) {
+    auto list_sync = [&] { asm volatile("bar.sync 1, %0;" ::"r"(LT) : "memory"); };
+    float tm = -INFINITY, tnan = 0.f;
+    for (int k = tid; k < a.top; k += LT) {
+      float t;
+      li[k] = entry<T>(a, r, k, t);
+      lq[k] = t;
+      if (li[k] >= 0) {
+        tm = fmaxf(tm, t);
+        if (t != t) tnan = 1.f;
+      }
     }
-  }
-  tm = warp_max(tm);
-  if (lane == 0) sh[0][w] = tm;
-  const bool some = __syncthreads_or(tm > -INFINITY || tnan);
-  tm = few_max<NW>(lane < NW ? sh[0][lane] : -INFINITY);
-  float tsum = 0.f, tdot = 0.f;
-  for (int k = tid; k < a.top; k += NT) {
-    float e = 0.f;
-    if (li[k] >= 0) {
-      const float d = (lq[k] - tm) * inv_tau;
-      e = expf(d);
-      tsum += e;
-      tdot += e > 0.f ? e * d : 0.f;
+    tm = warp_max(tm);
+    tnan = warp_max(tnan);
+    if (lane == 0) {
+      lsh[0][w] = tm;
+      lsh[1][w] = tnan;
     }
-    lq[k] = e;  // q times the sum
-  }
-  tsum = warp_sum(tsum);
-  tdot = warp_sum(tdot);
-  if (lane == 0) {
-    sh[1][w] = tsum;
-    sh[2][w] = tdot;
-  }
-  __syncthreads();
-  tsum = few_sum<NW>(lane < NW ? sh[1][lane] : 0.f);
-  const float inv_t = some ? 1.f / tsum : 0.f;
-  // listed cells are marked; where a class is met again (its bit is there
-  // already), the q of equal classes are added, in list order, for the first
-  // of them (the others: -1)
-  bool again = false;
-  for (int k = tid; k < a.top; k += NT) {
-    const int c = li[k];
-    if (c < c0 || c >= c0 + n) continue;
-    const int at = c - (int)c0 - head + V;  // byte at / V, bit at % V
-    const uint32_t bit = 1u << (8 * (at / V & 3) + at % V);
-    again |= (atomicOr(&marks[at / V >> 2], bit) & bit) != 0;
-    lsum[k] = lq[k] * inv_t;
-  }
-  if (__syncthreads_or(again)) {
-    for (int k = tid; k < a.top; k += NT) {
+    list_sync();
+    tm = few_max<NW>(lane < list_warps ? lsh[0][lane] : -INFINITY);
+    tnan = few_max<NW>(lane < list_warps ? lsh[1][lane] : 0.f);
+    float tsum = 0.f, tdot = 0.f;
+    for (int k = tid; k < a.top; k += LT) {
+      float e = 0.f;
+      if (li[k] >= 0) {
+        const float d = (lq[k] - tm) * inv_tau;
+        e = expf(d);
+        tsum += e;
+        tdot += e > 0.f ? e * d : 0.f;
+      }
+      lq[k] = e;  // q times the sum
+    }
+    tsum = warp_sum(tsum);
+    tdot = warp_sum(tdot);
+    if (lane == 0) {
+      lsh[2][w] = tsum;
+      lsh[3][w] = tdot;
+    }
+    // listed cells are marked; where a class is met again (its bit is there
+    // already), the q of equal classes are added, in list order, for the first
+    // of them (the others: -1)
+    bool again = false;
+    for (int k = tid; k < a.top; k += LT) {
       const int c = li[k];
       if (c < c0 || c >= c0 + n) continue;
-      float sum = 0.f;
+      const int at = c - (int)c0 - head + V;  // byte at / V, bit at % V
+      const uint32_t bit = 1u << (8 * (at / V & 3) + at % V);
+      again |= (atomicOr(&marks[at / V >> 2], bit) & bit) != 0;
+    }
+    again = __any_sync(0xffffffffu, again);
+    if (lane == 0) lsh[4][w] = again ? 1.f : 0.f;
+    list_sync();
+    tsum = few_sum<NW>(lane < list_warps ? lsh[2][lane] : 0.f);
+    tdot = few_sum<NW>(lane < list_warps ? lsh[3][lane] : 0.f);
+    again = few_max<NW>(lane < list_warps ? lsh[4][lane] : 0.f) > 0.f;
+    const bool some = tm > -INFINITY || tnan > 0.f;
+    const float inv_t = some ? 1.f / tsum : 0.f;
+    for (int k = tid; k < a.top; k += LT) {
+      const int c = li[k];
+      if (c < c0 || c >= c0 + n) continue;
+      float sum = lq[k];
       bool first = true;
-      for (int j = 0; j < a.top; ++j)
-        if (li[j] == c) {
-          first = first && j >= k;
-          sum += lq[j];
-        }
+      if (again) {
+        sum = 0.f;
+        for (int j = 0; j < a.top; ++j)
+          if (li[j] == c) {
+            first = first && j >= k;
+            sum += lq[j];
+          }
+      }
       lsum[k] = first ? sum * inv_t : -1.f;
+    }
+    if (tid == 0) {
+      list[0] = some ? 1.f : 0.f;
+      list[1] = inv_t;
+      list[2] = some ? tdot * inv_t - logf(tsum) : 0.f;  // sum q log q = sum e d / S - log S
     }
   }
 
@@ -285,12 +328,14 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
     s = warp_sum(s * exp2_fast((m - wbase) * k2));
     m = wm;
   }
-  if (lane == 0) {  // sh's readers are past the last barrier
+  if (lane == 0) {
     sh[0][w] = m;
     sh[1][w] = s;
   }
   __syncthreads();
+  const bool some = list[0] > 0.f;
   if (w == 0) {
+    const float inv_t = list[1];
     m = lane < NW ? sh[0][lane] : -INFINITY;
     s = lane < NW ? sh[1][lane] : 0.f;
     const float sm = few_max<NW>(m), base = sm == -INFINITY ? 0.f : sm;
@@ -327,11 +372,14 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
       st_peer(&peer[3][rank], lane, qs);
     }
     __syncwarp();
+    if (size > 1) cluster_arrive();
   } else if (size > 1) {
+    // nothing of these warps is for other CTAs, and their own has them since
+    // the last barrier
     cluster_wait();
+    cluster_arrive_relaxed();
   }
   if (size > 1) {
-    cluster_arrive();
     cluster_wait();
   } else {
     __syncthreads();
@@ -345,23 +393,28 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   if (rank == 0 && w == 0) {
     const float pq = there ? peer[3][lane] : 0.f;
     dot = few_sum<kMaxCluster>(pq == 0.f ? 0.f : peer[2][lane] + pq * ((pb - base) * inv_tau));
-    tdot = few_sum<NW>(lane < NW ? sh[2][lane] : 0.f);
   }
   if (rank == 0 && tid == 0) {
     const float log_s = logf(s);  // a row of -inf: -inf
     if (a.lse) a.lse[r] = m * inv_tau + log_s;
     float l = 0.f;
-    if (some) {
-      // sum q log q = sum e d / S - log S
-      const float qlogq = tdot * inv_t - logf(tsum);
-      l = dot == -INFINITY ? INFINITY : a.temperature * a.temperature * (qlogq + (log_s - dot));
-    }
+    if (some) l = dot == -INFINITY ? INFINITY : a.temperature * a.temperature * (list[2] + (log_s - dot));
     if (a.row_loss) a.row_loss[r] = l;
+    if (ALONE && a.loss) {  // the last row to get here adds them up, in order
+      __threadfence();
+      if (atomicAdd(&a.counters[1], 1u) == (unsigned)(a.rows - 1)) {
+        __threadfence();
+        double t = 0.0;
+        for (int64_t i = 0; i < a.rows; ++i) t += (double)__ldcg(a.row_loss + i);
+        a.loss[0] = (float)(t / (double)div);
+        a.counters[1] = 0u;
+      }
+    }
   }
   if (!a.dz) return;
-  const float cf = some ? a.temperature * up / div : 0.f;
+  const float cf = some ? __fdividef(a.temperature * up, div) : 0.f;
   // p = exp((z - m) / tau) / s: nearer than exp(z / tau - lse), whose lse is rounded
-  const float inv_s = s > 0.f || s != s ? 1.f / s : 0.f;
+  const float inv_s = s > 0.f || s != s ? __fdividef(1.f, s) : 0.f;
   auto grad = [&](int c) {  // of cell c
     const int at = c - head + V;
     float z = to_f32(cell[c]), q = 0.f;
@@ -431,17 +484,23 @@ __global__ void __launch_bounds__(1024) distill_mean_kernel(DistillArgs a) {
 }
 
 // ------------------------------------------------------------- host side ---
-int cluster_for(int64_t row_bytes) {
+// About 16384 classes a CTA: 32 KB of bf16 (six CTAs an SM) or 64 KB of float32.
+// Measured on 8192 x 131072 bf16: 32 KB 1073 us, 64 KB 1161 us; on 1537 x 50021
+// float32: 32 KB 164 us, 64 KB 150 us.
+// Few rows are spread wider: 8 x 32000 float32 takes 7.5 us in 4096 classes a
+// CTA, 8.9 us in 16384.
+int cluster_for(int64_t rows, int64_t classes) {
+  const int64_t target = rows * kMaxCluster <= 2 * sm_count() ? kSegTarget / 4 : kSegTarget;
   int c = 1;
-  while (c < kMaxCluster && row_bytes > c * kSegTarget) c *= 2;
+  while (c < kMaxCluster && classes > c * target) c *= 2;
   return c;
 }
 
-template <typename T, int NT>
+template <typename T, int NT, bool ALONE>
 int launch(const DistillArgs& a, int cluster, cudaStream_t st) {
   const size_t smem = (size_t)a.top * 16 + (size_t)mark_words((int)a.seg, 16 / sizeof(T)) * 4 + 16 +
                       (size_t)a.seg * sizeof(T) + 16;
-  constexpr auto kern = distill_kernel<T, NT>;
+  constexpr auto kern = distill_kernel<T, NT, ALONE>;
   TL_TRY((allow_smem<kern, kSmemMost>()));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.rows * cluster));
@@ -460,20 +519,24 @@ int launch(const DistillArgs& a, int cluster, cudaStream_t st) {
 
 template <typename T>
 int run(DistillArgs a, cudaStream_t st) {
-  if (a.divisor == 0.f) {
+  // one launch instead of three: 8 x 32000 float32 takes 10.9 us a call instead of 17.4
+  const bool alone = a.rows <= 16 && a.rows * a.top <= 4096;
+  if (a.divisor == 0.f && !alone) {
     const int64_t blocks = std::min<int64_t>((a.rows + 7) / 8, 4LL * sm_count());
     distill_count_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(a);
     TL_TRY(after_launch());
   }
   constexpr int64_t V = 16 / sizeof(T);
-  const int cluster = cluster_for(a.classes * (int64_t)sizeof(T));
+  const int cluster = cluster_for(a.rows, a.classes);
   // segments start at multiples of 32 classes: 16-byte aligned in an aligned row
   a.seg = ((a.classes + cluster - 1) / cluster + 31) / 32 * 32;
   static_assert(32 % V == 0, "aligned segments");
+  if (alone)
+    return a.seg <= 2048 ? launch<T, 128, true>(a, cluster, st) : launch<T, 256, true>(a, cluster, st);
   if (a.seg <= 2048)
-    TL_TRY((launch<T, 128>(a, cluster, st)));
+    TL_TRY((launch<T, 128, false>(a, cluster, st)));
   else
-    TL_TRY((launch<T, 256>(a, cluster, st)));
+    TL_TRY((launch<T, 256, false>(a, cluster, st)));
   if (a.loss || a.divisor == 0.f) {
     distill_mean_kernel<<<1, 1024, 0, st>>>(a);
     TL_TRY(after_launch());
@@ -518,6 +581,8 @@ int tl_distill_topk(int dtype, int64_t rows, int64_t classes, int64_t top, const
   a.upstream = upstream; a.loss = loss; a.lse = lse; a.dz = dz; a.lddz = lddz;
   a.accumulate = accumulate;
   TL_TRY(tl::check(dtype, a, top));
+  a.k2 = (float)(1.4426950408889634 / (double)temperature);
+  a.inv_tau = (float)(1.0 / (double)temperature);
   if (!loss && !row_loss && !lse && !dz) return TL_ERR_INVALID_ARG;
   if (!scratch || !tl::aligned_to(scratch, 16) || scratch_bytes < tl_distill_topk_scratch_bytes(rows))
     return TL_ERR_INVALID_ARG;
