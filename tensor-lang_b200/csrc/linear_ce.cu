@@ -55,7 +55,8 @@ namespace {
 constexpr int BK = 64;                   // bf16 per stage row: 128 bytes
 constexpr int TILE_BYTES = 128 * BK * 2; // 16 KB: 128 rows of A, or of B, per CTA
 constexpr int NST = 6;
-constexpr int EPI_WARPS = 8;
+constexpr int EPI_WARPS = 8;             // two per quarter of the rows
+constexpr int CW = 128;                  // columns of an epilogue warp
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int STG_TILE = 4096;           // per epilogue warp: 32 rows x 128 bytes
 constexpr int SMEM_BYTES = NST * 2 * TILE_BYTES + EPI_WARPS * STG_TILE + 1024 + 256;
@@ -77,7 +78,9 @@ struct TileParams {
   int splits;     // K split this many ways (kSum)
   // kStats, kGrad
   const float* bias;      // of this piece's columns, or null
-  const int32_t* target;  // [M]: class relative to the whole vocabulary, or -1
+  const void* target;     // [M], of the whole vocabulary
+  int index_type;
+  int64_t classes;
   int col0;               // first class of this piece
   float2* part;           // kStats: [slot][part_ld] (maximum, sum of exp)
   int64_t part_ld;
@@ -190,6 +193,21 @@ __device__ __forceinline__ void store_slab16(const CUtensorMap* map, uint32_t st
   }
 }
 
+// 32 rows (a lane each) x 32 columns of float32 through the warp's staging tile,
+// element (row, j) at j ^ row: no bank conflicts by rows or by columns.  `lane` is
+// hidden from the compiler, which otherwise keeps all 32 addresses in registers
+// across the tiles.
+__device__ __forceinline__ void stage_slab(float* stage, int lane, const float* v) {
+  asm volatile("" : "+r"(lane));
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 32; ++j) stage[lane * 32 + (j ^ lane)] = v[j];
+  __syncwarp();
+}
+__device__ __forceinline__ float staged(const float* stage, int lane, int row) {
+  return stage[row * 32 + (lane ^ row)];
+}
+
 // A: x, g or x^T ...; TA 0: stored [M][K], 1: [K][M].  TB 0: B stored [K][N], 1: [N][K].
 template <int TA, int TB, int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
@@ -236,9 +254,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 
   // The stage ring (it) and the two accumulators (cg) run on across tiles, so
   // the next tile's loads and MMAs overlap this one's epilogue.
-  if (warp == 0) {
-    // ------------------------------------------------------------ producer
-    if (lane == 0) {
+  if (warp < 2) {
+    if (warp == 0 && lane == 0) {
+      // ---------------------------------------------------------- producer
       const uint32_t full0 = mapa_shared(smem_u32(&full[0]), 0);
       bool ok = true;
       uint32_t it = 0;
@@ -276,10 +294,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         }
       }
     }
-    __syncwarp();
-  } else if (warp == 1) {
-    // --------------------------------------------------------- MMA (leader)
-    if (leader && lane == 0) {
+    if (warp == 1 && leader && lane == 0) {
+      // -------------------------------------------------------- MMA (leader)
       bool ok = true;
       uint32_t it = 0, cg = 0;
       for (int g = first; g < tiles && ok; g += step) {
@@ -313,17 +329,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     __syncwarp();
   } else {
     // ----------------------------------------------------------- epilogue
-    const int e = warp - 2, quarter = warp & 3, half = e >> 2;
+    const int e = warp - 2, quarter = warp & 3, group = e >> 2;
     const uint32_t free0 = mapa_shared(smem_u32(&acc_free[0]), 0);
-    const uint32_t tbase = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
-    const uint32_t stg = smem_u32(staging + e * STG_TILE);
-    float v[128];
+    const uint32_t tbase = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(group * CW);
+    float* stage = reinterpret_cast<float*>(staging + e * STG_TILE);
+    const uint32_t stg = smem_u32(stage);
+    float v[CW];
     bool ok = true;
     uint32_t cg = 0;
     for (int g = first; g < tiles && ok; g += step) {
       const Tile t = tile_of(p, g);
 #pragma unroll
-      for (int j = 0; j < 128; ++j) v[j] = 0.f;
+      for (int j = 0; j < CW; ++j) v[j] = 0.f;
       for (int c = 0; c < t.nk; c += p.kc, ++cg) {
         const uint32_t b = cg & 1;
         if (!mbar_wait(smem_u32(&acc_full[b]), (cg >> 1) & 1)) {
@@ -333,7 +350,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         fence_after();
         __syncwarp();
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
+        for (int q = 0; q < CW / 16; ++q) {
           float r[16];
           tmem_ld16(tbase + b * 256 + q * 16, r);
 #pragma unroll
@@ -346,90 +363,88 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       const int r0 = t.m0 + 128 * (int)rank + quarter * 32, row = r0 + lane;
-      const int n0 = t.n0 + half * 128;
-      const int cols = min(128, p.N - n0);  // of this warp; may be <= 0
+      const int n0 = t.n0 + group * CW;
+      const int cols = min(CW, p.N - n0);  // of this warp; may be <= 0
       if (r0 >= p.M || cols <= 0) continue;
       const bool live = row < p.M;
 
       if constexpr (EPI == kStats || EPI == kGrad) {
         if (p.bias) {
 #pragma unroll
-          for (int j = 0; j < 128; ++j)
+          for (int j = 0; j < CW; ++j)
             if (j < cols) v[j] += __ldg(p.bias + n0 + j);
         }
-        const int target = live ? p.target[row] - p.col0 - n0 : -1;  // in this warp's columns
+        const int cls = live ? (int)class_index(p.target, p.index_type, row, p.classes) : -1;
+        const int target = cls < 0 ? -1 : cls - p.col0 - n0;  // in this warp's columns
         if constexpr (EPI == kStats) {
-          if (cols < 128) {
+          if (cols < CW) {
 #pragma unroll
-            for (int j = 0; j < 128; ++j)
+            for (int j = 0; j < CW; ++j)
               if (j >= cols) v[j] = -INFINITY;
           }
           float m = v[0];
 #pragma unroll
-          for (int j = 1; j < 128; ++j) m = fmaxf(m, v[j]);
+          for (int j = 1; j < CW; ++j) m = fmaxf(m, v[j]);
           const float base = m == -INFINITY ? 0.f : m;
           float s = 0.f;
 #pragma unroll
-          for (int j = 0; j < 128; ++j) s += exp_fast(v[j] - base);
+          for (int j = 0; j < CW; ++j) s += exp_fast(v[j] - base);
           if (live) {
-            p.part[(int64_t)(n0 >> 7) * p.part_ld + row] = make_float2(m, s);
+            p.part[(int64_t)(n0 / CW) * p.part_ld + row] = make_float2(m, s);
             if (target >= 0 && target < cols) {
               float z = 0.f;
 #pragma unroll
-              for (int j = 0; j < 128; ++j) z = j == target ? v[j] : z;
+              for (int j = 0; j < CW; ++j) z = j == target ? v[j] : z;
               p.zt[row] = z;
             }
           }
         } else {
           // g = p - onehot; 0 for rows without a target
-          const bool counts = live && p.target[row] >= 0;
-          const float lse = counts ? p.lse[row] : 0.f;
-          // nothing left of the row: p = 0
-          const bool none = lse == -INFINITY;
+          const bool counts = cls >= 0;
+          const float lse = counts ? p.lse[row] : INFINITY;
+          // nothing left of the row: p = 0, as for the rows that do not count
+          const float off = lse == -INFINITY ? INFINITY : lse;
+          float* cs = p.colsum ? p.colsum + (int64_t)(r0 >> 5) * p.N + n0 : nullptr;
+          if (cs && lane == 0) bulk_wait_read();
 #pragma unroll
-          for (int j = 0; j < 128; ++j) {
-            v[j] = counts && !none ? exp_fast(v[j] - lse) : 0.f;
-            if (counts && j == target) v[j] -= 1.f;
-          }
-          if (p.colsum) {  // before g is rounded
-            float* cs = p.colsum + (int64_t)(r0 >> 5) * p.N + n0;
+          for (int sl = 0; sl < CW / 64; ++sl) {  // one slab after the other: registers
+            if (64 * sl >= cols) break;
+            float* u = v + 64 * sl;
 #pragma unroll
-            for (int sl = 0; sl < 4; ++sl) {
+            for (int j = 0; j < 64; ++j) u[j] = exp_fast(u[j] - off);
+            if (!counts) {  // a NaN or infinite logit included
+#pragma unroll
+              for (int j = 0; j < 64; ++j) u[j] = 0.f;
+            }
+            if (target >= 64 * sl && target < min(cols, 64 * sl + 64)) {
+#pragma unroll
+              for (int j = 0; j < 64; ++j) u[j] -= j == target - 64 * sl ? 1.f : 0.f;
+            }
+            if (cs) {  // before g is rounded
               if (lane == 0) bulk_wait_read();
-              __syncwarp();
-              // element (row lane, column j) at j ^ lane: no bank conflicts either way
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                asm volatile("st.shared.f32 [%0], %1;" ::"r"(stg + 4u * (uint32_t)(lane * 32 + (j ^ lane))),
-                             "f"(v[32 * sl + j])
-                             : "memory");
-              __syncwarp();
-              float s = 0.f;
-#pragma unroll
-              for (int r = 0; r < 32; ++r) {
-                float q;
-                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(q)
-                             : "r"(stg + 4u * (uint32_t)(r * 32 + (lane ^ r)))
-                             : "memory");
-                s += q;
+              for (int h = 0; h < 2; ++h) {
+                stage_slab(stage, lane, u + 32 * h);
+                float s = 0.f;
+#pragma unroll 8
+                for (int r = 0; r < 32; ++r) s += staged(stage, lane, r);
+                const int c = 64 * sl + 32 * h + lane;
+                if (c < cols) cs[c] = s;
               }
-              if (32 * sl + lane < cols) cs[32 * sl + lane] = s;
               __syncwarp();
             }
-          }
-          for (int pl = 0; pl < p.planes; ++pl) {
-#pragma unroll
-            for (int sl = 0; sl < 2; ++sl) {
+            for (int pl = 0; pl < p.planes; ++pl) {
               uint32_t w[32];
 #pragma unroll
-              for (int j = 0; j < 32; ++j) w[j] = take_bf16(v[64 * sl + 2 * j], v[64 * sl + 2 * j + 1]);
-              if (64 * sl < cols) store_slab16(&tmC, stg, lane, w, n0 + 64 * sl, r0, pl);
+              for (int j = 0; j < 32; ++j) w[j] = take_bf16(u[2 * j], u[2 * j + 1]);
+              store_slab16(&tmC, stg, lane, w, n0 + 64 * sl, r0, pl);
             }
+            asm volatile("" ::: "memory");
           }
         }
       } else if constexpr (EPI == kSum) {
 #pragma unroll
-        for (int sl = 0; sl < 4; ++sl) {
+        for (int sl = 0; sl < CW / 32; ++sl) {
           if (32 * sl >= cols) break;
           if (lane == 0) bulk_wait_read();
           __syncwarp();
@@ -449,54 +464,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         }
       } else {
         const float scale = *p.scale;
-#pragma unroll
-        for (int j = 0; j < 128; ++j) v[j] *= scale;
         if (p.tma_out) {
           if (p.out_bf16) {
 #pragma unroll
-            for (int sl = 0; sl < 2; ++sl) {
+            for (int sl = 0; sl < CW / 64; ++sl) {
               if (64 * sl >= cols) break;
               uint32_t w[32];
 #pragma unroll
-              for (int j = 0; j < 32; ++j) w[j] = pack2_bf16(v[64 * sl + 2 * j], v[64 * sl + 2 * j + 1]);
+              for (int j = 0; j < 32; ++j)
+                w[j] = pack2_bf16(scale * v[64 * sl + 2 * j], scale * v[64 * sl + 2 * j + 1]);
               store_slab16(&tmC, stg, lane, w, n0 + 64 * sl, r0, 0);
+              asm volatile("" ::: "memory");
             }
           } else {
 #pragma unroll
-            for (int sl = 0; sl < 4; ++sl) {
+            for (int sl = 0; sl < CW / 32; ++sl) {
               if (32 * sl >= cols) break;
               uint32_t w[32];
 #pragma unroll
-              for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(v[32 * sl + j]);
+              for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(scale * v[32 * sl + j]);
               store_slab16(&tmC, stg, lane, w, n0 + 32 * sl, r0, 0);
+              asm volatile("" ::: "memory");
             }
           }
         } else {
           // any alignment, or adding to what is there: through shared memory,
           // a row's 32 columns per access
 #pragma unroll
-          for (int sl = 0; sl < 4; ++sl) {
+          for (int sl = 0; sl < CW / 32; ++sl) {
             if (32 * sl >= cols) break;
-            __syncwarp();
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              asm volatile("st.shared.f32 [%0], %1;" ::"r"(stg + 4u * (uint32_t)(lane * 32 + (j ^ lane))),
-                           "f"(v[32 * sl + j])
-                           : "memory");
-            __syncwarp();
+            stage_slab(stage, lane, v + 32 * sl);
             const int c = 32 * sl + lane, rows = min(32, p.M - r0);
+            if (c >= cols) continue;
+            const int64_t at = (int64_t)r0 * p.ldo + n0 + c;
+#pragma unroll 4
             for (int r = 0; r < rows; ++r) {
-              float q;
-              asm volatile("ld.shared.f32 %0, [%1];" : "=f"(q)
-                           : "r"(stg + 4u * (uint32_t)(r * 32 + (lane ^ r)))
-                           : "memory");
-              if (c >= cols) continue;
-              const int64_t at = (int64_t)(r0 + r) * p.ldo + n0 + c;
+              const float q = scale * staged(stage, lane, r);
               if (p.out_bf16) {
-                __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + at;
+                __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + at + r * p.ldo;
                 *o = __float2bfloat16_rn(p.accumulate ? __bfloat162float(*o) + q : q);
               } else {
-                float* o = static_cast<float*>(p.out) + at;
+                float* o = static_cast<float*>(p.out) + at + r * p.ldo;
                 *o = p.accumulate ? *o + q : q;
               }
             }
@@ -516,25 +524,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   }
 }
 
-// Scratch words before the arrays, zero between calls: [0] rows joined so far.
+// Scratch words before the arrays; joined (blocks done) is zero between calls.
 struct Head {
   unsigned joined;
-  unsigned pad0;
-  float scale;   // backward: upstream / divisor
-  float inv;     // unused slot kept for alignment
+  float scale;  // backward: upstream / divisor
 };
 
-// Classes of the rows as int32 (-1: none); no order, no sums.
-__global__ void __launch_bounds__(256) targets_kernel(const void* target, int type, int64_t rows,
-                                                      int64_t classes, int32_t* out) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows; i += 256LL * gridDim.x)
-    out[i] = (int32_t)class_index(target, type, i, classes);
-}
+struct Targets {
+  const void* p;
+  int type;
+  int64_t rows, classes;
+  __device__ __forceinline__ int64_t at(int64_t r) const { return class_index(p, type, r, classes); }
+};
 
 // Rows with a target, by one block; every thread gets the count.
-__device__ __forceinline__ int64_t count_targets(const int32_t* t, int64_t rows, long long* sh) {
+__device__ __forceinline__ int64_t count_targets(const Targets& t, long long* sh) {
   long long n = 0;
-  for (int64_t i = threadIdx.x; i < rows; i += blockDim.x) n += t[i] >= 0;
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < t.rows; i += blockDim.x) n += t.at(i) >= 0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
   __syncthreads();
@@ -546,11 +553,11 @@ __device__ __forceinline__ int64_t count_targets(const int32_t* t, int64_t rows,
 }
 
 // scale = upstream / divisor
-__global__ void __launch_bounds__(1024) scale_kernel(const int32_t* t, int64_t rows, float divisor,
-                                                     const float* upstream, float* scale) {
+__global__ void __launch_bounds__(1024) scale_kernel(Targets t, float divisor, const float* upstream,
+                                                     float* scale) {
   __shared__ long long sh[32];
   float d = divisor;
-  if (!(d > 0.f)) d = fmaxf(1.f, (float)count_targets(t, rows, sh));
+  if (!(d > 0.f)) d = fmaxf(1.f, (float)count_targets(t, sh));
   if (threadIdx.x == 0) *scale = (upstream ? *upstream : 1.f) / d;
 }
 
@@ -560,38 +567,59 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   m = M;
 }
 
-// Joins a piece's partials of 32 rows: warp w takes slots w, w + 8, ...; the
-// last piece writes lse and the losses, and the last block the mean.
+// Joins a piece's partials of R rows per block, 256 / R threads a row; the last
+// piece writes lse and the losses, and the last block the mean.
+template <int R>
 __global__ void __launch_bounds__(256) join_kernel(const float2* part, int64_t part_ld, int slots,
-                                                   int64_t rows, const int32_t* target,
-                                                   const float* zt, float2* run, int first, int last,
-                                                   float divisor, float* row_loss, float* lse,
-                                                   float* loss, Head* head) {
-  __shared__ float2 sh[8][33];
+                                                   Targets target, const float* zt, float2* run,
+                                                   int first, int last, float divisor,
+                                                   float* row_loss, float* lse, float* loss,
+                                                   Head* head) {
+  constexpr int L = 256 / R;
+  __shared__ float2 sh[L][R + 1];
   __shared__ unsigned ticket;
   __shared__ long long shn[8];
   __shared__ double shd[8];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int64_t row = (int64_t)blockIdx.x * 32 + lane;
+  const int r = threadIdx.x % R, l = threadIdx.x / R;
+  const int64_t row = (int64_t)blockIdx.x * R + r, rows = target.rows;
   float m = -INFINITY, s = 0.f;
-  if (row < rows)
-    for (int i = w; i < slots; i += 8) {
-      const float2 q = __ldcs(part + (int64_t)i * part_ld + row);
-      join(m, s, q.x, q.y);
+  if (row < rows) {
+    const float2* q = part + row;
+    int i = l;
+    for (; i + 3 * L < slots; i += 4 * L) {  // four loads on their way
+      float2 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = __ldcs(q + (int64_t)(i + k * L) * part_ld);
+      const float M = fmaxf(fmaxf(fmaxf(v[0].x, v[1].x), fmaxf(v[2].x, v[3].x)), m);
+      const float base = M == -INFINITY ? 0.f : M;
+      s *= exp_fast(m - base);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s += v[k].y * exp_fast(v[k].x - base);
+      m = M;
     }
-  sh[w][lane] = make_float2(m, s);
-  __syncthreads();
-  if (w == 0 && row < rows) {
-    for (int i = 1; i < 8; ++i) join(m, s, sh[i][lane].x, sh[i][lane].y);
+    for (; i < slots; i += L) {
+      const float2 v = __ldcs(q + (int64_t)i * part_ld);
+      join(m, s, v.x, v.y);
+    }
+  }
+  sh[l][r] = make_float2(m, s);
+  for (int h = L / 2; h > 0; h >>= 1) {
+    __syncthreads();
+    if (l < h) {
+      join(m, s, sh[l + h][r].x, sh[l + h][r].y);
+      sh[l][r] = make_float2(m, s);
+    }
+  }
+  if (l == 0 && row < rows) {
     if (!first) join(m, s, run[row].x, run[row].y);
     if (!last) {
       run[row] = make_float2(m, s);
     } else {
-      const float l = m + logf(s);  // a row of -inf: -inf
-      if (lse) lse[row] = l;
+      const float log_s = logf(s);  // a row of -inf: -inf
+      if (lse) lse[row] = m + log_s;
       float v = 0.f;
       // (m - zt) + log s: lse - zt would round lse first
-      if (target[row] >= 0) v = zt[row] == -INFINITY ? INFINITY : (m - zt[row]) + logf(s);
+      if (target.at(row) >= 0) v = zt[row] == -INFINITY ? INFINITY : (m - zt[row]) + log_s;
       row_loss[row] = v;
     }
   }
@@ -603,10 +631,11 @@ __global__ void __launch_bounds__(256) join_kernel(const float2* part, int64_t p
   if (ticket != gridDim.x - 1) return;
   __threadfence();
   double t = 0.0;
+#pragma unroll 4
   for (int64_t i = threadIdx.x; i < rows; i += 256) t += (double)__ldcg(row_loss + i);
   t = warp_sum(t);
-  if (lane == 0) shd[w] = t;
-  const int64_t n = divisor > 0.f ? 1 : count_targets(target, rows, shn);
+  if ((threadIdx.x & 31) == 0) shd[threadIdx.x >> 5] = t;
+  const int64_t n = divisor > 0.f ? 1 : count_targets(target, shn);
   __syncthreads();
   if (threadIdx.x == 0) {
     t = 0.0;
@@ -617,36 +646,92 @@ __global__ void __launch_bounds__(256) join_kernel(const float2* part, int64_t p
   }
 }
 
+// Eight elements of a row from any element offset, those past `left` zero.
+__device__ __forceinline__ void load8(const float* p, int64_t left, float (&v)[8]) {
+  if (left >= 8 && ((uintptr_t)p & 15) == 0) {
+    const float4 a = ld_stream4(p), b = ld_stream4(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? p[i] : 0.f;
+  }
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, int64_t left, float (&v)[8]) {
+  if (left >= 9) {  // words of two; where p lies between words, up to element 8
+    const uint32_t* q = reinterpret_cast<const uint32_t*>((uintptr_t)p & ~(uintptr_t)3);
+    const bool odd = ((uintptr_t)p & 2) != 0;
+    uint32_t w[5];
+    w[0] = odd ? (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(p)) << 16 : __ldg(q);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) w[i] = __ldg(q + i);
+    w[4] = odd ? __ldg(q + 4) : 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t x = odd ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+      v[2 * i] = __uint_as_float(x << 16);
+      v[2 * i + 1] = __uint_as_float(x & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? __bfloat162float(p[i]) : 0.f;
+  }
+}
+
 // The terms of a matrix as bf16 planes [planes][rows][ld], columns past `cols`
 // zero: three that sum to a float32 matrix exactly, or a copy of a bf16 one
-// whose rows TMA cannot address.
+// whose rows TMA cannot address.  ld is a multiple of 8.
 template <typename T>
 __global__ void __launch_bounds__(256) planes_kernel(const T* __restrict__ X, int64_t ldx, int64_t rows,
                                                      int64_t cols, int planes,
                                                      __nv_bfloat16* __restrict__ out, int64_t ld) {
-  const int64_t pairs = ld / 2, n = rows * pairs;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += 256LL * gridDim.x) {
-    const int64_t r = i / pairs, c = 2 * (i - r * pairs);
-    float a = c < cols ? to_f32(X[r * ldx + c]) : 0.f;
-    float b = c + 1 < cols ? to_f32(X[r * ldx + c + 1]) : 0.f;
-    for (int p = 0; p < planes; ++p)
-      *reinterpret_cast<uint32_t*>(out + ((int64_t)p * rows + r) * ld + c) = take_bf16(a, b);
+  const int64_t plane = rows * ld;
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    const T* src = X + r * ldx;
+    __nv_bfloat16* dst = out + r * ld;
+    for (int64_t c = 8 * ((int64_t)blockIdx.x * 256 + threadIdx.x); c < ld; c += 8 * 256LL * gridDim.x) {
+      float v[8];
+      load8(src + c, cols - c, v);
+      for (int p = 0; p < planes; ++p)
+        *reinterpret_cast<uint4*>(dst + p * plane + c) =
+            make_uint4(take_bf16(v[0], v[1]), take_bf16(v[2], v[3]), take_bf16(v[4], v[5]),
+                       take_bf16(v[6], v[7]));
+    }
   }
 }
 
-// dx = scale * (sum of the splits' sums) (+ dx)
+// dx = scale * (sum of the splits' sums) (+ dx); a block a row, four columns a
+// thread (ld is a multiple of 4).
 template <typename T>
 __global__ void __launch_bounds__(256) dx_kernel(const float* __restrict__ sums, int splits, int64_t rows,
                                                  int64_t cols, int64_t ld, const float* scale, T* dx,
                                                  int64_t lddx, int accumulate) {
   const float k = *scale;
-  const int64_t n = rows * cols;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += 256LL * gridDim.x) {
-    const int64_t r = i / cols, c = i - r * cols;
-    float s = 0.f;
-    for (int p = 0; p < splits; ++p) s += sums[((int64_t)p * rows + r) * ld + c];
-    T* o = dx + r * lddx + c;
-    from_f32(o, (accumulate ? to_f32(*o) : 0.f) + k * s);
+  const bool vec = cols % 4 == 0 && lddx % 4 == 0 && ((uintptr_t)dx & 15) == 0;
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    T* o = dx + r * lddx;
+    for (int64_t c = 4 * (int64_t)threadIdx.x; c < cols; c += 1024) {
+      float4 s = __ldcs(reinterpret_cast<const float4*>(sums + r * ld + c));
+      for (int p = 1; p < splits; ++p) {
+        const float4 q = __ldcs(reinterpret_cast<const float4*>(sums + ((int64_t)p * rows + r) * ld + c));
+        s.x += q.x; s.y += q.y; s.z += q.z; s.w += q.w;
+      }
+      float v[4] = {k * s.x, k * s.y, k * s.z, k * s.w};
+      const int n = (int)min((int64_t)4, cols - c);
+      if (accumulate) {
+        for (int i = 0; i < n; ++i) v[i] += to_f32(o[c + i]);
+      }
+      if (vec) {
+        if constexpr (sizeof(T) == 4)
+          *reinterpret_cast<float4*>(o + c) = make_float4(v[0], v[1], v[2], v[3]);
+        else
+          *reinterpret_cast<uint2*>(o + c) = make_uint2(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < n) from_f32(o + c + i, v[i]);
+      }
+    }
   }
 }
 
@@ -741,6 +826,7 @@ struct Call {
   float divisor;
   char* scratch;
   cudaStream_t st;
+  Targets targets() const { return {target, index_type, rows, classes}; }
   bool f32() const { return dtype == TL_F32; }
   int planes() const { return f32() ? 3 : 1; }
   int terms() const { return f32() ? kTerms : 1; }
@@ -753,7 +839,7 @@ struct Plan {
   int64_t fpiece, bpiece;          // classes per piece, forward and backward
   int64_t part_ld;                 // rows of the forward's partials
   int splits;                      // of K in dx
-  int64_t targets, xplanes, wplanes, zt, run, row_loss, part, g, sums, colsum, total;  // offsets
+  int64_t xplanes, wplanes, zt, run, row_loss, part, g, sums, colsum, total;  // offsets
 };
 
 // splits of K that let few tiles of dx fill the GPU: whole waves of clusters
@@ -783,7 +869,7 @@ Plan make_plan(int dtype, int trans_w, int64_t rows, int64_t classes, int64_t wi
   q.part_ld = up_to(rows, 32);
   const int64_t cap = 512LL << 20;
   // the partials (8 bytes per row and 128 classes) and the terms of W
-  q.fpiece = std::min(piece(q.part_ld / 16, cap), piece(width * 2 * P, cap));
+  q.fpiece = std::min(piece(q.part_ld * 8 / CW, cap), piece(width * 2 * P, cap));
   q.bpiece = std::min(piece(rows * 2 * P, cap), piece(width * 2 * P, cap));
   q.splits = backward ? dx_splits(rows, width, q.bpiece) : 1;
   int64_t at = 1024;
@@ -792,7 +878,6 @@ Plan make_plan(int dtype, int trans_w, int64_t rows, int64_t classes, int64_t wi
     at = up_to(at + bytes, 1024);
     return o;
   };
-  q.targets = take(rows * 4);
   q.xplanes = take(P * rows * up_to(width, 8) * 2);
   const int64_t wp = backward ? std::max(q.fpiece, q.bpiece) : q.fpiece;
   q.wplanes = take(P * (trans_w ? wp * up_to(width, 8) : width * up_to(wp, 8)) * 2);
@@ -800,7 +885,7 @@ Plan make_plan(int dtype, int trans_w, int64_t rows, int64_t classes, int64_t wi
   q.zt = take(rows * 4);
   q.run = take(rows * 8);
   q.row_loss = take(rows * 4);
-  q.part = take(q.fpiece / 128 * q.part_ld * 8);
+  q.part = take(q.fpiece / CW * q.part_ld * 8);
   q.total = at;
   if (backward) {
     at = common;
@@ -815,8 +900,9 @@ Plan make_plan(int dtype, int trans_w, int64_t rows, int64_t classes, int64_t wi
 template <typename T>
 int write_planes(const T* X, int64_t ldx, int64_t rows, int64_t cols, int planes, __nv_bfloat16* out,
                  int64_t ld, cudaStream_t st) {
-  const int64_t blocks = std::min<int64_t>((rows * (ld / 2) + 255) / 256, 16LL * sm_count());
-  planes_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(X, ldx, rows, cols, planes, out, ld);
+  const int64_t across = (ld / 8 + 255) / 256;
+  const dim3 grid((unsigned)std::min<int64_t>(across, 16), (unsigned)std::min<int64_t>(rows, 65535));
+  planes_kernel<T><<<grid, 256, 0, st>>>(X, ldx, rows, cols, planes, out, ld);
   return after_launch();
 }
 
@@ -855,20 +941,18 @@ int logits(const Call& c, const Planes& x, const Planes& w, const CUtensorMap& o
   p.kc = c.kc();
   p.splits = 1;
   p.bias = c.bias ? c.bias + c0 : nullptr;
+  p.target = c.target;
+  p.index_type = c.index_type;
+  p.classes = c.classes;
   p.col0 = (int)c0;
   return c.trans_w ? launch_tiles<0, 1, EPI>(a, b, out, p, c.st)
                    : launch_tiles<0, 0, EPI>(a, b, out, p, c.st);
 }
 
 int forward(const Call& c, const Plan& q, float* loss, float* row_loss, float* lse) {
-  int32_t* targets = reinterpret_cast<int32_t*>(c.scratch + q.targets);
-  targets_kernel<<<(unsigned)std::min<int64_t>((c.rows + 255) / 256, 4LL * sm_count()), 256, 0, c.st>>>(
-      c.target, c.index_type, c.rows, c.classes, targets);
-  TL_TRY(after_launch());
   Planes x, w;
   TL_TRY(as_planes(c, c.x, c.ldx, c.rows, c.width, q.xplanes, &x));
   TileParams p{};
-  p.target = targets;
   p.part = reinterpret_cast<float2*>(c.scratch + q.part);
   p.part_ld = q.part_ld;
   p.zt = reinterpret_cast<float*>(c.scratch + q.zt);
@@ -879,10 +963,17 @@ int forward(const Call& c, const Plan& q, float* loss, float* row_loss, float* l
     const int64_t n = std::min(q.fpiece, c.classes - c0);
     TL_TRY(w_planes(c, q, c0, n, &w));
     TL_TRY(logits<kStats>(c, x, w, none, p, c0, n));
-    join_kernel<<<(unsigned)(q.part_ld / 32), 256, 0, c.st>>>(
-        p.part, q.part_ld, (int)((n + 127) / 128), c.rows, targets, p.zt,
-        reinterpret_cast<float2*>(c.scratch + q.run), c0 == 0, c0 + n == c.classes, c.divisor, row_loss,
-        lse, loss, reinterpret_cast<Head*>(c.scratch));
+    // few rows: more threads for each
+    auto join_rows = [&](auto kern, int64_t r) {
+      kern<<<(unsigned)((c.rows + r - 1) / r), 256, 0, c.st>>>(
+          p.part, q.part_ld, (int)((n + CW - 1) / CW), c.targets(), p.zt,
+          reinterpret_cast<float2*>(c.scratch + q.run), c0 == 0, c0 + n == c.classes, c.divisor, row_loss,
+          lse, loss, reinterpret_cast<Head*>(c.scratch));
+    };
+    if (c.rows >= 4096)
+      join_rows(join_kernel<32>, 32);
+    else
+      join_rows(join_kernel<4>, 4);
     TL_TRY(after_launch());
   }
   return TL_OK;
@@ -890,12 +981,8 @@ int forward(const Call& c, const Plan& q, float* loss, float* row_loss, float* l
 
 int backward(const Call& c, const Plan& q, const float* lse, const float* upstream, void* dx, int64_t lddx,
              void* dW, int64_t lddw, float* dbias, int accumulate) {
-  int32_t* targets = reinterpret_cast<int32_t*>(c.scratch + q.targets);
   float* scale = &reinterpret_cast<Head*>(c.scratch)->scale;
-  targets_kernel<<<(unsigned)std::min<int64_t>((c.rows + 255) / 256, 4LL * sm_count()), 256, 0, c.st>>>(
-      c.target, c.index_type, c.rows, c.classes, targets);
-  TL_TRY(after_launch());
-  scale_kernel<<<1, 1024, 0, c.st>>>(targets, c.rows, c.divisor, upstream, scale);
+  scale_kernel<<<1, 1024, 0, c.st>>>(c.targets(), c.divisor, upstream, scale);
   TL_TRY(after_launch());
   Planes x, w;
   TL_TRY(as_planes(c, c.x, c.ldx, c.rows, c.width, q.xplanes, &x));
@@ -910,8 +997,7 @@ int backward(const Call& c, const Plan& q, const float* lse, const float* upstre
     CUtensorMap a, b, o;
     if (!make_map3(&o, g.p, false, g.planes, g.rows, g.cols, g.ld, 64, 32)) return TL_ERR_UNSUPPORTED;
     TileParams p{};
-    p.target = targets;
-    p.lse = lse;
+      p.lse = lse;
     p.planes = c.planes();
     p.colsum = dbias ? colsum : nullptr;
     TL_TRY(logits<kGrad>(c, x, w, o, p, c0, n));
@@ -955,7 +1041,7 @@ int backward(const Call& c, const Plan& q, const float* lse, const float* upstre
     }
   }
   if (dx) {
-    const int64_t blocks = std::min<int64_t>((c.rows * c.width + 255) / 256, 16LL * sm_count());
+    const int64_t blocks = std::min<int64_t>(c.rows, 32LL * sm_count());
     if (c.f32())
       dx_kernel<float><<<(unsigned)blocks, 256, 0, c.st>>>(sums, q.splits, c.rows, c.width, sums_ld, scale,
                                                            static_cast<float*>(dx), lddx,
