@@ -208,6 +208,23 @@ __device__ __forceinline__ float staged(const float* stage, int lane, int row) {
   return stage[row * 32 + (lane ^ row)];
 }
 
+// Sum over the warp's lanes of column `lane` of their 32 values each: in five
+// steps a lane hands over the half of its columns that its partner keeps.
+template <int N>
+__device__ __forceinline__ float column_sum_of(const float* v, int lane) {
+  if constexpr (N == 1) {
+    return v[0];
+  } else {
+    float k[N / 2];
+    const bool up = lane & (N / 2);
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j)
+      k[j] = (up ? v[j + N / 2] : v[j]) + __shfl_xor_sync(0xffffffffu, up ? v[j] : v[j + N / 2], N / 2);
+    return column_sum_of<N / 2>(k, lane);
+  }
+}
+__device__ __forceinline__ float column_sum(const float* v, int lane) { return column_sum_of<32>(v, lane); }
+
 // A: x, g or x^T ...; TA 0: stored [M][K], 1: [K][M].  TB 0: B stored [K][N], 1: [N][K].
 template <int TA, int TB, int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
@@ -370,9 +387,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 
       if constexpr (EPI == kStats || EPI == kGrad) {
         if (p.bias) {
+          const float* b = p.bias + n0;
+          if (cols == CW && ((uintptr_t)b & 15) == 0) {
 #pragma unroll
-          for (int j = 0; j < CW; ++j)
-            if (j < cols) v[j] += __ldg(p.bias + n0 + j);
+            for (int j = 0; j < CW; j += 4) {
+              const float4 q = __ldg(reinterpret_cast<const float4*>(b + j));
+              v[j] += q.x; v[j + 1] += q.y; v[j + 2] += q.z; v[j + 3] += q.w;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < CW; ++j)
+              if (j < cols) v[j] += __ldg(b + j);
+          }
         }
         const int cls = live ? (int)class_index(p.target, p.index_type, row, p.classes) : -1;
         const int target = cls < 0 ? -1 : cls - p.col0 - n0;  // in this warp's columns
@@ -405,7 +431,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           // nothing left of the row: p = 0, as for the rows that do not count
           const float off = lse == -INFINITY ? INFINITY : lse;
           float* cs = p.colsum ? p.colsum + (int64_t)(r0 >> 5) * p.N + n0 : nullptr;
-          if (cs && lane == 0) bulk_wait_read();
 #pragma unroll
           for (int sl = 0; sl < CW / 64; ++sl) {  // one slab after the other: registers
             if (64 * sl >= cols) break;
@@ -421,17 +446,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
               for (int j = 0; j < 64; ++j) u[j] -= j == target - 64 * sl ? 1.f : 0.f;
             }
             if (cs) {  // before g is rounded
-              if (lane == 0) bulk_wait_read();
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                stage_slab(stage, lane, u + 32 * h);
-                float s = 0.f;
-#pragma unroll 8
-                for (int r = 0; r < 32; ++r) s += staged(stage, lane, r);
+                const float s = column_sum(u + 32 * h, lane);
                 const int c = 64 * sl + 32 * h + lane;
                 if (c < cols) cs[c] = s;
+                asm volatile("" ::: "memory");
               }
-              __syncwarp();
             }
             for (int pl = 0; pl < p.planes; ++pl) {
               uint32_t w[32];
