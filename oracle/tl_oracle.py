@@ -31,12 +31,16 @@ from typing import Dict, List, Optional
 
 import numpy as np
 
+from . import lm_ops
+
 try:  # exact erf for gelu; scipy is optional, math.erf is the fallback
     from scipy.special import erf as _erf
 except Exception:  # pragma: no cover
     _erf = np.vectorize(math.erf)
 
 SEMANTICS_EXTENSIONS = {
+    "lm_ops": "linear_cross_entropy, distill_topk, residual_norm, scaled_norm: the operators of a "
+              "language-model head, defined in oracle/lm_ops.py",
     "gelu": "exact 0.5*x*(1+erf(x/sqrt(2))); the reference has grammar/type rules "
             "(tensorlang.lark:175, type_checker.py:274) but no kernel",
     "swish": "x*sigmoid(x); same gap as gelu",
@@ -68,7 +72,9 @@ SEMANTICS_EXTENSIONS = {
 _BIN = {"add": np.add, "minus": np.subtract, "mult": np.multiply, "div": np.divide}
 _RECORDED_REFERENCE = {"add", "minus", "mult", "div", "matmul", "relu", "sigmoid", "tanh",
                        "softmax", "sum", "mean", "mse_loss"}
-_RECORDED_EXTENDED = _RECORDED_REFERENCE | {"linear", "cross_entropy", "layer_norm", "gelu", "swish"}
+_RECORDED_EXTENDED = _RECORDED_REFERENCE | {"linear", "cross_entropy", "layer_norm", "gelu", "swish",
+                                            "linear_cross_entropy", "distill_topk",
+                                            "residual_norm", "scaled_norm"}
 KERNEL_FREE = ("name", "tensor_literal", "load")
 
 
@@ -150,8 +156,10 @@ def infer_shape(expr: dict, shapes: Dict[str, tuple]) -> tuple:
             return ()
         ax = int(ax) % len(s)
         return tuple(d for i, d in enumerate(s) if i != ax)
-    if t in ("mse_loss", "cross_entropy"):
+    if t in ("mse_loss", "cross_entropy", "linear_cross_entropy", "distill_topk"):
         return ()
+    if t in ("residual_norm", "scaled_norm"):
+        return shapes[expr["args"][0]]
     if t == "transpose":
         s = shapes[expr["tensor"]]
         axes = expr.get("axes")
@@ -196,6 +204,50 @@ def _sigmoid(x):
 def _argfirst(x, axis, largest):
     """First index of the max (min) along ``axis``; NaN-free inputs."""
     return (np.argmax(x, axis=axis) if largest else np.argmin(x, axis=axis))
+
+
+def _gate_mode(x, gate) -> str:
+    return ("none" if gate is None else "channel" if gate.ndim == 1 else
+            "token" if gate.shape == (x.shape[0], 1) and x.shape[1] != 1 else "full")
+
+
+def _lm_op(t, expr, args, g=None):
+    """(value, gradients of the arguments for the gradient g of the value) of a
+    language-model operator, in float64 (``lm_ops``)."""
+    a = [np.asarray(v, dtype=np.float64) for v in args]
+    if t == "linear_cross_entropy":
+        x, w, b, q = a
+        r = lm_ops.linear_ce(x, w, _classes(q), b, expr.get("divisor") or 0.0,
+                             1.0 if g is None else float(np.asarray(g).item()))
+        return r["loss"], [r["dx"], r["dw"], r["dbias"], None]
+    if t == "distill_topk":
+        z, tv, ti = a
+        r = lm_ops.distill_topk(z, tv, _classes(ti), expr.get("temperature", 1.0),
+                                expr.get("divisor") or 0.0,
+                                1.0 if g is None else float(np.asarray(g).item()))
+        return r["loss"], [r["dz"], None, None]
+    kind, eps = expr.get("norm", "rms"), expr.get("eps", 1e-5)
+    if t == "scaled_norm":
+        x, w = a
+        n = lm_ops.residual_norm(x, w_pre=w, kind=kind, eps=eps)[1]
+        r = None if g is None else lm_ops.residual_norm_vjp(x, None, np.asarray(g, np.float64), w_pre=w,
+                                                            kind=kind, eps=eps)
+        return n, None if r is None else [r["dx"], r["dw_pre"]]
+    x, u, w = a[:3]
+    gate = a[3] if len(a) > 3 else None
+    mode = _gate_mode(x, gate)
+    kw = dict(u=u, w_post=w, gate=gate.ravel() if mode == "token" else gate, gate_mode=mode,
+              alpha=expr.get("alpha", 1.0), kind=kind, eps=eps)
+    y = lm_ops.residual_norm(x, **kw)[0]
+    if g is None:
+        return y, None
+    r = lm_ops.residual_norm_vjp(x, np.asarray(g, np.float64), None, **kw)
+    return y, [r["dx"], r["du"], r["dw_post"]] + ([] if gate is None else [r["dgate"].reshape(gate.shape)])
+
+
+def _classes(q):
+    """Class indices stored as float; a value that is no whole number names none."""
+    return np.where(np.isfinite(q) & (q == np.trunc(q)), q, -1).astype(np.int64)
 
 
 def op_forward(expr: dict, vals: Dict[str, np.ndarray], dt=np.float64,
@@ -311,6 +363,8 @@ def op_forward(expr: dict, vals: Dict[str, np.ndarray], dt=np.float64,
             pp = (p * q).sum(axis=1)
         pp = np.minimum(np.maximum(pp, lo), hi)
         return np.asarray(-np.log(pp).sum() / T(p.shape[0]), dtype=dt)
+    if t in ("linear_cross_entropy", "distill_topk", "residual_norm", "scaled_norm"):
+        return np.asarray(_lm_op(t, expr, [vals[n] for n in expr["args"]])[0], dtype=dt)
     if t == "transpose":  # :1949-1972
         x = vals[expr["tensor"]]
         axes = expr.get("axes")
@@ -494,6 +548,10 @@ class _Graph:
             gm = (np.sum(g * -1 / std, axis=ax, keepdims=True)
                   + gv * np.sum(-2 * (x - mean), axis=ax, keepdims=True) / n)
             self._acc(ins[0], g / std + gv * 2 * (x - mean) / n + gm / n)
+        elif op in ("linear_cross_entropy", "distill_topk", "residual_norm", "scaled_norm"):
+            for n, d in zip(ins, _lm_op(op, node.meta, [T[n] for n in ins], g)[1]):
+                if d is not None:
+                    self._acc(n, d)
         elif op == "mse_loss":
             p, q = T[ins[0]], T[ins[1]]
             sg = g.item() if g.size == 1 else g
@@ -580,6 +638,8 @@ class OracleProgram:
                 ax = len(self.env[e["tensor"]]) - 1
             eps = e.get("eps")
             meta = {"axis": int(ax), "eps": 1e-5 if eps is None else float(eps)}
+        elif t in ("linear_cross_entropy", "distill_topk", "residual_norm", "scaled_norm"):
+            meta = e
         self._record(t, node["name"], _expr_inputs(e), meta)
 
     def _literal(self, node):

@@ -30,7 +30,8 @@ from typing import Dict, List, Optional, Tuple
 
 from . import runtime as rt
 from .shapes import Shape, numel
-from .steps import EW, Copy, LibCall, Memset0, Step
+from .steps import (EW, Copy, LibCall, Memset0, Step, distill_args, lse_of, norm_args,
+                    zeroed_scratch)
 
 
 class Node:
@@ -307,9 +308,99 @@ class BackwardPlanner:
                                        ("int", cols), ("float", float(node.meta.get("eps", 1e-5))),
                                        ("int", 0 if first else 1)],
                                       [x, g] + ([] if first else [gx]), [gx]))
+        elif op == "linear_cross_entropy":
+            self._vjp_linear_ce(node)
+        elif op == "distill_topk":
+            self._vjp_distill(node)
+        elif op in ("residual_norm", "scaled_norm"):
+            self._vjp_norm(node)
         else:
             # the reference prints "No backward implemented" and skips (autograd.py:309-311)
             return
+
+    # -- operators with several gradients from one call ------------------------
+    def _targets(self, wanted):
+        """Where a call writes the gradients of ``wanted`` (operand, TL_ACC flag)
+        pairs: {flag: tensor}, the accumulate flags, and the values to add
+        afterwards (an operand that appears twice gets its second gradient in a
+        tensor of its own, since one call may not write a tensor twice)."""
+        where, acc, later = {}, 0, []
+        for name, flag in wanted:
+            if name is None or name not in self.requires:
+                continue
+            g = grad_name(name)
+            self.shapes.setdefault(g, tuple(self.shapes[name]))
+            if g in where.values():
+                where[flag] = self._tmp(tuple(self.shapes[name]))
+                later.append((name, where[flag]))
+                continue
+            if not self._first(name):
+                acc |= flag
+            where[flag] = g
+        return where, acc, later
+
+    def _multi(self, label, fname, args, reads, where, acc, flags, later, scratch):
+        added = [where[f] for f in where if acc & f]
+        self.steps.append(LibCall(label, fname, args, list(reads) + added,
+                                  [where[f] for f in flags if f in where] + [scratch]))
+        for name, value in later:
+            self._accumulate_value(name, value, tuple(self.shapes[value]))
+
+    def _vjp_linear_ce(self, node: Node):
+        x, w, b, t, rows, width, classes, divisor = node.meta["kinfo"][2:10]
+        g, lse = grad_name(node.out), lse_of(node.out)
+        flags = (rt.ACC_DX, rt.ACC_DW, rt.ACC_DBIAS)
+        where, acc, later = self._targets(zip((x, w, b), flags))
+        if not where:
+            return
+        out = lambda f: ("ptr", where[f]) if f in where else ("null",)  # noqa: E731
+        scratch = zeroed_scratch(self.shapes, "linear_ce", rt.lib().tl_linear_ce_scratch_bytes(
+            rt.F32, 0, rows, classes, width, 1))
+        args = [("int", rt.F32), ("int", 0), ("int", rows), ("int", classes), ("int", width),
+                ("ptr", x), ("int", width), ("ptr", w), ("int", classes), ("ptr", b), ("ptr", t),
+                ("int", rt.IDX_F32), ("float", divisor), ("ptr", lse), ("ptr", g),
+                out(rt.ACC_DX), ("int", width), out(rt.ACC_DW), ("int", classes),
+                out(rt.ACC_DBIAS), ("int", acc), ("ptr", scratch), ("bytes", scratch)]
+        self._multi(f"linear_cross_entropy_bwd:{node.out}", "tl_linear_ce_backward", args,
+                    [x, w, b, t, lse, g], where, acc, flags, later, scratch)
+
+    def _vjp_distill(self, node: Node):
+        z, tv, ti, rows, classes, top, tau, divisor = node.meta["kinfo"][2:10]
+        if z not in self.requires:
+            return  # the teacher gets no gradient
+        first = self._first(z)
+        g, gz = grad_name(node.out), grad_name(z)
+        self.shapes.setdefault(gz, tuple(self.shapes[z]))
+        args = distill_args(self.shapes, z, tv, ti, rows, classes, top, tau, divisor, upstream=g,
+                            dz=gz, accumulate=0 if first else 1)
+        self.steps.append(LibCall(f"distill_topk_bwd:{gz}", "tl_distill_topk", args,
+                                  [z, tv, ti, g] + ([] if first else [gz]),
+                                  [gz, zeroed_scratch(self.shapes, "distill", 0)]))
+
+    def _vjp_norm(self, node: Node):
+        g = grad_name(node.out)
+        flags = (rt.ACC_DX, rt.ACC_DU, rt.ACC_DGATE, rt.ACC_DW_POST, rt.ACC_DW_PRE)
+        if node.op == "residual_norm":
+            x, u, w, gate, rows, cols, norm, mode, alpha, eps = node.meta["kinfo"][2:12]
+            head = norm_args(rows, cols, norm, x, u, w, gate, mode, alpha, None, eps)
+            where, acc, later = self._targets(zip((x, u, gate, w), flags))
+            dy, dn, reads = ("ptr", g), ("null",), [x, u, w] + ([gate] if gate else [])
+        else:
+            x, w, rows, cols, norm, eps = node.meta["kinfo"][2:8]
+            head = norm_args(rows, cols, norm, x, None, None, None, "none", 1.0, w, eps)
+            where, acc, later = self._targets(((x, rt.ACC_DX), (w, rt.ACC_DW_PRE)))
+            dy, dn, reads = ("null",), ("ptr", g), [x, w]
+        if not where:
+            return
+        out = lambda f: ("ptr", where[f]) if f in where else ("null",)  # noqa: E731
+        scratch = zeroed_scratch(self.shapes, "residual_norm",
+                                 rt.lib().tl_residual_norm_scratch_bytes(rows, cols))
+        args = head + [dy, ("int", cols), dn, ("int", cols), out(rt.ACC_DX), ("int", cols),
+                       out(rt.ACC_DU), ("int", cols), out(rt.ACC_DGATE), ("int", cols),
+                       out(rt.ACC_DW_POST), out(rt.ACC_DW_PRE), ("int", acc), ("ptr", scratch),
+                       ("bytes", scratch)]
+        self._multi(f"{node.op}_bwd:{node.out}", "tl_residual_norm_backward", args, reads + [g],
+                    where, acc, flags, later, scratch)
 
     def _vjp_gemm(self, node: Node):
         """matmul autograd.py:520-537; linear :619-646."""

@@ -40,7 +40,7 @@ from .shapes import Shape, complete_env, expr_inputs, numel
 from .steps import Step
 
 # ops that consume the batch axis (their output is no longer per-example)
-_BATCH_REDUCING = {"mse_loss", "cross_entropy"}
+_BATCH_REDUCING = {"mse_loss", "cross_entropy", "linear_cross_entropy", "distill_topk"}
 
 
 # ---------------------------------------------------------------------------
@@ -349,6 +349,23 @@ def loss_divisors(ast: list, shapes: Dict[str, Shape], derived: set) -> dict:
     return out
 
 
+def check_loss_divisors(ast: list, derived: set) -> None:
+    """linear_cross_entropy and distill_topk divide by the rows that count, which
+    each rank knows of its own batch only: over several ranks the program has
+    to name the divisor of the global batch."""
+    def visit(nodes):
+        for n in nodes:
+            if n["type"] == "for":
+                visit(n["body"])
+            elif n["type"] == "let" and isinstance(n.get("expr"), dict):
+                e = n["expr"]
+                if e["type"] in ("linear_cross_entropy", "distill_topk") and \
+                        e["args"][0] in derived and not e.get("divisor"):
+                    raise NotImplementedError(f"{e['type']} {n['name']} over a sharded batch "
+                                              "without a divisor")
+    visit(ast)
+
+
 def _batch_dependent(grad: str, bw: List[Step]) -> bool:
     """Whether a replicated tensor's gradient can differ between ranks: some
     backward step writes it from data.  Gradients that are only zero-filled
@@ -378,6 +395,8 @@ class DataParallelProgram:
         self.derived = batch_derived(ast, sharded)
         local = shard_shapes(gshapes, self.derived, comm.world)
         divisors = loss_divisors(ast, gshapes, self.derived)
+        if comm.world > 1:
+            check_loss_divisors(ast, self.derived)
         self.global_shapes = gshapes
         self.replicated_grads: List[str] = []
 

@@ -28,18 +28,22 @@ import numpy as np
 
 from . import runtime as rt
 from .autograd import BackwardPlanner, Node, grad_name
+from .blocknorm import fuse_block_norms
 from .dataio import check_shape, load_data_file
 from .epilogue import fuse_gemm_epilogues
 from .head import fuse_classifier_head
 from .pairs import fuse_bias_colsums, plan_gemm_pairs
 from .kernel_generator import KernelGenerator
 from .shapes import Shape, broadcast, complete_env, expr_inputs, numel
-from .steps import EW, Copy, LibCall, Memset0, RegionStep, Step, fuse, kinfo_to_step
+from .steps import (EW, ZEROED, Copy, LibCall, Memset0, RegionStep, Step, fuse,
+                    kinfo_to_step)
 
 KERNEL_FREE = ("name", "tensor_literal", "load")
 RECORDED_REFERENCE = {"add", "minus", "mult", "div", "matmul", "relu", "sigmoid", "tanh",
                       "softmax", "sum", "mean", "mse_loss"}
-RECORDED_EXTENDED = RECORDED_REFERENCE | {"linear", "cross_entropy", "layer_norm", "gelu", "swish"}
+RECORDED_EXTENDED = RECORDED_REFERENCE | {"linear", "cross_entropy", "layer_norm", "gelu", "swish",
+                                          "linear_cross_entropy", "distill_topk", "residual_norm",
+                                          "scaled_norm"}
 
 
 def lower_let(name: str, expr: dict, shapes: Dict[str, Shape], gen: KernelGenerator) -> tuple:
@@ -98,6 +102,24 @@ def lower_let(name: str, expr: dict, shapes: Dict[str, Shape], gen: KernelGenera
     if t == "cross_entropy":
         p, q = expr["args"]
         return gen.cross_entropy("cross_entropy", name, p, shapes[p], shapes[q], q)[1]
+    if t == "linear_cross_entropy":
+        x, w, b, q = expr["args"]
+        return gen.linear_cross_entropy(t, name, x, w, b, q, shapes[x], shapes[w], shapes[q],
+                                        expr.get("divisor"))[1]
+    if t == "distill_topk":
+        z, tv, ti = expr["args"]
+        return gen.distill_topk(t, name, z, tv, ti, shapes[z], shapes[tv], shapes[ti],
+                                expr.get("temperature", 1.0), expr.get("divisor"))[1]
+    if t == "residual_norm":
+        x, u, w = expr["args"][:3]
+        g = expr["args"][3] if len(expr["args"]) > 3 else None
+        return gen.residual_norm(t, name, x, u, w, g, shapes[x], shapes[u], shapes[w],
+                                 shapes[g] if g else None, expr.get("norm", "rms"),
+                                 expr.get("alpha", 1.0), expr.get("eps", 1e-5))[1]
+    if t == "scaled_norm":
+        x, w = expr["args"]
+        return gen.scaled_norm(t, name, x, w, shapes[x], shapes[w], expr.get("norm", "rms"),
+                               expr.get("eps", 1e-5))[1]
     if t == "mse_loss":
         p, q = expr["args"]
         return gen.mse_loss("mse_loss", name, p, q, numel(shapes[p]))[1]
@@ -290,6 +312,8 @@ class Program:
                 ax = len(self.shapes[e["tensor"]]) - 1
             eps = e.get("eps")
             meta = {"axis": int(ax), "eps": 1e-5 if eps is None else float(eps)}
+        elif t in ("linear_cross_entropy", "distill_topk", "residual_norm", "scaled_norm"):
+            meta = {"kinfo": lower_let(node["name"], e, self.shapes, self.gen)}
         self._record(t, node["name"], expr_inputs(e), meta)
 
     def _literal_value(self, node) -> np.ndarray:
@@ -451,6 +475,7 @@ class Program:
 
     def _fuse_all(self):
         if self.fuse_ops:
+            fuse_block_norms(self)
             fuse_gemm_epilogues(self)
             if self.fuse_head:
                 fuse_classifier_head(self)
@@ -551,7 +576,8 @@ class Program:
                 continue
             if base not in self.shapes:
                 raise KeyError(f"no shape known for tensor {base!r}")
-            self.buffers[base] = rt.DeviceBuffer(self.dev, self.shapes[base])
+            self.buffers[base] = rt.DeviceBuffer(self.dev, self.shapes[base],
+                                                 zero=base.startswith(ZEROED))
         for n, v in self.initial.items():
             self.buffers[self.alias.get(n, n)].upload(v)
         scratch_bytes = self._scratch_bytes()

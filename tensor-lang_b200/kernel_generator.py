@@ -20,6 +20,9 @@ Differences, all additions:
 * ``argmax``/``argmin`` accept axis 0 (``'argmax_axis0'``, ``'argmin_axis0'``)
   and ``argmin`` the full tensor (``'argmin_full'``);
 * shapes the reference returns ``None`` for raise ``NotImplementedError``;
+* ``linear_cross_entropy``, ``distill_topk``, ``residual_norm`` and
+  ``scaled_norm``: the operators of a language-model head (no reference
+  counterpart; ``include/tlb200.h``);
 * ``numpy_broadcast=True`` (the backend's ``semantics="numpy"``) gives a
   square 2-D op 1-D the NumPy kernel (``B[j]``) instead of the per-row one.
 """
@@ -40,11 +43,29 @@ _SIGNATURES = {
     "concat": ("concat",), "reshape": ("reshape",), "instance_norm": ("instance_norm",),
     "batch_norm": ("batch_norm",), "transpose": ("transpose",), "mse_loss": ("mse_loss",),
     "cross_entropy": ("cross_entropy",),
+    "linear_cross_entropy": ("linear_cross_entropy",), "distill_topk": ("distill_topk",),
+    "residual_norm": ("residual_norm",), "scaled_norm": ("scaled_norm",),
 }
+
+NORMS = ("layer", "rms")
 
 
 def _prod(shape) -> int:
     return int(np.prod([int(d) for d in shape])) if len(shape) else 1
+
+
+def _divisor(d) -> float:
+    """A loss's divisor: 0 stands for the rows that count."""
+    if d is None:
+        return 0.0
+    if not float(d) > 0:
+        raise ValueError(f"loss divisor {d}")
+    return float(d)
+
+
+def _norm_kind(norm):
+    if norm not in NORMS:
+        raise ValueError(f"norm must be one of {NORMS}, not {norm!r}")
 
 
 class KernelGenerator:
@@ -251,6 +272,70 @@ class KernelGenerator:
 
     def mse_loss(self, op_type, name, pred_name, target_name, total_elements):
         return "", (f"{op_type}", name, pred_name, target_name, total_elements)
+
+    # -- language-model head and block boundary --------------------------------
+    def linear_cross_entropy(self, op_type, name, input_name, weight_name, bias_name, target_name,
+                             input_shape, weight_shape, target_shape, divisor=None):
+        """Cross entropy of linear(x, W, b) with class-index targets, without
+        keeping the logits; the mean over the rows that have a class, or the
+        sum over a given divisor."""
+        self._validate("linear_cross_entropy", op_type)
+        if len(input_shape) != 2 or len(weight_shape) != 2 or input_shape[1] != weight_shape[0] or \
+                tuple(target_shape) != (input_shape[0],):
+            raise NotImplementedError(f"linear_cross_entropy of {tuple(input_shape)} @ "
+                                      f"{tuple(weight_shape)} vs {tuple(target_shape)}")
+        return "", (op_type, name, input_name, weight_name, bias_name, target_name,
+                    int(input_shape[0]), int(input_shape[1]), int(weight_shape[1]),
+                    _divisor(divisor))
+
+    def distill_topk(self, op_type, name, logits_name, teacher_name, index_name, logits_shape,
+                     teacher_shape, index_shape, temperature=1.0, divisor=None):
+        """KL divergence from a teacher's top logits (values and class indices)
+        to the softmax of the logits, both at a temperature."""
+        self._validate("distill_topk", op_type)
+        if len(logits_shape) != 2 or len(teacher_shape) != 2 or \
+                tuple(teacher_shape) != tuple(index_shape) or teacher_shape[0] != logits_shape[0]:
+            raise NotImplementedError(f"distill_topk of {tuple(logits_shape)} vs "
+                                      f"{tuple(teacher_shape)}, {tuple(index_shape)}")
+        if not 0 < float(temperature) < float("inf"):
+            raise ValueError(f"distill_topk temperature {temperature}")
+        return "", (op_type, name, logits_name, teacher_name, index_name, int(logits_shape[0]),
+                    int(logits_shape[1]), int(teacher_shape[1]), float(temperature),
+                    _divisor(divisor))
+
+    def residual_norm(self, op_type, name, x_name, block_name, weight_name, gate_name, x_shape,
+                      block_shape, weight_shape, gate_shape, norm="rms", alpha=1.0, eps=1e-5):
+        """alpha * x + gate * (norm(block) * weight); the gate a vector [cols],
+        one value per row [rows, 1], a matrix, or absent."""
+        self._validate("residual_norm", op_type)
+        _norm_kind(norm)
+        s = tuple(x_shape)
+        if len(s) != 2 or tuple(block_shape) != s or tuple(weight_shape) != (s[1],):
+            raise NotImplementedError(f"residual_norm of {s}, {tuple(block_shape)} with weight "
+                                      f"{tuple(weight_shape)}")
+        if gate_name is None:
+            mode = "none"
+        elif tuple(gate_shape) == (s[1],):
+            mode = "channel"
+        elif tuple(gate_shape) == s:
+            mode = "full"
+        elif tuple(gate_shape) == (s[0], 1):
+            mode = "token"
+        else:
+            raise NotImplementedError(f"residual_norm gate {tuple(gate_shape)} for {s}")
+        return "", (op_type, name, x_name, block_name, weight_name, gate_name, int(s[0]),
+                    int(s[1]), norm, mode, float(alpha), float(eps))
+
+    def scaled_norm(self, op_type, name, tensor_name, weight_name, input_shape, weight_shape,
+                    norm="rms", eps=1e-5):
+        """norm(x) * weight along the last axis of a matrix."""
+        self._validate("scaled_norm", op_type)
+        _norm_kind(norm)
+        if len(input_shape) != 2 or tuple(weight_shape) != (input_shape[1],):
+            raise NotImplementedError(f"scaled_norm of {tuple(input_shape)} with weight "
+                                      f"{tuple(weight_shape)}")
+        return "", (op_type, name, tensor_name, weight_name, int(input_shape[0]),
+                    int(input_shape[1]), norm, float(eps))
 
     # -- data movement ---------------------------------------------------------
     def slice(self, op_type, name, tensor_name, slice_specs, input_shape, output_shape):

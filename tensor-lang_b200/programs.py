@@ -303,6 +303,66 @@ def mlp3_inputs(B=65536, I=1024, H=4096, C=10, seed=0, rows=None) -> Dict[str, n
 
 
 # ---------------------------------------------------------------------------
+# language-model head: last block boundary, head, both losses, SGD
+# ---------------------------------------------------------------------------
+
+def lm_head_train(B=256, D=128, V=1000, K=8, epochs=3, lr=0.05, norm="rms", gate="channel",
+                  temperature=2.0) -> list:
+    """A training loop over the end of a language model: a block (one linear
+    layer), the norms around it with its gate and the residual, then cross
+    entropy over the vocabulary and distillation from a teacher's top logits.
+    The operators have no .tl syntax: the program is an AST."""
+    gshape = {"channel": (D,), "token": (B, 1), "full": (B, D)}[gate]
+    ast = [
+        _let("x", _fill((B, D)), (B, D)),
+        _let("t", _fill((B,)), (B,)),
+        _let("top", _fill((B, K)), (B, K)),
+        _let("topi", _fill((B, K)), (B, K)),
+        _let("Wb", _fill((D, D)), (D, D), grad=True),
+        _let("bb", _fill((D,)), (D,), grad=True),
+        _let("wp", _fill((D,)), (D,), grad=True),
+        _let("g", _fill(gshape), gshape, grad=True),
+        _let("wn", _fill((D,)), (D,), grad=True),
+        _let("Wv", _fill((D, V)), (D, V), grad=True),
+        _let("bv", _fill((V,)), (V,), grad=True),
+        _let("lr", _lit([lr], (1, 1)), (1, 1)),
+        _let("lr1", _lit([lr], (1,)), (1,)),
+    ]
+    body = [
+        _let("u", _call("linear", "x", "Wb", "bb")),
+        _let("y", {"type": "residual_norm", "args": ["x", "u", "wp", "g"], "norm": norm,
+                   "alpha": 0.9, "eps": 1e-5}),
+        _let("n", {"type": "scaled_norm", "args": ["y", "wn"], "norm": norm, "eps": 1e-5}),
+        _let("ce", _call("linear_cross_entropy", "n", "Wv", "bv", "t")),
+        _let("z", _call("linear", "n", "Wv", "bv")),
+        _let("kd", {"type": "distill_topk", "args": ["z", "top", "topi"],
+                    "temperature": float(temperature)}),
+        _let("loss", _call("add", "ce", "kd")),
+        {"type": "backward", "loss_tensor": "loss"},
+    ]
+    params = [("Wb", 2), ("bb", 1), ("wp", 1), ("g", len(gshape)), ("wn", 1), ("Wv", 2), ("bv", 1)]
+    body += _sgd_lets(params)
+    body += [{"type": "rebind", "name": p, "expr": {"type": "name", "name": f"{p}_new"}}
+             for p, _ in params]
+    return ast + [{"type": "for", "loop_var": "i", "iterations": int(epochs), "body": body}]
+
+
+def lm_head_inputs(B=256, D=128, V=1000, K=8, gate="channel", seed=0) -> Dict[str, np.ndarray]:
+    rng = np.random.default_rng(seed)
+    f = lambda *s, a=1.0, b=0.0: (rng.standard_normal(s) * a + b).astype(np.float32)  # noqa: E731
+    gshape = {"channel": (D,), "token": (B, 1), "full": (B, D)}[gate]
+    d = {"x": f(B, D), "Wb": f(D, D, a=D ** -0.5), "bb": f(D, a=0.1), "wp": f(D, a=0.1, b=1.0),
+         "g": f(*gshape, a=0.5), "wn": f(D, a=0.1, b=1.0), "Wv": f(D, V, a=D ** -0.5),
+         "bv": f(V, a=0.1), "top": f(B, K, a=2.0, b=5.0)}
+    t = rng.integers(0, V, B)
+    t[rng.integers(0, B, B // 16)] = -100  # padding
+    ti = rng.integers(0, V, (B, K))
+    ti[np.arange(K)[None, :] >= rng.integers(1, K + 1, B)[:, None]] = -1
+    d["t"], d["topi"] = t.astype(np.float32), ti.astype(np.float32)
+    return d
+
+
+# ---------------------------------------------------------------------------
 # .tl source text of the same programs
 # ---------------------------------------------------------------------------
 

@@ -97,8 +97,10 @@ def out_shape(expr: dict, shapes: Dict[str, Shape]) -> Shape:
             return ()
         ax = int(ax) % len(s)
         return tuple(d for i, d in enumerate(s) if i != ax)
-    if t in ("mse_loss", "cross_entropy"):
+    if t in ("mse_loss", "cross_entropy", "linear_cross_entropy", "distill_topk"):
         return ()
+    if t in ("residual_norm", "scaled_norm"):
+        return _t(shapes[expr["args"][0]])
     if t == "transpose":
         s = _t(shapes[expr["tensor"]])
         axes = expr.get("axes")

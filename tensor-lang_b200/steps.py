@@ -19,6 +19,25 @@ from .region import Region, Seg, classify
 from .shapes import Shape, numel
 
 
+# tensors of this prefix are zero-filled when they are allocated: scratch of the
+# entry points that ask for it, one per entry point (their calls run one after
+# another on the program's stream)
+ZEROED = "__zeroed_"
+
+
+def zeroed_scratch(shapes: Dict[str, Shape], what: str, nbytes: int) -> str:
+    """The scratch tensor of entry point ``what``, large enough for this call."""
+    name = ZEROED + what
+    have = shapes.get(name, (0,))[0]
+    shapes[name] = (max(have, (int(nbytes) + 3) // 4),)
+    return name
+
+
+def lse_of(loss: str) -> str:
+    """The tensor in which a fused loss keeps its rows' log sums for backward."""
+    return f"__{loss}_lse"
+
+
 class Step:
     label = "step"
     reads: List[str] = []
@@ -190,6 +209,32 @@ def _vec_access(out_shape: Shape, arg_shape: Shape) -> str:
     return "col"
 
 
+_NORM = {"layer": rt.NORM_LAYER, "rms": rt.NORM_RMS}
+_GATE = {"none": rt.GATE_NONE, "channel": rt.GATE_CHANNEL, "token": rt.GATE_TOKEN,
+         "full": rt.GATE_FULL}
+
+
+def _ptr(name: Optional[str]):
+    return ("ptr", name) if name else ("null",)
+
+
+def norm_args(rows, cols, norm, x, u, w_post, gate, mode, alpha, w_pre, eps) -> list:
+    """The arguments tl_residual_norm and its backward begin with."""
+    return [("int", rt.F32), ("int", _NORM[norm]), ("int", rows), ("int", cols), ("ptr", x),
+            ("int", cols), _ptr(u), ("int", cols), _ptr(w_post), _ptr(gate),
+            ("int", _GATE[mode]), ("int", cols), ("float", alpha), _ptr(w_pre), ("float", eps)]
+
+
+def distill_args(shapes, z, teacher, index, rows, classes, top, tau, divisor, loss=None,
+                 upstream=None, dz=None, accumulate=0) -> list:
+    scratch = zeroed_scratch(shapes, "distill", rt.lib().tl_distill_topk_scratch_bytes(rows))
+    return [("int", rt.F32), ("int", rows), ("int", classes), ("int", top), ("ptr", z),
+            ("int", classes), ("ptr", teacher), ("int", top), ("ptr", index), ("int", top),
+            ("int", rt.IDX_F32), ("float", tau), ("float", divisor), _ptr(upstream), _ptr(loss),
+            ("null",), ("null",), _ptr(dz), ("int", classes), ("int", accumulate),
+            ("ptr", scratch), ("bytes", scratch)]
+
+
 def kinfo_to_step(k: tuple, shapes: Dict[str, Shape], divisor_scale: Optional[dict] = None) -> Step:
     kind = k[0]
     if kind == "general_broadcast":
@@ -303,6 +348,34 @@ def kinfo_to_step(k: tuple, shapes: Dict[str, Shape], divisor_scale: Optional[di
         return LibCall(f"cross_entropy:{name}", "tl_cross_entropy",
                        [("ptr", p), ("ptr", t), ("ptr", name), ("int", B), ("int", C),
                         ("int", 1 if kind.endswith("onehot") else 0), ("scratch",)], [p, t], [name])
+    if kind == "linear_cross_entropy":
+        x, w, b, t, rows, width, classes, divisor = k[2:10]
+        lse = lse_of(name)
+        shapes[lse] = (rows,)
+        scratch = zeroed_scratch(shapes, "linear_ce", rt.lib().tl_linear_ce_scratch_bytes(
+            rt.F32, 0, rows, classes, width, 1))
+        return LibCall(f"linear_cross_entropy:{name}", "tl_linear_ce",
+                       [("int", rt.F32), ("int", 0), ("int", rows), ("int", classes), ("int", width),
+                        ("ptr", x), ("int", width), ("ptr", w), ("int", classes), ("ptr", b),
+                        ("ptr", t), ("int", rt.IDX_F32), ("float", divisor), ("ptr", name),
+                        ("null",), ("ptr", lse), ("ptr", scratch), ("bytes", scratch)],
+                       [x, w, b, t], [name, lse, scratch])
+    if kind == "distill_topk":
+        z, tv, ti, rows, classes, top, tau, divisor = k[2:10]
+        return LibCall(f"distill_topk:{name}", "tl_distill_topk",
+                       distill_args(shapes, z, tv, ti, rows, classes, top, tau, divisor, loss=name),
+                       [z, tv, ti], [name, zeroed_scratch(shapes, "distill", 0)])
+    if kind == "residual_norm":
+        x, u, w, g, rows, cols, norm, mode, alpha, eps = k[2:12]
+        return LibCall(f"residual_norm:{name}", "tl_residual_norm",
+                       norm_args(rows, cols, norm, x, u, w, g, mode, alpha, None, eps) +
+                       [("ptr", name), ("int", cols), ("null",), ("int", cols)],
+                       [x, u, w] + ([g] if g else []), [name])
+    if kind == "scaled_norm":
+        x, w, rows, cols, norm, eps = k[2:8]
+        return LibCall(f"scaled_norm:{name}", "tl_residual_norm",
+                       norm_args(rows, cols, norm, x, None, None, None, "none", 1.0, w, eps) +
+                       [("null",), ("int", cols), ("ptr", name), ("int", cols)], [x, w], [name])
     if kind == "mse_loss":  # :1891-1943
         p, t, n = k[2], k[3], int(k[4])
         return LibCall(f"mse_loss:{name}", "tl_mse_loss",

@@ -150,3 +150,76 @@ def test_linear_ce_backward_refuses():
         ({"lse": None}, BAD), ({"dx": None, "dw": None, "dbias": None}, BAD), ({"lddx": 15}, BAD),
         ({"lddw": 99}, BAD), ({"acc": 8}, BAD), ({"dx": P}, BAD), ({"dw": 2 * P}, BAD), ({"dw": P}, BAD),
         ({"dx": 7 * P}, BAD), ({"nb": nb - 1}, BAD)])
+
+
+# -- lowering ----------------------------------------------------------------
+
+def _steps(P):
+    P._fuse_all()
+    return [s for s in P._all_steps() if hasattr(s, "fname")]
+
+
+def test_program_lowers_to_one_call_per_block_boundary():
+    """With a fetch list the two norms are one call in each direction."""
+    P = tl.Program(tl.programs.lm_head_train(B=64, D=32, V=100, K=4), None, fetch=["loss", "Wv"])
+    names = [s.fname for s in _steps(P)]
+    assert names.count("tl_residual_norm") == 1 and names.count("tl_residual_norm_backward") == 1
+    assert names.count("tl_linear_ce") == 1 and names.count("tl_linear_ce_backward") == 1
+    assert names.count("tl_distill_topk") == 2
+    b = next(s for s in P._all_steps() if getattr(s, "fname", "") == "tl_residual_norm_backward")
+    # y's gradient comes from n alone, so the fused call has no dy
+    assert b.args[15] == ("null",) and b.args[17] == ("ptr", "n_grad") and b.args[25][0] == "ptr"
+    # a kept gradient of y keeps the two calls apart
+    P = tl.Program(tl.programs.lm_head_train(B=64, D=32, V=100, K=4), None, fetch=["loss", "y_grad"])
+    names = [s.fname for s in _steps(P)]
+    assert names.count("tl_residual_norm") == 1 and names.count("tl_residual_norm_backward") == 2
+    P = tl.Program(tl.programs.lm_head_train(B=64, D=32, V=100, K=4), None, fuse_ops=False)
+    names = [s.fname for s in _steps(P)]
+    assert names.count("tl_residual_norm") == 2 and names.count("tl_residual_norm_backward") == 2
+
+
+def test_second_gradient_of_one_operand_gets_its_own_tensor():
+    """residual_norm(x, x, ...): one call may not write a gradient twice."""
+    L = tl.programs._let
+    ast = [L("x", tl.programs._fill((4, 8)), (4, 8), grad=True), L("w", tl.programs._fill((8,)), (8,)),
+           L("y", {"type": "residual_norm", "args": ["x", "x", "w"]}),
+           L("s", {"type": "sum", "tensor": "y", "axis": None}), {"type": "backward", "loss_tensor": "s"}]
+    P = tl.Program(ast, None, fetch=["x_grad"])
+    b = next(s for s in _steps(P) if s.fname == "tl_residual_norm_backward")
+    dx, du = b.args[19], b.args[21]
+    assert dx == ("ptr", "x_grad") and du[0] == "ptr" and du != dx
+
+
+def test_generator_refuses_shapes():
+    g = tl.KernelGenerator()
+    for f, a in [(g.linear_cross_entropy, ("x", "w", "b", "t", (4, 8), (9, 5), (4,))),
+                 (g.linear_cross_entropy, ("x", "w", "b", "t", (4, 8), (8, 5), (4, 5))),
+                 (g.distill_topk, ("z", "v", "i", (4, 8), (4, 3), (4, 2))),
+                 (g.distill_topk, ("z", "v", "i", (4, 8), (3, 2), (3, 2))),
+                 (g.residual_norm, ("x", "u", "w", None, (4, 8), (4, 7), (8,), None)),
+                 (g.residual_norm, ("x", "u", "w", "g", (4, 8), (4, 8), (8,), (4,))),
+                 (g.scaled_norm, ("x", "w", (4, 8), (4,)))]:
+        with pytest.raises(NotImplementedError):
+            f(f.__name__, "out", *a)
+    with pytest.raises(ValueError):
+        g.scaled_norm("scaled_norm", "n", "x", "w", (4, 8), (8,), norm="batch")
+    with pytest.raises(ValueError):
+        g.distill_topk("distill_topk", "l", "z", "v", "i", (4, 8), (4, 3), (4, 3), temperature=0.0)
+    with pytest.raises(ValueError):
+        g.linear_cross_entropy("linear_cross_entropy", "l", "x", "w", "b", "t", (4, 8), (8, 5), (4,),
+                               divisor=-1.0)
+    with pytest.raises(ValueError):
+        g.distill_topk("linear", "l", "z", "v", "i", (4, 8), (4, 3), (4, 3))
+
+
+def test_sharded_batches_name_their_divisor():
+    from tensor_lang_b200 import dp
+    ast = tl.programs.lm_head_train(B=64, D=32, V=100, K=4)
+    derived = dp.batch_derived(ast, ("x", "t", "top", "topi"))
+    assert {"n", "z"} <= derived and "ce" not in derived and "Wv_new" not in derived
+    with pytest.raises(NotImplementedError):
+        dp.check_loss_divisors(ast, derived)
+    for node in ast[-1]["body"]:
+        if node["type"] == "let" and node["expr"]["type"] in ("linear_cross_entropy", "distill_topk"):
+            node["expr"]["divisor"] = 64
+    dp.check_loss_divisors(ast, derived)
