@@ -76,6 +76,8 @@ struct TileParams {
   int terms;      // 1, or kTerms
   int kc;         // k-blocks per accumulation chunk
   int splits;     // K split this many ways (kSum)
+  int nt;         // columns of a tile: 256, or fewer where that fills the GPU better
+  int a_rows;     // rows of A that a CTA loads (K-major A): 128, or all that exist
   // kStats, kGrad
   const float* bias;      // of this piece's columns, or null
   const void* target;     // [M], of the whole vocabulary
@@ -132,11 +134,11 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t tile, int k) {
   d |= (uint64_t)2 << 61;  // 128-byte swizzle
   return d;
 }
-// kind::f16, bf16 operands, float32 accumulator, 256 x 256 over the CTA pair
+// kind::f16, bf16 operands, float32 accumulator, 256 x nt over the CTA pair
 template <int A_MN, int B_MN>
-constexpr uint32_t idesc() {
+__device__ __forceinline__ uint32_t idesc(int nt) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16) |
-         ((uint32_t)(256 >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+         ((uint32_t)(nt >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
 }
 
 struct Tile {
@@ -146,14 +148,14 @@ struct Tile {
 // shares a few row blocks of A and of B in L2); splits of K outermost.
 __device__ __forceinline__ Tile tile_of(const TileParams& p, int g) {
   constexpr int kBand = 8;
-  const int mt = (p.M + 255) / 256, nt = (p.N + 255) / 256, nk = (p.K + BK - 1) / BK;
+  const int mt = (p.M + 255) / 256, nt = (p.N + p.nt - 1) / p.nt, nk = (p.K + BK - 1) / BK;
   Tile t;
   t.split = g / (mt * nt);
   const int r = g - t.split * mt * nt;
   const int band = r / (kBand * nt), in = r - band * kBand * nt;
   const int rows = min(kBand, mt - band * kBand);
   t.m0 = (band * kBand + in % rows) * 256;
-  t.n0 = in / rows * 256;
+  t.n0 = in / rows * p.nt;
   t.kb0 = (int)((int64_t)t.split * nk / p.splits);
   t.nk = (int)((int64_t)(t.split + 1) * nk / p.splits) - t.kb0;
   return t;
@@ -242,7 +244,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tiles = p.splits * ((p.M + 255) / 256) * ((p.N + 255) / 256);
+  const int tiles = p.splits * ((p.M + 255) / 256) * ((p.N + p.nt - 1) / p.nt);
   const int step = (int)(gridDim.x >> 1), first = (int)(blockIdx.x >> 1);
 
   if (threadIdx.x == 0) {
@@ -279,7 +281,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       uint32_t it = 0;
       for (int g = first; g < tiles && ok; g += step) {
         const Tile t = tile_of(p, g);
-        const int m0 = t.m0 + 128 * (int)rank, n0 = t.n0 + 128 * (int)rank;
+        const int m0 = t.m0 + 128 * (int)rank, n0 = t.n0 + p.nt / 2 * (int)rank;
+        // rows of A that do not exist are not loaded: their results are not kept,
+        // whatever the stage holds there
+        const bool have_a = m0 < p.M;
+        const uint32_t a_bytes = TA == 0 ? (uint32_t)p.a_rows * 128u : (uint32_t)TILE_BYTES;
+        const uint32_t bytes = (t.m0 + 128 < p.M ? 2u : 1u) * a_bytes + (uint32_t)p.nt * 128u;
         for (int c = 0; c < t.nk && ok; c += p.kc) {
           const int cend = min(c + p.kc, t.nk);
           for (int q = 0; q < p.terms && ok; ++q) {
@@ -292,9 +299,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
               }
               const uint32_t sA = smem_u32(smem + s * 2 * TILE_BYTES), sB = sA + TILE_BYTES;
               const uint32_t fb = full0 + 8u * s;
-              if (leader) mbar_expect_tx(smem_u32(&full[s]), 4 * TILE_BYTES);
+              if (leader) mbar_expect_tx(smem_u32(&full[s]), bytes);
               const int k0 = (t.kb0 + kb) * BK;
-              if constexpr (TA == 0) {
+              if (!have_a) {
+              } else if constexpr (TA == 0) {
                 tma_load_3d_pair(sA, &tmA, fb, k0, m0, pa);
               } else {
                 tma_load_3d_pair(sA, &tmA, fb, m0, k0, pa);
@@ -304,7 +312,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 tma_load_3d_pair(sB, &tmB, fb, k0, n0, pb);
               } else {
                 tma_load_3d_pair(sB, &tmB, fb, n0, k0, pb);
-                tma_load_3d_pair(sB + 8192, &tmB, fb, n0 + 64, k0, pb);
+                if (p.nt > 128) tma_load_3d_pair(sB + 8192, &tmB, fb, n0 + 64, k0, pb);
               }
             }
           }
@@ -313,6 +321,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
     if (warp == 1 && leader && lane == 0) {
       // -------------------------------------------------------- MMA (leader)
+      const uint32_t id = idesc<TA, 1 - TB>(p.nt);
       bool ok = true;
       uint32_t it = 0, cg = 0;
       for (int g = first; g < tiles && ok; g += step) {
@@ -335,7 +344,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             const uint32_t sA = smem_u32(smem + s * 2 * TILE_BYTES), sB = sA + TILE_BYTES;
 #pragma unroll
             for (int k = 0; k < BK / 16; ++k)
-              mma2_bf16(acc, tile_desc<TA>(sA, k), tile_desc<1 - TB>(sB, k), idesc<TA, 1 - TB>(),
+              mma2_bf16(acc, tile_desc<TA>(sA, k), tile_desc<1 - TB>(sB, k), id,
                         (i == 0 && k == 0) ? 0u : 1u);
             mma2_commit_both(smem_u32(&empty[s]));
           }
@@ -381,7 +390,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       if (!ok) break;
       const int r0 = t.m0 + 128 * (int)rank + quarter * 32, row = r0 + lane;
       const int n0 = t.n0 + group * CW;
-      const int cols = min(CW, p.N - n0);  // of this warp; may be <= 0
+      const int cols = min(min(CW, p.nt - group * CW), p.N - n0);  // of this warp; may be <= 0
       if (r0 >= p.M || cols <= 0) continue;
       const bool live = row < p.M;
 
@@ -416,7 +425,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int j = 0; j < CW; ++j) s += exp_fast(v[j] - base);
           if (live) {
-            p.part[(int64_t)(n0 / CW) * p.part_ld + row] = make_float2(m, s);
+            p.part[(int64_t)(t.n0 / p.nt * (p.nt > CW ? 2 : 1) + group) * p.part_ld + row] = make_float2(m, s);
             if (target >= 0 && target < cols) {
               float z = 0.f;
 #pragma unroll
@@ -808,32 +817,77 @@ bool make_map3(CUtensorMap* m, const void* base, bool f32, int64_t planes, int64
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+constexpr int64_t up_to(int64_t n, int64_t k) { return (n + k - 1) / k * k; }
+
 // An operand in memory that TMA can address: bf16 planes.
 struct Planes {
   const __nv_bfloat16* p;
   int64_t planes, rows, cols, ld;
 };
 // as the K-major operand (stored [MN][K]) or the MN-major one ([K][MN])
-bool k_major(CUtensorMap* m, const Planes& x) {
-  return make_map3(m, x.p, false, x.planes, x.rows, x.cols, x.ld, 64, 128);
+bool k_major(CUtensorMap* m, const Planes& x, int box_rows) {
+  return make_map3(m, x.p, false, x.planes, x.rows, x.cols, x.ld, 64, (uint32_t)box_rows);
 }
 bool mn_major(CUtensorMap* m, const Planes& x) {
   return make_map3(m, x.p, false, x.planes, x.rows, x.cols, x.ld, 64, 64);
 }
 
+// Columns of a tile: 256, except
+//  - where half-size tiles still fit one wave of clusters: the narrowest that do
+//    (steps are what the epilogue's slabs and B's boxes allow);
+//  - between one and four waves of a K-major B: 224 or 192 where that ends
+//    sooner (a wave costs its tiles' columns and a fixed part worth about 32).
+//    Scoring 1 token x 32768 classes x 4096: 224 columns, 57 us; 256, 71 us.
+//    An MN-major B's boxes are 64 columns of 128 bytes: with 128-column tiles
+//    96 tokens x 65536 classes x 2048 took 90 us, with 256 60 us.
+template <int EPI>
+int tile_columns(int64_t M, int64_t N, int splits, bool b_mn_major) {
+  const int64_t slots = std::max(1, sm_count() / 2), mt = (M + 255) / 256 * splits;
+  const int64_t tiles = mt * ((N + 255) / 256);
+  if (tiles >= 4 * slots) return 256;
+  const int step = b_mn_major ? 128 : EPI == kStats || EPI == kSum ? 32 : 64;
+  if (2 * tiles <= slots) {
+    for (int nt = std::max(step, 64); nt < 256; nt += step)
+      if (mt * ((N + nt - 1) / nt) <= slots) return nt;
+    return 256;
+  }
+  if (b_mn_major) return 256;
+  int best = 256;
+  int64_t cost = INT64_MAX;
+  for (int nt = 256; nt >= 192; nt -= step) {
+    const int64_t waves = (mt * ((N + nt - 1) / nt) + slots - 1) / slots, c = waves * (nt + 32);
+    if (c < cost) {
+      cost = c;
+      best = nt;
+    }
+  }
+  return best;
+}
+
 template <int TA, int TB, int EPI>
-int launch_tiles(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c, const TileParams& p,
-                 cudaStream_t st) {
+int launch_tiles(const Planes& A, const Planes& B, const CUtensorMap& c, TileParams p, cudaStream_t st) {
   constexpr auto kern = vocab_tile_kernel<TA, TB, EPI>;
   TL_TRY((allow_smem<kern, SMEM_BYTES>()));
-  const int64_t tiles = (int64_t)p.splits * ((p.M + 255) / 256) * ((p.N + 255) / 256);
+  p.nt = tile_columns<EPI>(p.M, p.N, p.splits, TB == 0);
+  p.a_rows = TA == 0 ? (int)std::min<int64_t>(128, up_to(p.M, 8)) : 128;
+  CUtensorMap a, b;
+  if (!(TA == 0 ? k_major(&a, A, p.a_rows) : mn_major(&a, A)) ||
+      !(TB == 1 ? k_major(&b, B, p.nt / 2) : mn_major(&b, B)))
+    return TL_ERR_UNSUPPORTED;
+  const int64_t tiles = (int64_t)p.splits * ((p.M + 255) / 256) * ((p.N + p.nt - 1) / p.nt);
   if (tiles > INT32_MAX / 2) return TL_ERR_UNSUPPORTED;
   const int64_t clusters = std::min<int64_t>(tiles, std::max(1, sm_count() / 2));
   kern<<<(unsigned)(2 * clusters), THREADS, SMEM_BYTES, st>>>(a, b, c, p);
   return after_launch();
 }
 
-constexpr int64_t up_to(int64_t n, int64_t k) { return (n + k - 1) / k * k; }
+// The partials a product of kStats leaves per row: one for each epilogue warp's
+// columns, none for columns that do not exist.
+int stat_slots(int64_t M, int64_t N, bool b_mn_major) {
+  const int nt = tile_columns<kStats>(M, N, 1, b_mn_major);
+  const int64_t before = (N - 1) / nt;
+  return (int)(before * (nt > CW ? 2 : 1) + (N - before * nt > CW ? 2 : 1));
+}
 
 struct Call {
   int dtype, trans_w, index_type;
@@ -858,6 +912,7 @@ struct Call {
 // How a call is cut: classes per piece, and where its arrays are in scratch.
 struct Plan {
   int64_t fpiece, bpiece;          // classes per piece, forward and backward
+  int64_t dpiece;                  // the forward's where W is read where it is
   int64_t part_ld;                 // rows of the forward's partials
   int splits;                      // of K in dx
   int64_t xplanes, wplanes, zt, run, row_loss, part, g, sums, colsum, total;  // offsets
@@ -890,7 +945,8 @@ Plan make_plan(int dtype, int trans_w, int64_t rows, int64_t classes, int64_t wi
   q.part_ld = up_to(rows, 32);
   const int64_t cap = 512LL << 20;
   // the partials (8 bytes per row and 128 classes) and the terms of W
-  q.fpiece = std::min(piece(q.part_ld * 8 / CW, cap), piece(width * 2 * P, cap));
+  q.dpiece = piece(q.part_ld * 8 / CW, cap);
+  q.fpiece = std::min(q.dpiece, piece(width * 2 * P, cap));
   q.bpiece = std::min(piece(rows * 2 * P, cap), piece(width * 2 * P, cap));
   q.splits = backward ? dx_splits(rows, width, q.bpiece) : 1;
   int64_t at = 1024;
@@ -906,7 +962,10 @@ Plan make_plan(int dtype, int trans_w, int64_t rows, int64_t classes, int64_t wi
   q.zt = take(rows * 4);
   q.run = take(rows * 8);
   q.row_loss = take(rows * 4);
-  q.part = take(q.fpiece / CW * q.part_ld * 8);
+  // two per tile: of 256 columns, or of at least 64 where there are few tiles
+  // (tile_columns: less than 2 * sm_count() of 256)
+  const int64_t few = 16 * std::max(1, sm_count()) / ((rows + 255) / 256) + 8;
+  q.part = take((q.dpiece / CW + few) * q.part_ld * 8);
   q.total = at;
   if (backward) {
     at = common;
@@ -927,10 +986,15 @@ int write_planes(const T* X, int64_t ldx, int64_t rows, int64_t cols, int planes
   return after_launch();
 }
 
+// Whether TMA can address a matrix of the call's type as it is.
+bool direct(const Call& c, const void* X, int64_t ldx) {
+  return !c.f32() && ldx % 8 == 0 && aligned_to(X, 16);
+}
+
 // rows x cols of X as planes: itself where TMA can address it, else a copy
 int as_planes(const Call& c, const void* X, int64_t ldx, int64_t rows, int64_t cols, int64_t scratch_at,
               Planes* out) {
-  if (!c.f32() && ldx % 8 == 0 && aligned_to(X, 16)) {
+  if (direct(c, X, ldx)) {
     *out = {static_cast<const __nv_bfloat16*>(X), 1, rows, cols, ldx};
     return TL_OK;
   }
@@ -953,8 +1017,6 @@ int w_planes(const Call& c, const Plan& q, int64_t c0, int64_t n, Planes* out) {
 template <int EPI>
 int logits(const Call& c, const Planes& x, const Planes& w, const CUtensorMap& out, TileParams p,
            int64_t c0, int64_t n) {
-  CUtensorMap a, b;
-  if (!k_major(&a, x) || !(c.trans_w ? k_major(&b, w) : mn_major(&b, w))) return TL_ERR_UNSUPPORTED;
   p.M = (int)c.rows;
   p.N = (int)n;
   p.K = (int)c.width;
@@ -966,8 +1028,8 @@ int logits(const Call& c, const Planes& x, const Planes& w, const CUtensorMap& o
   p.index_type = c.index_type;
   p.classes = c.classes;
   p.col0 = (int)c0;
-  return c.trans_w ? launch_tiles<0, 1, EPI>(a, b, out, p, c.st)
-                   : launch_tiles<0, 0, EPI>(a, b, out, p, c.st);
+  return c.trans_w ? launch_tiles<0, 1, EPI>(x, w, out, p, c.st)
+                   : launch_tiles<0, 0, EPI>(x, w, out, p, c.st);
 }
 
 int forward(const Call& c, const Plan& q, float* loss, float* row_loss, float* lse) {
@@ -980,14 +1042,15 @@ int forward(const Call& c, const Plan& q, float* loss, float* row_loss, float* l
   if (!row_loss) row_loss = reinterpret_cast<float*>(c.scratch + q.row_loss);
   CUtensorMap none;
   memset(&none, 0, sizeof(none));
-  for (int64_t c0 = 0; c0 < c.classes; c0 += q.fpiece) {
-    const int64_t n = std::min(q.fpiece, c.classes - c0);
+  const int64_t piece = direct(c, c.w, c.ldw) ? q.dpiece : q.fpiece;
+  for (int64_t c0 = 0; c0 < c.classes; c0 += piece) {
+    const int64_t n = std::min(piece, c.classes - c0);
     TL_TRY(w_planes(c, q, c0, n, &w));
     TL_TRY(logits<kStats>(c, x, w, none, p, c0, n));
     // few rows: more threads for each
     auto join_rows = [&](auto kern, int64_t r) {
       kern<<<(unsigned)((c.rows + r - 1) / r), 256, 0, c.st>>>(
-          p.part, q.part_ld, (int)((n + CW - 1) / CW), c.targets(), p.zt,
+          p.part, q.part_ld, stat_slots(c.rows, n, !c.trans_w), c.targets(), p.zt,
           reinterpret_cast<float2*>(c.scratch + q.run), c0 == 0, c0 + n == c.classes, c.divisor, row_loss,
           lse, loss, reinterpret_cast<Head*>(c.scratch));
     };
@@ -1015,7 +1078,7 @@ int backward(const Call& c, const Plan& q, const float* lse, const float* upstre
     const int64_t n = std::min(q.bpiece, c.classes - c0);
     TL_TRY(w_planes(c, q, c0, n, &w));
     const Planes g{reinterpret_cast<__nv_bfloat16*>(c.scratch + q.g), c.planes(), c.rows, n, q.bpiece};
-    CUtensorMap a, b, o;
+    CUtensorMap o;
     if (!make_map3(&o, g.p, false, g.planes, g.rows, g.cols, g.ld, 64, 32)) return TL_ERR_UNSUPPORTED;
     TileParams p{};
       p.lse = lse;
@@ -1032,11 +1095,10 @@ int backward(const Call& c, const Plan& q, const float* lse, const float* upstre
       p.K = (int)n;
       p.splits = q.splits;
       p.add = c0 > 0;
-      if (!k_major(&a, g) || !(c.trans_w ? mn_major(&b, w) : k_major(&b, w)) ||
-          !make_map3(&o, sums, true, q.splits, c.rows, c.width, sums_ld, 32, 32))
+      if (!make_map3(&o, sums, true, q.splits, c.rows, c.width, sums_ld, 32, 32))
         return TL_ERR_UNSUPPORTED;
-      TL_TRY((c.trans_w ? launch_tiles<0, 0, kSum>(a, b, o, p, c.st)
-                        : launch_tiles<0, 1, kSum>(a, b, o, p, c.st)));
+      TL_TRY((c.trans_w ? launch_tiles<0, 0, kSum>(g, w, o, p, c.st)
+                        : launch_tiles<0, 1, kSum>(g, w, o, p, c.st)));
     }
     if (dW) {  // [classes][width] = g^T x, or [width][classes] = x^T g
       p.M = (int)(c.trans_w ? n : c.width);
@@ -1052,8 +1114,7 @@ int backward(const Call& c, const Plan& q, const float* lse, const float* upstre
                   make_map3(&o, p.out, c.f32(), 1, p.M, p.N, lddw, c.f32() ? 32 : 64, 32);
       const Planes& A = c.trans_w ? g : x;
       const Planes& B = c.trans_w ? x : g;
-      if (!mn_major(&a, A) || !mn_major(&b, B)) return TL_ERR_UNSUPPORTED;
-      TL_TRY((launch_tiles<1, 0, kOut>(a, b, o, p, c.st)));
+      TL_TRY((launch_tiles<1, 0, kOut>(A, B, o, p, c.st)));
     }
     if (dbias) {
       dbias_kernel<<<(unsigned)((n + 31) / 32), 256, 0, c.st>>>(
