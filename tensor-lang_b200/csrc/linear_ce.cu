@@ -57,7 +57,12 @@ constexpr int TILE_BYTES = 128 * BK * 2; // 16 KB: 128 rows of A, or of B, per C
 constexpr int NST = 6;
 constexpr int EPI_WARPS = 8;             // two per quarter of the rows
 constexpr int CW = 128;                  // columns of an epilogue warp
-constexpr int THREADS = 64 + 32 * EPI_WARPS;
+// Three warpgroups: loads and MMAs (and two idle warps), then the epilogue's two.
+// A launch of 384 threads gives each 168 registers; the first group keeps 72 and
+// the others take 216 (128 * 72 + 256 * 216 = 384 * 168): an epilogue thread holds
+// 128 sums, and with 168 registers it spilled (2 to 4% slower).
+constexpr int THREADS = 128 + 32 * EPI_WARPS;
+constexpr int kFewRegs = 72, kManyRegs = 216;
 constexpr int STG_TILE = 4096;           // per epilogue warp: 32 rows x 128 bytes
 constexpr int SMEM_BYTES = NST * 2 * TILE_BYTES + EPI_WARPS * STG_TILE + 1024 + 256;
 constexpr int TMEM_COLS = 512;
@@ -227,6 +232,14 @@ __device__ __forceinline__ float column_sum_of(const float* v, int lane) {
 }
 __device__ __forceinline__ float column_sum(const float* v, int lane) { return column_sum_of<32>(v, lane); }
 
+// The calls' kernels overlap their beginnings: each lets the next one start at
+// once (griddepcontrol.launch_dependents) and waits for the one before it, whose
+// results are visible then, before it touches memory.
+__device__ __forceinline__ void wait_for_previous_kernel() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // A: x, g or x^T ...; TA 0: stored [M][K], 1: [K][M].  TB 0: B stored [K][N], 1: [N][K].
 template <int TA, int TB, int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
@@ -247,6 +260,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   const int tiles = p.splits * ((p.M + 255) / 256) * ((p.N + p.nt - 1) / p.nt);
   const int step = (int)(gridDim.x >> 1), first = (int)(blockIdx.x >> 1);
 
+  if (threadIdx.x == 32) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmA) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmB) : "memory");
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < NST; ++s) {
       mbar_init(smem_u32(&full[s]), 1);
@@ -270,10 +287,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   cluster_sync_all();
   fence_after();
   const uint32_t tmem = *tmem_slot;
+  wait_for_previous_kernel();
 
   // The stage ring (it) and the two accumulators (cg) run on across tiles, so
   // the next tile's loads and MMAs overlap this one's epilogue.
-  if (warp < 2) {
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
     if (warp == 0 && lane == 0) {
       // ---------------------------------------------------------- producer
       const uint32_t full0 = mapa_shared(smem_u32(&full[0]), 0);
@@ -354,8 +373,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
     __syncwarp();
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegs));
     // ----------------------------------------------------------- epilogue
-    const int e = warp - 2, quarter = warp & 3, group = e >> 2;
+    const int e = warp - 4, quarter = warp & 3, group = e >> 2;
     const uint32_t free0 = mapa_shared(smem_u32(&acc_free[0]), 0);
     const uint32_t tbase = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(group * CW);
     float* stage = reinterpret_cast<float*>(staging + e * STG_TILE);
@@ -586,6 +606,7 @@ __device__ __forceinline__ int64_t count_targets(const Targets& t, long long* sh
 __global__ void __launch_bounds__(1024) scale_kernel(Targets t, float divisor, const float* upstream,
                                                      float* scale) {
   __shared__ long long sh[32];
+  wait_for_previous_kernel();
   float d = divisor;
   if (!(d > 0.f)) d = fmaxf(1.f, (float)count_targets(t, sh));
   if (threadIdx.x == 0) *scale = (upstream ? *upstream : 1.f) / d;
@@ -610,6 +631,7 @@ __global__ void __launch_bounds__(256) join_kernel(const float2* part, int64_t p
   __shared__ unsigned ticket;
   __shared__ long long shn[8];
   __shared__ double shd[8];
+  wait_for_previous_kernel();
   const int r = threadIdx.x % R, l = threadIdx.x / R;
   const int64_t row = (int64_t)blockIdx.x * R + r, rows = target.rows;
   float m = -INFINITY, s = 0.f;
@@ -715,6 +737,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) planes_kernel(const T* __restrict__ X, int64_t ldx, int64_t rows,
                                                      int64_t cols, int planes,
                                                      __nv_bfloat16* __restrict__ out, int64_t ld) {
+  wait_for_previous_kernel();
   const int64_t plane = rows * ld;
   for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
     const T* src = X + r * ldx;
@@ -736,6 +759,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) dx_kernel(const float* __restrict__ sums, int splits, int64_t rows,
                                                  int64_t cols, int64_t ld, const float* scale, T* dx,
                                                  int64_t lddx, int accumulate) {
+  wait_for_previous_kernel();
   const float k = *scale;
   const bool vec = cols % 4 == 0 && lddx % 4 == 0 && ((uintptr_t)dx & 15) == 0;
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
@@ -770,6 +794,7 @@ __global__ void __launch_bounds__(256) dbias_kernel(const float* __restrict__ co
                                                     int64_t cols, const float* scale, float* dbias,
                                                     int accumulate) {
   __shared__ float sh[8][33];
+  wait_for_previous_kernel();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
   float s = 0.f;
@@ -784,6 +809,24 @@ __global__ void __launch_bounds__(256) dbias_kernel(const float* __restrict__ co
 }
 
 // ------------------------------------------------------------- host side ---
+// A launch that may begin while the stream's previous kernel runs
+// (wait_for_previous_kernel).
+template <typename... P, typename... A>
+int launch(void (*kern)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  TL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...));
+  return after_launch();
+}
+
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                 const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -877,8 +920,7 @@ int launch_tiles(const Planes& A, const Planes& B, const CUtensorMap& c, TilePar
   const int64_t tiles = (int64_t)p.splits * ((p.M + 255) / 256) * ((p.N + p.nt - 1) / p.nt);
   if (tiles > INT32_MAX / 2) return TL_ERR_UNSUPPORTED;
   const int64_t clusters = std::min<int64_t>(tiles, std::max(1, sm_count() / 2));
-  kern<<<(unsigned)(2 * clusters), THREADS, SMEM_BYTES, st>>>(a, b, c, p);
-  return after_launch();
+  return launch(kern, dim3((unsigned)(2 * clusters)), THREADS, SMEM_BYTES, st, a, b, c, p);
 }
 
 // The partials a product of kStats leaves per row: one for each epilogue warp's
@@ -982,8 +1024,7 @@ int write_planes(const T* X, int64_t ldx, int64_t rows, int64_t cols, int planes
                  int64_t ld, cudaStream_t st) {
   const int64_t across = (ld / 8 + 255) / 256;
   const dim3 grid((unsigned)std::min<int64_t>(across, 16), (unsigned)std::min<int64_t>(rows, 65535));
-  planes_kernel<T><<<grid, 256, 0, st>>>(X, ldx, rows, cols, planes, out, ld);
-  return after_launch();
+  return launch(planes_kernel<T>, grid, 256, 0, st, X, ldx, rows, cols, planes, out, ld);
 }
 
 // Whether TMA can address a matrix of the call's type as it is.
@@ -1049,16 +1090,12 @@ int forward(const Call& c, const Plan& q, float* loss, float* row_loss, float* l
     TL_TRY(logits<kStats>(c, x, w, none, p, c0, n));
     // few rows: more threads for each
     auto join_rows = [&](auto kern, int64_t r) {
-      kern<<<(unsigned)((c.rows + r - 1) / r), 256, 0, c.st>>>(
-          p.part, q.part_ld, stat_slots(c.rows, n, !c.trans_w), c.targets(), p.zt,
+      return launch(
+          kern, dim3((unsigned)((c.rows + r - 1) / r)), 256, 0, c.st, p.part, q.part_ld, stat_slots(c.rows, n, !c.trans_w), c.targets(), p.zt,
           reinterpret_cast<float2*>(c.scratch + q.run), c0 == 0, c0 + n == c.classes, c.divisor, row_loss,
           lse, loss, reinterpret_cast<Head*>(c.scratch));
     };
-    if (c.rows >= 4096)
-      join_rows(join_kernel<32>, 32);
-    else
-      join_rows(join_kernel<4>, 4);
-    TL_TRY(after_launch());
+    TL_TRY(c.rows >= 4096 ? join_rows(join_kernel<32>, 32) : join_rows(join_kernel<4>, 4));
   }
   return TL_OK;
 }
@@ -1066,8 +1103,7 @@ int forward(const Call& c, const Plan& q, float* loss, float* row_loss, float* l
 int backward(const Call& c, const Plan& q, const float* lse, const float* upstream, void* dx, int64_t lddx,
              void* dW, int64_t lddw, float* dbias, int accumulate) {
   float* scale = &reinterpret_cast<Head*>(c.scratch)->scale;
-  scale_kernel<<<1, 1024, 0, c.st>>>(c.targets(), c.divisor, upstream, scale);
-  TL_TRY(after_launch());
+  TL_TRY(launch(scale_kernel, dim3(1), 1024, 0, c.st, c.targets(), c.divisor, upstream, scale));
   Planes x, w;
   TL_TRY(as_planes(c, c.x, c.ldx, c.rows, c.width, q.xplanes, &x));
   const int64_t es = (int64_t)elem_bytes(c.dtype);
@@ -1117,22 +1153,18 @@ int backward(const Call& c, const Plan& q, const float* lse, const float* upstre
       TL_TRY((launch_tiles<1, 0, kOut>(A, B, o, p, c.st)));
     }
     if (dbias) {
-      dbias_kernel<<<(unsigned)((n + 31) / 32), 256, 0, c.st>>>(
-          colsum, up_to(c.rows, 32) / 32, n, scale, dbias + c0, accumulate & TL_ACC_DBIAS);
-      TL_TRY(after_launch());
+      TL_TRY(launch(dbias_kernel, dim3((unsigned)((n + 31) / 32)), 256, 0, c.st, colsum, up_to(c.rows, 32) / 32,
+                    n, scale, dbias + c0, accumulate & TL_ACC_DBIAS));
     }
   }
   if (dx) {
     const int64_t blocks = std::min<int64_t>(c.rows, 32LL * sm_count());
     if (c.f32())
-      dx_kernel<float><<<(unsigned)blocks, 256, 0, c.st>>>(sums, q.splits, c.rows, c.width, sums_ld, scale,
-                                                           static_cast<float*>(dx), lddx,
-                                                           accumulate & TL_ACC_DX);
+      TL_TRY(launch(dx_kernel<float>, dim3((unsigned)blocks), 256, 0, c.st, sums, q.splits, c.rows, c.width,
+                    sums_ld, scale, static_cast<float*>(dx), lddx, accumulate & TL_ACC_DX));
     else
-      dx_kernel<__nv_bfloat16><<<(unsigned)blocks, 256, 0, c.st>>>(
-          sums, q.splits, c.rows, c.width, sums_ld, scale, static_cast<__nv_bfloat16*>(dx), lddx,
-          accumulate & TL_ACC_DX);
-    TL_TRY(after_launch());
+      TL_TRY(launch(dx_kernel<__nv_bfloat16>, dim3((unsigned)blocks), 256, 0, c.st, sums, q.splits, c.rows,
+                    c.width, sums_ld, scale, static_cast<__nv_bfloat16*>(dx), lddx, accumulate & TL_ACC_DX));
   }
   return TL_OK;
 }
