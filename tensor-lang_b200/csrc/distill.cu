@@ -149,6 +149,7 @@ __device__ __forceinline__ bool row_counts(const DistillArgs& a, int64_t r) {
 // Rows with a valid entry, one warp per row.
 template <typename T>
 __global__ void __launch_bounds__(256) distill_count_kernel(DistillArgs a) {
+  wait_for_previous_kernel();
   const int lane = threadIdx.x & 31;
   unsigned n = 0;
   for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < a.rows; r += 8LL * gridDim.x)
@@ -190,6 +191,7 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   T* cell = cells + phase;
   const int head = min(n, phase ? V - phase : 0), mid = (n - head) / V * V;
   if (size > 1) cluster_arrive_relaxed();  // every CTA of the cluster runs: waited for before the exchange
+  wait_for_previous_kernel();
 
   // each thread brings in what it reads in the first pass, so waiting for its
   // own copies is enough; the row's ends, outside the 16-byte copies, are one
@@ -467,6 +469,7 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
 // The mean, in double, and the counter cleared for the next call.
 __global__ void __launch_bounds__(1024) distill_mean_kernel(DistillArgs a) {
   __shared__ double sh[32];
+  wait_for_previous_kernel();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   double t = 0.0;
   if (a.loss)
@@ -497,24 +500,12 @@ int cluster_for(int64_t rows, int64_t classes) {
 }
 
 template <typename T, int NT, bool ALONE>
-int launch(const DistillArgs& a, int cluster, cudaStream_t st) {
+int launch_rows(const DistillArgs& a, int cluster, cudaStream_t st) {
   const size_t smem = (size_t)a.top * 16 + (size_t)mark_words((int)a.seg, 16 / sizeof(T)) * 4 + 16 +
                       (size_t)a.seg * sizeof(T) + 16;
   constexpr auto kern = distill_kernel<T, NT, ALONE>;
   TL_TRY((allow_smem<kern, kSmemMost>()));
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(a.rows * cluster));
-  cfg.blockDim = dim3(NT);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = (unsigned)cluster;
-  at.val.clusterDim.y = at.val.clusterDim.z = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  TL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, a));
-  return after_launch();
+  return launch_in_clusters(cluster, kern, dim3((unsigned)(a.rows * cluster)), NT, smem, st, a);
 }
 
 template <typename T>
@@ -523,8 +514,7 @@ int run(DistillArgs a, cudaStream_t st) {
   const bool alone = a.rows <= 16 && a.rows * a.top <= 4096;
   if (a.divisor == 0.f && !alone) {
     const int64_t blocks = std::min<int64_t>((a.rows + 7) / 8, 4LL * sm_count());
-    distill_count_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(a);
-    TL_TRY(after_launch());
+    TL_TRY(launch(distill_count_kernel<T>, dim3((unsigned)blocks), 256, 0, st, a));
   }
   constexpr int64_t V = 16 / sizeof(T);
   const int cluster = cluster_for(a.rows, a.classes);
@@ -532,14 +522,13 @@ int run(DistillArgs a, cudaStream_t st) {
   a.seg = ((a.classes + cluster - 1) / cluster + 31) / 32 * 32;
   static_assert(32 % V == 0, "aligned segments");
   if (alone)
-    return a.seg <= 2048 ? launch<T, 128, true>(a, cluster, st) : launch<T, 256, true>(a, cluster, st);
+    return a.seg <= 2048 ? launch_rows<T, 128, true>(a, cluster, st) : launch_rows<T, 256, true>(a, cluster, st);
   if (a.seg <= 2048)
-    TL_TRY((launch<T, 128, false>(a, cluster, st)));
+    TL_TRY((launch_rows<T, 128, false>(a, cluster, st)));
   else
-    TL_TRY((launch<T, 256, false>(a, cluster, st)));
+    TL_TRY((launch_rows<T, 256, false>(a, cluster, st)));
   if (a.loss || a.divisor == 0.f) {
-    distill_mean_kernel<<<1, 1024, 0, st>>>(a);
-    TL_TRY(after_launch());
+    TL_TRY(launch(distill_mean_kernel, dim3(1), 1024, 0, st, a));
   }
   return TL_OK;
 }

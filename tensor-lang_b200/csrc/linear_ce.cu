@@ -232,14 +232,6 @@ __device__ __forceinline__ float column_sum_of(const float* v, int lane) {
 }
 __device__ __forceinline__ float column_sum(const float* v, int lane) { return column_sum_of<32>(v, lane); }
 
-// The calls' kernels overlap their beginnings: each lets the next one start at
-// once (griddepcontrol.launch_dependents) and waits for the one before it, whose
-// results are visible then, before it touches memory.
-__device__ __forceinline__ void wait_for_previous_kernel() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
 // A: x, g or x^T ...; TA 0: stored [M][K], 1: [K][M].  TB 0: B stored [K][N], 1: [N][K].
 template <int TA, int TB, int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
@@ -809,24 +801,6 @@ __global__ void __launch_bounds__(256) dbias_kernel(const float* __restrict__ co
 }
 
 // ------------------------------------------------------------- host side ---
-// A launch that may begin while the stream's previous kernel runs
-// (wait_for_previous_kernel).
-template <typename... P, typename... A>
-int launch(void (*kern)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  TL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...));
-  return after_launch();
-}
-
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                 const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,

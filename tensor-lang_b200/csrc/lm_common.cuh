@@ -61,6 +61,14 @@ __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162flo
 __device__ __forceinline__ void from_f32(float* p, float x) { *p = x; }
 __device__ __forceinline__ void from_f32(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
+// The kernels of these operators overlap their beginnings: each lets the next one start at
+// once (griddepcontrol.launch_dependents) and waits for the one before it, whose
+// results are visible then, before it touches memory.
+__device__ __forceinline__ void wait_for_previous_kernel() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // Class index i of an index array (TL_IDX_*), or -1 when it is not in [0, n):
 // such entries take no part.  A float index is the class the value names
 // exactly (cross_entropy's class-index targets, kernel_generator.py:1816-1885,
@@ -92,6 +100,32 @@ int allow_smem() {
   if (dev < 64) done.fetch_or(1ull << dev);
   return TL_OK;
 }
+// A launch that may begin while the stream's previous kernel runs
+// (wait_for_previous_kernel), in clusters of `cluster` CTAs.
+template <typename... P, typename... A>
+int launch_in_clusters(int cluster, void (*kern)(P...), dim3 grid, int threads, size_t smem,
+                       cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2] = {};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  TL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...));
+  return after_launch();
+}
+template <typename... P, typename... A>
+int launch(void (*kern)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+  return launch_in_clusters(1, kern, grid, threads, smem, st, args...);
+}
+
 inline bool aligned_to(const void* p, size_t n) { return ((uintptr_t)p % n) == 0; }
 inline size_t elem_bytes(int dtype) { return dtype == TL_BF16 ? 2 : 4; }
 inline bool dtype_ok(int dtype) { return dtype == TL_F32 || dtype == TL_BF16; }
