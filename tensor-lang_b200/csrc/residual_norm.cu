@@ -112,13 +112,18 @@ struct RowIo {
   static constexpr int E = VEC * NV, H = E / 2;
   int cols;  // at most 16 * NT
   int t;
-  __device__ __forceinline__ int at(int j) const { return (j * NT + t) * VEC; }
-  __device__ __forceinline__ bool in(int i) const { return at(i / VEC) < cols; }
-  __device__ __forceinline__ bool full() const { return at(NV - 1) < cols; }
+  int left;  // cols - t * VEC: vector j exists where j * NT * VEC is below
+  __device__ __forceinline__ RowIo(int cols_, int t_) : cols(cols_), t(t_), left(cols_ - t_ * VEC) {}
+  __device__ __forceinline__ bool has(int j) const { return j * NT * VEC < left; }
+  __device__ __forceinline__ bool in(int i) const { return has(i / VEC); }
+  __device__ __forceinline__ bool full() const { return has(NV - 1); }
+  // column of element i
+  __device__ __forceinline__ int col(int i) const { return ((i / VEC) * NT + t) * VEC + i % VEC; }
   __device__ __forceinline__ void store(T* p, const float2 (&v)[H], bool add) const {
+    p += t * VEC;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (at(j) >= cols) continue;
+      if (!has(j)) continue;
       float q[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
@@ -127,11 +132,11 @@ struct RowIo {
       }
       if (add) {
         float o[VEC];
-        ld_vec<VEC>(p + at(j), o);
+        ld_vec<VEC>(p + j * NT * VEC, o);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) q[i] += o[i];
       }
-      st_vec<VEC>(p + at(j), q);
+      st_vec<VEC>(p + j * NT * VEC, q);
     }
   }
 };
@@ -195,18 +200,18 @@ struct Ahead {
 #pragma unroll
         for (int q = 0; q < NA; ++q) {
           if (!p[q]) continue;
-          const T* src = static_cast<const T*>(p[q]) + r * ld[q];
-          unsigned char* dst = buf + (slot * na + q) * kArray + io.t * kBytes;
+          const T* src = static_cast<const T*>(p[q]) + r * ld[q] + io.t * VEC;
+          const uint32_t dst = (uint32_t)__cvta_generic_to_shared(buf + (slot * na + q) * kArray +
+                                                                  io.t * kBytes);
 #pragma unroll
           for (int j = 0; j < NV; ++j) {
-            if (io.at(j) >= io.cols) continue;
-            const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst + j * NT * kBytes);
+            if (!io.has(j)) continue;
+            const uint32_t d = dst + j * NT * kBytes;
+            const T* from = src + j * NT * VEC;
             if constexpr (kBytes == 16)
-              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src + io.at(j))
-                           : "memory");
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(from) : "memory");
             else
-              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d), "l"(src + io.at(j))
-                           : "memory");
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d), "l"(from) : "memory");
           }
         }
       }
@@ -229,13 +234,13 @@ struct Ahead {
   __device__ __forceinline__ void load(const Io& io, int q, int64_t r, int slot,
                                        float2 (&v)[Io::H]) const {
     const T* src = kStaged ? reinterpret_cast<const T*>(buf + (slot * na + q) * kArray + io.t * kBytes)
-                           : static_cast<const T*>(p[q]) + r * ld[q];
+                           : static_cast<const T*>(p[q]) + r * ld[q] + io.t * VEC;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       float e[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) e[i] = 0.f;
-      if (io.at(j) < io.cols) ld_vec<VEC>(kStaged ? src + j * NT * VEC : src + io.at(j), e);
+      if (io.has(j)) ld_vec<VEC>(src + j * NT * VEC, e);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         const int k = j * VEC + i;
@@ -260,7 +265,7 @@ struct RowWeights {
       float e[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int c = io.at((4 * i + k) / VEC) + (4 * i + k) % VEC;
+        const int c = io.col(4 * i + k);
         e[k] = c < io.cols ? (w ? to_f32(w[c]) : 1.f) * (g ? to_f32(g[c]) : 1.f) : 0.f;
       }
       p[i * NT + io.t] = make_float4(e[0], e[1], e[2], e[3]);
@@ -286,7 +291,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) residual_norm_kernel(NormArgs a
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ float sh[2 * 3 * (NT / 32)];
   RowSum<NT> sum{sh};
-  const Io io{(int)a.cols, (int)threadIdx.x};
+  const Io io((int)a.cols, (int)threadIdx.x);
   const float inv_c = 1.f / (float)a.cols;
   const bool full_gate = a.gate_mode == TL_GATE_FULL;
   const Ahead<T, NT, VEC, NV, 3> rows{{a.x, a.u, full_gate ? a.gate : nullptr}, {a.ldx, a.ldu, a.ldg},
@@ -354,7 +359,7 @@ __global__ void __launch_bounds__(NT, NT <= 256 ? 512 / NT : 1)
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ float sh[2 * 3 * (NT / 32)];
   RowSum<NT> sum{sh};
-  const Io io{(int)a.cols, (int)threadIdx.x};
+  const Io io((int)a.cols, (int)threadIdx.x);
   const bool full_gate = a.gate_mode == TL_GATE_FULL, token_gate = a.gate_mode == TL_GATE_TOKEN;
   const Ahead<T, NT, VEC, NV, 5> rows{{a.u, a.x, a.dn, a.dy, full_gate ? a.gate : nullptr},
                                       {a.ldu, a.ldx, a.lddn, a.lddy, a.ldg},
@@ -516,8 +521,8 @@ __global__ void __launch_bounds__(NT, NT <= 256 ? 512 / NT : 1)
   float* part = a.part + (int64_t)blockIdx.x * 2 * a.cols;
 #pragma unroll
   for (int i = 0; i < Io::E; ++i) {
-    const int64_t c = io.at(i / VEC) + i % VEC;
-    if (c >= a.cols) continue;
+    const int c = io.col(i);
+    if (c >= io.cols) continue;
     part[c] = i & 1 ? s_post[i / 2].y : s_post[i / 2].x;
     part[a.cols + c] = i & 1 ? s_pre[i / 2].y : s_pre[i / 2].x;
   }
