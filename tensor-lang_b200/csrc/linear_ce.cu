@@ -95,6 +95,9 @@ struct TileParams {
   const float* lse;       // kGrad
   float* colsum;          // kGrad: [M / 32 rounded up][N] sums of g, or null
   int planes;             // kGrad: terms of g (1 or 3)
+  float divisor;          // kGrad: an idle warp writes upstream / divisor (0: rows with
+  const float* upstream;  // a target) to *scale_out, where that is not null
+  float* scale_out;
   // kSum
   int add;                // add to the sums there
   // kOut
@@ -363,6 +366,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         }
       }
     }
+    if (EPI == kGrad && warp == 2 && blockIdx.x == 0 && p.scale_out) {
+      int n = 0;
+#pragma unroll 4
+      for (int i = lane; i < p.M; i += 32) n += class_index(p.target, p.index_type, i, p.classes) >= 0;
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (lane == 0)
+        *p.scale_out = (p.upstream ? *p.upstream : 1.f) / (p.divisor > 0.f ? p.divisor : fmaxf(1.f, (float)n));
+    }
     __syncwarp();
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegs));
@@ -592,16 +603,6 @@ __device__ __forceinline__ int64_t count_targets(const Targets& t, long long* sh
   n = 0;
   for (unsigned i = 0; i < blockDim.x / 32; ++i) n += sh[i];
   return n;
-}
-
-// scale = upstream / divisor
-__global__ void __launch_bounds__(1024) scale_kernel(Targets t, float divisor, const float* upstream,
-                                                     float* scale) {
-  __shared__ long long sh[32];
-  wait_for_previous_kernel();
-  float d = divisor;
-  if (!(d > 0.f)) d = fmaxf(1.f, (float)count_targets(t, sh));
-  if (threadIdx.x == 0) *scale = (upstream ? *upstream : 1.f) / d;
 }
 
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
@@ -1077,7 +1078,6 @@ int forward(const Call& c, const Plan& q, float* loss, float* row_loss, float* l
 int backward(const Call& c, const Plan& q, const float* lse, const float* upstream, void* dx, int64_t lddx,
              void* dW, int64_t lddw, float* dbias, int accumulate) {
   float* scale = &reinterpret_cast<Head*>(c.scratch)->scale;
-  TL_TRY(launch(scale_kernel, dim3(1), 1024, 0, c.st, c.targets(), c.divisor, upstream, scale));
   Planes x, w;
   TL_TRY(as_planes(c, c.x, c.ldx, c.rows, c.width, q.xplanes, &x));
   const int64_t es = (int64_t)elem_bytes(c.dtype);
@@ -1093,6 +1093,9 @@ int backward(const Call& c, const Plan& q, const float* lse, const float* upstre
     TileParams p{};
       p.lse = lse;
     p.planes = c.planes();
+    p.divisor = c.divisor;
+    p.upstream = upstream;
+    p.scale_out = c0 == 0 ? scale : nullptr;
     p.colsum = dbias ? colsum : nullptr;
     TL_TRY(logits<kGrad>(c, x, w, o, p, c0, n));
     p = TileParams{};
