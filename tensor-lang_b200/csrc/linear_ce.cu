@@ -54,7 +54,10 @@ namespace {
 
 constexpr int BK = 64;                   // bf16 per stage row: 128 bytes
 constexpr int TILE_BYTES = 128 * BK * 2; // 16 KB: 128 rows of A, or of B, per CTA
-constexpr int NST = 6;
+// The ring of operand stages: six of 32 KB, or more where tiles are narrow or A has
+// few rows, so that as many bytes are on their way.
+constexpr int RING_BYTES = 6 * 2 * TILE_BYTES;
+constexpr int MAX_STAGES = 24;
 constexpr int EPI_WARPS = 8;             // two per quarter of the rows
 constexpr int CW = 128;                  // columns of an epilogue warp
 // Three warpgroups: loads and MMAs (and two idle warps), then the epilogue's two.
@@ -64,7 +67,7 @@ constexpr int CW = 128;                  // columns of an epilogue warp
 constexpr int THREADS = 128 + 32 * EPI_WARPS;
 constexpr int kFewRegs = 72, kManyRegs = 216;
 constexpr int STG_TILE = 4096;           // per epilogue warp: 32 rows x 128 bytes
-constexpr int SMEM_BYTES = NST * 2 * TILE_BYTES + EPI_WARPS * STG_TILE + 1024 + 256;
+constexpr int SMEM_BYTES = RING_BYTES + EPI_WARPS * STG_TILE + 1024 + 512;
 constexpr int TMEM_COLS = 512;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
 
@@ -83,6 +86,8 @@ struct TileParams {
   int splits;     // K split this many ways (kSum)
   int nt;         // columns of a tile: 256, or fewer where that fills the GPU better
   int a_rows;     // rows of A that a CTA loads (K-major A): 128, or all that exist
+  int stages;     // of the ring, stage_bytes apart, B's half of a stage at b_at
+  int stage_bytes, b_at;
   // kStats, kGrad
   const float* bias;      // of this piece's columns, or null
   const void* target;     // [M], of the whole vocabulary
@@ -242,10 +247,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                       const __grid_constant__ CUtensorMap tmC, const TileParams p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  unsigned char* staging = smem + NST * 2 * TILE_BYTES;
-  uint64_t* full = (uint64_t*)(staging + EPI_WARPS * STG_TILE);  // [NST] loads of both CTAs -> MMA
-  uint64_t* empty = full + NST;                                  // [NST] MMA -> each producer
-  uint64_t* acc_full = empty + NST;                              // [2] MMA -> each epilogue
+  unsigned char* staging = smem + RING_BYTES;
+  uint64_t* full = (uint64_t*)(staging + EPI_WARPS * STG_TILE);  // [stages] loads of both CTAs -> MMA
+  uint64_t* empty = full + MAX_STAGES;                           // [stages] MMA -> each producer
+  uint64_t* acc_full = empty + MAX_STAGES;                       // [2] MMA -> each epilogue
   uint64_t* acc_free = acc_full + 2;                             // [2] both epilogues -> MMA
   uint32_t* tmem_slot = (uint32_t*)(acc_free + 2);
 
@@ -260,7 +265,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmB) : "memory");
   }
   if (threadIdx.x == 0) {
-    for (int s = 0; s < NST; ++s) {
+    for (int s = 0; s < p.stages; ++s) {
       mbar_init(smem_u32(&full[s]), 1);
       mbar_init(smem_u32(&empty[s]), 1);
     }
@@ -284,15 +289,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   const uint32_t tmem = *tmem_slot;
   wait_for_previous_kernel();
 
-  // The stage ring (it) and the two accumulators (cg) run on across tiles, so
-  // the next tile's loads and MMAs overlap this one's epilogue.
+  // The stage ring (s, with the parity of its turn) and the two accumulators (cg)
+  // run on across tiles, so the next tile's loads and MMAs overlap this one's
+  // epilogue.
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
     if (warp == 0 && lane == 0) {
       // ---------------------------------------------------------- producer
       const uint32_t full0 = mapa_shared(smem_u32(&full[0]), 0);
       bool ok = true;
-      uint32_t it = 0;
+      int s = 0;
+      uint32_t turn = 0;
       for (int g = first; g < tiles && ok; g += step) {
         const Tile t = tile_of(p, g);
         const int m0 = t.m0 + 128 * (int)rank, n0 = t.n0 + p.nt / 2 * (int)rank;
@@ -305,14 +312,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           const int cend = min(c + p.kc, t.nk);
           for (int q = 0; q < p.terms && ok; ++q) {
             const int pa = p.terms == 1 ? 0 : kTermA[q], pb = p.terms == 1 ? 0 : kTermB[q];
-            for (int kb = c; kb < cend; ++kb, ++it) {
-              const uint32_t s = it % NST, ph = (it / NST) & 1;
-              if (it >= NST && !mbar_wait(smem_u32(&empty[s]), ph ^ 1)) {
+            for (int kb = c; kb < cend; ++kb) {
+              if (turn > 0 && !mbar_wait(smem_u32(&empty[s]), (turn & 1) ^ 1)) {
                 ok = false;
                 break;
               }
-              const uint32_t sA = smem_u32(smem + s * 2 * TILE_BYTES), sB = sA + TILE_BYTES;
-              const uint32_t fb = full0 + 8u * s;
+              const uint32_t sA = smem_u32(smem + s * p.stage_bytes), sB = sA + (uint32_t)p.b_at;
+              const uint32_t fb = full0 + 8u * (uint32_t)s;
               if (leader) mbar_expect_tx(smem_u32(&full[s]), bytes);
               const int k0 = (t.kb0 + kb) * BK;
               if (!have_a) {
@@ -328,6 +334,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 tma_load_3d_pair(sB, &tmB, fb, n0, k0, pb);
                 if (p.nt > 128) tma_load_3d_pair(sB + 8192, &tmB, fb, n0 + 64, k0, pb);
               }
+              if (++s == p.stages) {
+                s = 0;
+                ++turn;
+              }
             }
           }
         }
@@ -337,7 +347,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       // -------------------------------------------------------- MMA (leader)
       const uint32_t id = idesc<TA, 1 - TB>(p.nt);
       bool ok = true;
-      uint32_t it = 0, cg = 0;
+      int s = 0;
+      uint32_t turn = 0, cg = 0;
       for (int g = first; g < tiles && ok; g += step) {
         const Tile t = tile_of(p, g);
         for (int c = 0; c < t.nk && ok; c += p.kc, ++cg) {
@@ -348,19 +359,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             break;
           }
           fence_after();
-          for (int i = 0; i < n; ++i, ++it) {
-            const uint32_t s = it % NST, ph = (it / NST) & 1;
-            if (!mbar_wait(smem_u32(&full[s]), ph)) {
+          for (int i = 0; i < n; ++i) {
+            if (!mbar_wait(smem_u32(&full[s]), turn & 1)) {
               ok = false;
               break;
             }
             fence_after();
-            const uint32_t sA = smem_u32(smem + s * 2 * TILE_BYTES), sB = sA + TILE_BYTES;
+            const uint32_t sA = smem_u32(smem + s * p.stage_bytes), sB = sA + (uint32_t)p.b_at;
 #pragma unroll
             for (int k = 0; k < BK / 16; ++k)
               mma2_bf16(acc, tile_desc<TA>(sA, k), tile_desc<1 - TB>(sB, k), id,
                         (i == 0 && k == 0) ? 0u : 1u);
             mma2_commit_both(smem_u32(&empty[s]));
+            if (++s == p.stages) {
+              s = 0;
+              ++turn;
+            }
           }
           mma2_commit_both(smem_u32(&acc_full[b]));
         }
@@ -888,6 +902,11 @@ int launch_tiles(const Planes& A, const Planes& B, const CUtensorMap& c, TilePar
   TL_TRY((allow_smem<kern, SMEM_BYTES>()));
   p.nt = tile_columns<EPI>(p.M, p.N, p.splits, TB == 0);
   p.a_rows = TA == 0 ? (int)std::min<int64_t>(128, up_to(p.M, 8)) : 128;
+  // the MMA reads 128 rows of A from a stage's start: past the loaded ones what
+  // follows in shared memory, whose products are not kept
+  p.b_at = p.a_rows * 128;
+  p.stage_bytes = p.b_at + p.nt / 2 * 128;
+  p.stages = std::min(MAX_STAGES, RING_BYTES / p.stage_bytes);
   CUtensorMap a, b;
   if (!(TA == 0 ? k_major(&a, A, p.a_rows) : mn_major(&a, A)) ||
       !(TB == 1 ? k_major(&b, B, p.nt / 2) : mn_major(&b, B)))
