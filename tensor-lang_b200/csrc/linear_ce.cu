@@ -131,22 +131,27 @@ __device__ __forceinline__ void tma_add_3d(const CUtensorMap* map, uint32_t src,
       : "memory");
 }
 
-// Shared-memory matrix descriptors (128-byte swizzle), 16-deep k-step k.
+// Shared-memory matrix descriptors (128-byte swizzle) of a tile's first 16-deep
+// k-step; kStep is what a further one adds.
 //   K-major tile: rows of 128 bytes, 8-row groups 1 KB apart; a k-step is 32
 //   bytes into the row.
 //   MN-major tile: chunks of 64 (M or N) x 64 k, 8 KB apart, a k a row of 128
 //   bytes; a k-step is 16 rows = 2 KB.
+// The address field counts 16 bytes and stays below its 14 bits (232 KB), so
+// stages and k-steps are additions: the issuing thread's loop is short, which
+// matters where a step's MMAs are (128 columns: 256 cycles).
 template <int MN>
-__device__ __forceinline__ uint64_t tile_desc(uint32_t tile, int k) {
-  const uint32_t a = tile + (MN ? 2048u : 32u) * (uint32_t)k;
+__device__ __forceinline__ uint64_t tile_desc(uint32_t tile) {
   uint64_t d = 0;
-  d |= (uint64_t)((a >> 4) & 0x3FFF);
+  d |= (uint64_t)((tile >> 4) & 0x3FFF);
   d |= (uint64_t)(((MN ? 8192 : 16) >> 4) & 0x3FFF) << 16;
   d |= (uint64_t)((1024 >> 4) & 0x3FFF) << 32;
   d |= (uint64_t)1 << 46;  // descriptor version for tcgen05
   d |= (uint64_t)2 << 61;  // 128-byte swizzle
   return d;
 }
+template <int MN>
+constexpr uint64_t kStep = (MN ? 2048 : 32) >> 4;
 // kind::f16, bf16 operands, float32 accumulator, 256 x nt over the CTA pair
 template <int A_MN, int B_MN>
 __device__ __forceinline__ uint32_t idesc(int nt) {
@@ -346,6 +351,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     if (warp == 1 && leader && lane == 0) {
       // -------------------------------------------------------- MMA (leader)
       const uint32_t id = idesc<TA, 1 - TB>(p.nt);
+      const uint64_t a0 = tile_desc<TA>(smem_u32(smem));
+      const uint64_t b0 = tile_desc<1 - TB>(smem_u32(smem) + (uint32_t)p.b_at);
+      const uint64_t stage16 = (uint64_t)(p.stage_bytes >> 4);
+      const uint32_t full_bar = smem_u32(full), empty_bar = smem_u32(empty);
+      uint64_t a_desc = a0, b_desc = b0;
       bool ok = true;
       int s = 0;
       uint32_t turn = 0, cg = 0;
@@ -360,20 +370,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           }
           fence_after();
           for (int i = 0; i < n; ++i) {
-            if (!mbar_wait(smem_u32(&full[s]), turn & 1)) {
+            if (!mbar_wait(full_bar + 8u * (uint32_t)s, turn & 1)) {
               ok = false;
               break;
             }
             fence_after();
-            const uint32_t sA = smem_u32(smem + s * p.stage_bytes), sB = sA + (uint32_t)p.b_at;
 #pragma unroll
             for (int k = 0; k < BK / 16; ++k)
-              mma2_bf16(acc, tile_desc<TA>(sA, k), tile_desc<1 - TB>(sB, k), id,
+              mma2_bf16(acc, a_desc + k * kStep<TA>, b_desc + k * kStep<1 - TB>, id,
                         (i == 0 && k == 0) ? 0u : 1u);
-            mma2_commit_both(smem_u32(&empty[s]));
+            mma2_commit_both(empty_bar + 8u * (uint32_t)s);
+            a_desc += stage16;
+            b_desc += stage16;
             if (++s == p.stages) {
               s = 0;
               ++turn;
+              a_desc = a0;
+              b_desc = b0;
             }
           }
           mma2_commit_both(smem_u32(&acc_full[b]));
