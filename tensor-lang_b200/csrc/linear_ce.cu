@@ -21,7 +21,8 @@
 // The product kernel computes 256 x 256 tiles by clusters of two CTAs
 // (tcgen05.mma.cta_group::2, operands by TMA in the 128-byte swizzle, two
 // accumulators of 256 columns in tensor memory), as gemm_tc.cu does for
-// float32 operands: warp 0 loads, warp 1 of the leading CTA issues the MMAs,
+// float32 operands, and 128 x 128 tiles by single CTAs where x has at most 128
+// rows: warp 0 loads, warp 1 of the leading CTA issues the MMAs,
 // eight warps drain finished chunks of K into registers and run the epilogue
 // while the next chunk or tile is multiplied.  Operands are read in the major
 // order they have in memory (K-major or MN-major boxes); nothing is transposed.
@@ -112,16 +113,55 @@ struct TileParams {
   int out_bf16, accumulate, tma_out;
 };
 
-// shared::cluster TMA load of a box at (c0, c1, plane), completing on the
-// leader's barrier
-__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar,
-                                                 int c0, int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-      "l"((uint64_t)map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
+// CG 2: a cluster of two CTAs works on a 256-row tile; CG 1: one CTA on a 128-row
+// tile (products of at most 128 rows).  TMA load of a box at (c0, c1, plane),
+// completing on `bar` (CG 2: the leader's).
+template <int CG>
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1,
+                                         int c2) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"((uint64_t)map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"((uint64_t)map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
 }
+template <int CG>
+__device__ __forceinline__ void mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                    uint32_t accumulate) {
+  if constexpr (CG == 2)
+    mma2_bf16(d_tmem, a_desc, b_desc, idesc, accumulate);
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// arrive on `bar` (CG 2: in both CTAs) once the MMAs issued so far are done
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if constexpr (CG == 2)
+    mma2_commit_both(bar);
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+                 : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void sync_ctas() {
+  if constexpr (CG == 2)
+    cluster_sync_all();
+  else
+    __syncthreads();
+}
+
 // float32 sums in memory += a staged tile (one addition per element)
 __device__ __forceinline__ void tma_add_3d(const CUtensorMap* map, uint32_t src, int c0, int c1,
                                            int c2) {
@@ -152,11 +192,11 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t tile) {
 }
 template <int MN>
 constexpr uint64_t kStep = (MN ? 2048 : 32) >> 4;
-// kind::f16, bf16 operands, float32 accumulator, 256 x nt over the CTA pair
-template <int A_MN, int B_MN>
+// kind::f16, bf16 operands, float32 accumulator, 128 CG x nt
+template <int CG, int A_MN, int B_MN>
 __device__ __forceinline__ uint32_t idesc(int nt) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16) |
-         ((uint32_t)(nt >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+         ((uint32_t)(nt >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
 }
 
 struct Tile {
@@ -164,15 +204,16 @@ struct Tile {
 };
 // Tile g: bands of eight M tiles, within a band M fastest (a wave of clusters
 // shares a few row blocks of A and of B in L2); splits of K outermost.
+template <int TM>
 __device__ __forceinline__ Tile tile_of(const TileParams& p, int g) {
   constexpr int kBand = 8;
-  const int mt = (p.M + 255) / 256, nt = (p.N + p.nt - 1) / p.nt, nk = (p.K + BK - 1) / BK;
+  const int mt = (p.M + TM - 1) / TM, nt = (p.N + p.nt - 1) / p.nt, nk = (p.K + BK - 1) / BK;
   Tile t;
   t.split = g / (mt * nt);
   const int r = g - t.split * mt * nt;
   const int band = r / (kBand * nt), in = r - band * kBand * nt;
   const int rows = min(kBand, mt - band * kBand);
-  t.m0 = (band * kBand + in % rows) * 256;
+  t.m0 = (band * kBand + in % rows) * TM;
   t.n0 = in / rows * p.nt;
   t.kb0 = (int)((int64_t)t.split * nk / p.splits);
   t.nk = (int)((int64_t)(t.split + 1) * nk / p.splits) - t.kb0;
@@ -246,8 +287,8 @@ __device__ __forceinline__ float column_sum_of(const float* v, int lane) {
 __device__ __forceinline__ float column_sum(const float* v, int lane) { return column_sum_of<32>(v, lane); }
 
 // A: x, g or x^T ...; TA 0: stored [M][K], 1: [K][M].  TB 0: B stored [K][N], 1: [N][K].
-template <int TA, int TB, int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+template <int CG, int TA, int TB, int EPI>
+__global__ void __launch_bounds__(THREADS, 1)
     vocab_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                       const __grid_constant__ CUtensorMap tmC, const TileParams p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -259,11 +300,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   uint64_t* acc_free = acc_full + 2;                             // [2] both epilogues -> MMA
   uint32_t* tmem_slot = (uint32_t*)(acc_free + 2);
 
-  const uint32_t rank = cluster_ctarank();
+  constexpr int TM = 128 * CG;  // rows of a tile
+  const uint32_t rank = CG == 2 ? cluster_ctarank() : 0u;
   const bool leader = rank == 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tiles = p.splits * ((p.M + 255) / 256) * ((p.N + p.nt - 1) / p.nt);
-  const int step = (int)(gridDim.x >> 1), first = (int)(blockIdx.x >> 1);
+  const int tiles = p.splits * ((p.M + TM - 1) / TM) * ((p.N + p.nt - 1) / p.nt);
+  const int step = (int)gridDim.x / CG, first = (int)blockIdx.x / CG;
 
   if (threadIdx.x == 32) {
     asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tmA) : "memory");
@@ -276,20 +318,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&acc_full[b]), 1);
-      mbar_init(smem_u32(&acc_free[b]), 2 * EPI_WARPS);
+      mbar_init(smem_u32(&acc_free[b]), CG * EPI_WARPS);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     smem_u32(tmem_slot)),
-                 "r"(TMEM_COLS)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    if constexpr (CG == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       smem_u32(tmem_slot)),
+                   "r"(TMEM_COLS)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       smem_u32(tmem_slot)),
+                   "r"(TMEM_COLS)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   fence_before();
-  cluster_sync_all();
+  sync_ctas<CG>();
   fence_after();
   const uint32_t tmem = *tmem_slot;
   wait_for_previous_kernel();
@@ -301,18 +351,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
     if (warp == 0 && lane == 0) {
       // ---------------------------------------------------------- producer
-      const uint32_t full0 = mapa_shared(smem_u32(&full[0]), 0);
+      const uint32_t full0 = CG == 2 ? mapa_shared(smem_u32(&full[0]), 0) : smem_u32(&full[0]);
       bool ok = true;
       int s = 0;
       uint32_t turn = 0;
       for (int g = first; g < tiles && ok; g += step) {
-        const Tile t = tile_of(p, g);
-        const int m0 = t.m0 + 128 * (int)rank, n0 = t.n0 + p.nt / 2 * (int)rank;
+        const Tile t = tile_of<TM>(p, g);
+        const int m0 = t.m0 + 128 * (int)rank, n0 = t.n0 + p.nt / CG * (int)rank;
         // rows of A that do not exist are not loaded: their results are not kept,
         // whatever the stage holds there
         const bool have_a = m0 < p.M;
         const uint32_t a_bytes = TA == 0 ? (uint32_t)p.a_rows * 128u : (uint32_t)TILE_BYTES;
-        const uint32_t bytes = (t.m0 + 128 < p.M ? 2u : 1u) * a_bytes + (uint32_t)p.nt * 128u;
+        const uint32_t bytes = (CG == 2 && t.m0 + 128 < p.M ? 2u : 1u) * a_bytes + (uint32_t)p.nt * 128u;
         for (int c = 0; c < t.nk && ok; c += p.kc) {
           const int cend = min(c + p.kc, t.nk);
           for (int q = 0; q < p.terms && ok; ++q) {
@@ -328,16 +378,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
               const int k0 = (t.kb0 + kb) * BK;
               if (!have_a) {
               } else if constexpr (TA == 0) {
-                tma_load_3d_pair(sA, &tmA, fb, k0, m0, pa);
+                load_box<CG>(sA, &tmA, fb, k0, m0, pa);
               } else {
-                tma_load_3d_pair(sA, &tmA, fb, m0, k0, pa);
-                tma_load_3d_pair(sA + 8192, &tmA, fb, m0 + 64, k0, pa);
+                load_box<CG>(sA, &tmA, fb, m0, k0, pa);
+                load_box<CG>(sA + 8192, &tmA, fb, m0 + 64, k0, pa);
               }
               if constexpr (TB == 1) {
-                tma_load_3d_pair(sB, &tmB, fb, k0, n0, pb);
+                load_box<CG>(sB, &tmB, fb, k0, n0, pb);
               } else {
-                tma_load_3d_pair(sB, &tmB, fb, n0, k0, pb);
-                if (p.nt > 128) tma_load_3d_pair(sB + 8192, &tmB, fb, n0 + 64, k0, pb);
+                load_box<CG>(sB, &tmB, fb, n0, k0, pb);
+                if (p.nt / CG > 64) load_box<CG>(sB + 8192, &tmB, fb, n0 + 64, k0, pb);
               }
               if (++s == p.stages) {
                 s = 0;
@@ -350,7 +400,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
     if (warp == 1 && leader && lane == 0) {
       // -------------------------------------------------------- MMA (leader)
-      const uint32_t id = idesc<TA, 1 - TB>(p.nt);
+      const uint32_t id = idesc<CG, TA, 1 - TB>(p.nt);
       const uint64_t a0 = tile_desc<TA>(smem_u32(smem));
       const uint64_t b0 = tile_desc<1 - TB>(smem_u32(smem) + (uint32_t)p.b_at);
       const uint64_t stage16 = (uint64_t)(p.stage_bytes >> 4);
@@ -360,7 +410,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       int s = 0;
       uint32_t turn = 0, cg = 0;
       for (int g = first; g < tiles && ok; g += step) {
-        const Tile t = tile_of(p, g);
+        const Tile t = tile_of<TM>(p, g);
         for (int c = 0; c < t.nk && ok; c += p.kc, ++cg) {
           const int n = (min(c + p.kc, t.nk) - c) * p.terms;
           const uint32_t b = cg & 1, acc = tmem + b * 256;
@@ -377,9 +427,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             fence_after();
 #pragma unroll
             for (int k = 0; k < BK / 16; ++k)
-              mma2_bf16(acc, a_desc + k * kStep<TA>, b_desc + k * kStep<1 - TB>, id,
-                        (i == 0 && k == 0) ? 0u : 1u);
-            mma2_commit_both(empty_bar + 8u * (uint32_t)s);
+              mma<CG>(acc, a_desc + k * kStep<TA>, b_desc + k * kStep<1 - TB>, id,
+                      (i == 0 && k == 0) ? 0u : 1u);
+            commit<CG>(empty_bar + 8u * (uint32_t)s);
             a_desc += stage16;
             b_desc += stage16;
             if (++s == p.stages) {
@@ -389,7 +439,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
               b_desc = b0;
             }
           }
-          mma2_commit_both(smem_u32(&acc_full[b]));
+          commit<CG>(smem_u32(&acc_full[b]));
         }
       }
     }
@@ -406,7 +456,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegs));
     // ----------------------------------------------------------- epilogue
     const int e = warp - 4, quarter = warp & 3, group = e >> 2;
-    const uint32_t free0 = mapa_shared(smem_u32(&acc_free[0]), 0);
+    const uint32_t free0 = CG == 2 ? mapa_shared(smem_u32(&acc_free[0]), 0) : smem_u32(&acc_free[0]);
     const uint32_t tbase = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(group * CW);
     float* stage = reinterpret_cast<float*>(staging + e * STG_TILE);
     const uint32_t stg = smem_u32(stage);
@@ -414,7 +464,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     bool ok = true;
     uint32_t cg = 0;
     for (int g = first; g < tiles && ok; g += step) {
-      const Tile t = tile_of(p, g);
+      const Tile t = tile_of<TM>(p, g);
 #pragma unroll
       for (int j = 0; j < CW; ++j) v[j] = 0.f;
       for (int c = 0; c < t.nk; c += p.kc, ++cg) {
@@ -434,7 +484,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         }
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(free0 + 8u * b);
+        if (lane == 0) {
+          if constexpr (CG == 2)
+            mbar_arrive_cluster(free0 + 8u * b);
+          else
+            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(free0 + 8u * b) : "memory");
+        }
       }
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -596,11 +651,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     __syncwarp();
   }
   fence_before();
-  cluster_sync_all();  // neither CTA frees tensor memory or exits while the pair works
+  sync_ctas<CG>();  // neither CTA frees tensor memory or exits while the pair works
   if (warp == 1) {
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS)
-                 : "memory");
+    if constexpr (CG == 2)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS)
+                   : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS)
+                   : "memory");
   }
 }
 
@@ -877,29 +936,34 @@ bool mn_major(CUtensorMap* m, const Planes& x) {
   return make_map3(m, x.p, false, x.planes, x.rows, x.cols, x.ld, 64, 64);
 }
 
-// Columns of a tile: 256, except
-//  - where half-size tiles still fit one wave of clusters: the narrowest that do
-//    (steps are what the epilogue's slabs and B's boxes allow);
-//  - between one and four waves of a K-major B: 224 or 192 where that ends
-//    sooner (a wave costs its tiles' columns and a fixed part worth about 32).
+// Whether a product's tiles are one CTA's: A's rows fit one (K-major A).
+bool one_cta(int64_t M) { return M <= 128; }
+
+// Columns of a tile: 256 (one CTA: 128), except
+//  - where half-size tiles still fit one wave: the narrowest that do (steps are
+//    what the epilogue's slabs and B's boxes allow);
+//  - between one and four waves of a K-major B: fewer where that ends sooner (a
+//    wave costs its tiles' columns and a fixed part worth about 32).
 //    Scoring 1 token x 32768 classes x 4096: 224 columns, 57 us; 256, 71 us.
 //    An MN-major B's boxes are 64 columns of 128 bytes: with 128-column tiles
-//    96 tokens x 65536 classes x 2048 took 90 us, with 256 60 us.
+//    of CTA pairs 96 tokens x 65536 classes x 2048 took 90 us, with 256 60 us.
 template <int EPI>
-int tile_columns(int64_t M, int64_t N, int splits, bool b_mn_major) {
-  const int64_t slots = std::max(1, sm_count() / 2), mt = (M + 255) / 256 * splits;
-  const int64_t tiles = mt * ((N + 255) / 256);
-  if (tiles >= 4 * slots) return 256;
-  const int step = b_mn_major ? 128 : EPI == kStats || EPI == kSum ? 32 : 64;
+int tile_columns(int64_t M, int64_t N, int splits, bool b_mn_major, bool one) {
+  const int wide = one ? 128 : 256;
+  const int64_t slots = std::max(1, one ? sm_count() : sm_count() / 2);
+  const int64_t mt = (one ? (M + 127) / 128 : (M + 255) / 256) * splits;
+  const int64_t tiles = mt * ((N + wide - 1) / wide);
+  if (tiles >= 4 * slots) return wide;
+  const int step = b_mn_major ? wide / 2 : EPI == kStats ? (one ? 16 : 32) : EPI == kSum ? 32 : 64;
   if (2 * tiles <= slots) {
-    for (int nt = std::max(step, 64); nt < 256; nt += step)
+    for (int nt = std::max(step, 64); nt < wide; nt += step)
       if (mt * ((N + nt - 1) / nt) <= slots) return nt;
-    return 256;
+    return wide;
   }
-  if (b_mn_major) return 256;
-  int best = 256;
+  if (b_mn_major) return wide;
+  int best = wide;
   int64_t cost = INT64_MAX;
-  for (int nt = 256; nt >= 192; nt -= step) {
+  for (int nt = wide; nt >= wide / 4 * 3; nt -= step) {
     const int64_t waves = (mt * ((N + nt - 1) / nt) + slots - 1) / slots, c = waves * (nt + 32);
     if (c < cost) {
       cost = c;
@@ -909,31 +973,41 @@ int tile_columns(int64_t M, int64_t N, int splits, bool b_mn_major) {
   return best;
 }
 
-template <int TA, int TB, int EPI>
-int launch_tiles(const Planes& A, const Planes& B, const CUtensorMap& c, TileParams p, cudaStream_t st) {
-  constexpr auto kern = vocab_tile_kernel<TA, TB, EPI>;
+template <int CG, int TA, int TB, int EPI>
+int launch_tiles_of(const Planes& A, const Planes& B, const CUtensorMap& c, TileParams p, cudaStream_t st) {
+  constexpr auto kern = vocab_tile_kernel<CG, TA, TB, EPI>;
   TL_TRY((allow_smem<kern, SMEM_BYTES>()));
-  p.nt = tile_columns<EPI>(p.M, p.N, p.splits, TB == 0);
+  constexpr int TM = 128 * CG;
+  p.nt = tile_columns<EPI>(p.M, p.N, p.splits, TB == 0, CG == 1);
   p.a_rows = TA == 0 ? (int)std::min<int64_t>(128, up_to(p.M, 8)) : 128;
   // the MMA reads 128 rows of A from a stage's start: past the loaded ones what
   // follows in shared memory, whose products are not kept
   p.b_at = p.a_rows * 128;
-  p.stage_bytes = p.b_at + p.nt / 2 * 128;
+  p.stage_bytes = p.b_at + p.nt / CG * 128;
   p.stages = std::min(MAX_STAGES, RING_BYTES / p.stage_bytes);
   CUtensorMap a, b;
   if (!(TA == 0 ? k_major(&a, A, p.a_rows) : mn_major(&a, A)) ||
-      !(TB == 1 ? k_major(&b, B, p.nt / 2) : mn_major(&b, B)))
+      !(TB == 1 ? k_major(&b, B, p.nt / CG) : mn_major(&b, B)))
     return TL_ERR_UNSUPPORTED;
-  const int64_t tiles = (int64_t)p.splits * ((p.M + 255) / 256) * ((p.N + p.nt - 1) / p.nt);
+  const int64_t tiles = (int64_t)p.splits * ((p.M + TM - 1) / TM) * ((p.N + p.nt - 1) / p.nt);
   if (tiles > INT32_MAX / 2) return TL_ERR_UNSUPPORTED;
-  const int64_t clusters = std::min<int64_t>(tiles, std::max(1, sm_count() / 2));
-  return launch(kern, dim3((unsigned)(2 * clusters)), THREADS, SMEM_BYTES, st, a, b, c, p);
+  const int64_t slots = std::max(1, sm_count() / CG);
+  return launch_in_clusters(CG, kern, dim3((unsigned)(CG * std::min(tiles, slots))), THREADS, SMEM_BYTES, st, a,
+                            b, c, p);
+}
+template <int TA, int TB, int EPI>
+int launch_tiles(const Planes& A, const Planes& B, const CUtensorMap& c, const TileParams& p,
+                 cudaStream_t st) {
+  if constexpr (TA == 0) {
+    if (one_cta(p.M)) return launch_tiles_of<1, TA, TB, EPI>(A, B, c, p, st);
+  }
+  return launch_tiles_of<2, TA, TB, EPI>(A, B, c, p, st);
 }
 
 // The partials a product of kStats leaves per row: one for each epilogue warp's
 // columns, none for columns that do not exist.
 int stat_slots(int64_t M, int64_t N, bool b_mn_major) {
-  const int nt = tile_columns<kStats>(M, N, 1, b_mn_major);
+  const int nt = tile_columns<kStats>(M, N, 1, b_mn_major, one_cta(M));
   const int64_t before = (N - 1) / nt;
   return (int)(before * (nt > CW ? 2 : 1) + (N - before * nt > CW ? 2 : 1));
 }
@@ -969,8 +1043,9 @@ struct Plan {
 
 // splits of K that let few tiles of dx fill the GPU: whole waves of clusters
 int dx_splits(int64_t rows, int64_t width, int64_t piece) {
-  const int64_t tiles = ((rows + 255) / 256) * ((width + 255) / 256), nk = piece / BK;
-  const int64_t slots = std::max(1, sm_count() / 2);
+  const bool one = one_cta(rows);
+  const int64_t tiles = one ? (width + 127) / 128 : ((rows + 255) / 256) * ((width + 255) / 256);
+  const int64_t slots = std::max(1, one ? sm_count() : sm_count() / 2), nk = piece / BK;
   int best = 1;
   double eff = 0;
   for (int s = 1; s <= 16 && (s == 1 || nk / s >= 8); ++s) {
