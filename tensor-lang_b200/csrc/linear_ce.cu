@@ -812,23 +812,23 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* p, int64_t left, floa
 // The terms of a matrix as bf16 planes [planes][rows][ld], columns past `cols`
 // zero: three that sum to a float32 matrix exactly, or a copy of a bf16 one
 // whose rows TMA cannot address.  ld is a multiple of 8.
-template <typename T>
+template <typename T, typename Index>
 __global__ void __launch_bounds__(256) planes_kernel(const T* __restrict__ X, int64_t ldx, int64_t rows,
                                                      int64_t cols, int planes,
                                                      __nv_bfloat16* __restrict__ out, int64_t ld) {
   wait_for_previous_kernel();
   const int64_t plane = rows * ld;
-  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
-    const T* src = X + r * ldx;
-    __nv_bfloat16* dst = out + r * ld;
-    for (int64_t c = 8 * ((int64_t)blockIdx.x * 256 + threadIdx.x); c < ld; c += 8 * 256LL * gridDim.x) {
-      float v[8];
-      load8(src + c, cols - c, v);
-      for (int p = 0; p < planes; ++p)
-        *reinterpret_cast<uint4*>(dst + p * plane + c) =
-            make_uint4(take_bf16(v[0], v[1]), take_bf16(v[2], v[3]), take_bf16(v[4], v[5]),
-                       take_bf16(v[6], v[7]));
-    }
+  const Index vecs = (Index)(ld / 8), n = (Index)rows * vecs, step = (Index)gridDim.x * 256;
+  for (Index i = (Index)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
+    const Index r = i / vecs;
+    const int64_t c = 8 * (int64_t)(i - r * vecs);
+    float v[8];
+    load8(X + (int64_t)r * ldx + c, cols - c, v);
+    __nv_bfloat16* dst = out + (int64_t)r * ld + c;
+    for (int p = 0; p < planes; ++p)
+      *reinterpret_cast<uint4*>(dst + p * plane) =
+          make_uint4(take_bf16(v[0], v[1]), take_bf16(v[2], v[3]), take_bf16(v[4], v[5]),
+                     take_bf16(v[6], v[7]));
   }
 }
 
@@ -1079,9 +1079,9 @@ Plan make_plan(int dtype, int trans_w, int64_t rows, int64_t classes, int64_t wi
     at = up_to(at + bytes, 1024);
     return o;
   };
-  q.xplanes = take(P * rows * up_to(width, 8) * 2);
+  q.xplanes = take(P * rows * up_to(width, 64) * 2);
   const int64_t wp = backward ? std::max(q.fpiece, q.bpiece) : q.fpiece;
-  q.wplanes = take(P * (trans_w ? wp * up_to(width, 8) : width * up_to(wp, 8)) * 2);
+  q.wplanes = take(P * (trans_w ? wp * up_to(width, 64) : width * up_to(wp, 64)) * 2);
   const int64_t common = at;
   q.zt = take(rows * 4);
   q.run = take(rows * 8);
@@ -1104,9 +1104,12 @@ Plan make_plan(int dtype, int trans_w, int64_t rows, int64_t classes, int64_t wi
 template <typename T>
 int write_planes(const T* X, int64_t ldx, int64_t rows, int64_t cols, int planes, __nv_bfloat16* out,
                  int64_t ld, cudaStream_t st) {
-  const int64_t across = (ld / 8 + 255) / 256;
-  const dim3 grid((unsigned)std::min<int64_t>(across, 16), (unsigned)std::min<int64_t>(rows, 65535));
-  return launch(planes_kernel<T>, grid, 256, 0, st, X, ldx, rows, cols, planes, out, ld);
+  const int64_t vecs = rows * (ld / 8);
+  const dim3 grid((unsigned)std::min<int64_t>((vecs + 255) / 256, 32LL * sm_count()));
+  // the index steps past the end by at most the grid's threads
+  return vecs < (1LL << 31)
+             ? launch(planes_kernel<T, uint32_t>, grid, 256, 0, st, X, ldx, rows, cols, planes, out, ld)
+             : launch(planes_kernel<T, uint64_t>, grid, 256, 0, st, X, ldx, rows, cols, planes, out, ld);
 }
 
 // Whether TMA can address a matrix of the call's type as it is.
@@ -1115,14 +1118,16 @@ bool direct(const Call& c, const void* X, int64_t ldx) {
 }
 
 // rows x cols of X as planes: itself where TMA can address it, else a copy
+// (or `copy`).  A copy's rows start at multiples of 128 bytes: a box's rows of 128
+// bytes then are one cache line each, not two.
 int as_planes(const Call& c, const void* X, int64_t ldx, int64_t rows, int64_t cols, int64_t scratch_at,
-              Planes* out) {
-  if (direct(c, X, ldx)) {
+              bool copy, Planes* out) {
+  if (!copy && direct(c, X, ldx)) {
     *out = {static_cast<const __nv_bfloat16*>(X), 1, rows, cols, ldx};
     return TL_OK;
   }
   __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(c.scratch + scratch_at);
-  *out = {dst, c.planes(), rows, cols, up_to(cols, 8)};
+  *out = {dst, c.planes(), rows, cols, up_to(cols, 64)};
   if (c.f32())
     return write_planes(static_cast<const float*>(X), ldx, rows, cols, 3, dst, out->ld, c.st);
   return write_planes(static_cast<const __nv_bfloat16*>(X), ldx, rows, cols, 1, dst, out->ld, c.st);
@@ -1132,8 +1137,15 @@ int as_planes(const Call& c, const void* X, int64_t ldx, int64_t rows, int64_t c
 int w_planes(const Call& c, const Plan& q, int64_t c0, int64_t n, Planes* out) {
   const int64_t es = (int64_t)elem_bytes(c.dtype);
   const char* w = static_cast<const char*>(c.w) + (c.trans_w ? c0 * c.ldw : c0) * es;
-  return c.trans_w ? as_planes(c, w, c.ldw, n, c.width, q.wplanes, out)
-                   : as_planes(c, w, c.ldw, c.width, n, q.wplanes, out);
+  return c.trans_w ? as_planes(c, w, c.ldw, n, c.width, q.wplanes, false, out)
+                   : as_planes(c, w, c.ldw, c.width, n, q.wplanes, false, out);
+}
+// x, read by every tile: where its rows straddle cache lines, and rows and classes
+// are many enough for a copy to pay (1537 x 1000 against 50021 classes: products
+// 142 -> 136 and 170 -> 159 us; 5000 x 2000 against 600 classes 118 -> 136 us in all).
+int x_planes(const Call& c, const Plan& q, Planes* out) {
+  const bool straddles = c.ldx % 64 || !aligned_to(c.x, 128);
+  return as_planes(c, c.x, c.ldx, c.rows, c.width, q.xplanes, straddles && c.rows >= 512 && c.classes >= 8192, out);
 }
 
 // The logits' product over classes c0 .. c0 + n, with epilogue EPI.
@@ -1157,7 +1169,7 @@ int logits(const Call& c, const Planes& x, const Planes& w, const CUtensorMap& o
 
 int forward(const Call& c, const Plan& q, float* loss, float* row_loss, float* lse) {
   Planes x, w;
-  TL_TRY(as_planes(c, c.x, c.ldx, c.rows, c.width, q.xplanes, &x));
+  TL_TRY(x_planes(c, q, &x));
   TileParams p{};
   p.part = reinterpret_cast<float2*>(c.scratch + q.part);
   p.part_ld = q.part_ld;
@@ -1186,7 +1198,7 @@ int backward(const Call& c, const Plan& q, const float* lse, const float* upstre
              void* dW, int64_t lddw, float* dbias, int accumulate) {
   float* scale = &reinterpret_cast<Head*>(c.scratch)->scale;
   Planes x, w;
-  TL_TRY(as_planes(c, c.x, c.ldx, c.rows, c.width, q.xplanes, &x));
+  TL_TRY(x_planes(c, q, &x));
   const int64_t es = (int64_t)elem_bytes(c.dtype);
   float* sums = reinterpret_cast<float*>(c.scratch + q.sums);
   float* colsum = reinterpret_cast<float*>(c.scratch + q.colsum);
