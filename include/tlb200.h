@@ -483,7 +483,8 @@ int  tl_distill_topk(int dtype, int64_t rows, int64_t classes, int64_t top, cons
  * target [rows] the index type; loss [1], row_loss and lse [rows] are float and
  * may be null.  A class whose bias is -inf takes no part; a row with no class
  * left has lse = -inf, gradient -onehot and, where it counts, loss +inf, as has
- * a row whose target is such a class. */
+ * a row whose target is such a class.  W is finite, masked classes included; x
+ * may hold anything in rows without a target. */
 size_t tl_linear_ce_scratch_bytes(int dtype, int trans_w, int64_t rows, int64_t classes,
                                   int64_t width, int backward);
 int  tl_linear_ce(int dtype, int trans_w, int64_t rows, int64_t classes, int64_t width,
@@ -495,8 +496,10 @@ int  tl_linear_ce(int dtype, int trans_w, int64_t rows, int64_t classes, int64_t
  *   g = (softmax(z) - onehot(target)) * upstream / divisor
  *   dx = g W^T    dW = x^T g (W's shape and order)    dbias = sum over rows of g
  * each may be null; none may overlap x or W.  accumulate: a sum of TL_ACC_DX,
- * TL_ACC_DW and TL_ACC_DBIAS.  Scratch of tl_linear_ce_scratch_bytes(...,
- * backward = 1) serves both calls. */
+ * TL_ACC_DW and TL_ACC_DBIAS.  softmax(z) is exp(z - lse), so a probability
+ * carries lse's rounding (2^-24 of |lse|) as well as the logit's: masks of the
+ * type's lowest value need one class of ordinary size beside them.  Scratch of
+ * tl_linear_ce_scratch_bytes(..., backward = 1) serves both calls. */
 #define TL_ACC_DW 2
 #define TL_ACC_DBIAS 4
 int  tl_linear_ce_backward(int dtype, int trans_w, int64_t rows, int64_t classes, int64_t width,

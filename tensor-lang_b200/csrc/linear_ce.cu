@@ -811,11 +811,13 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* p, int64_t left, floa
 
 // The terms of a matrix as bf16 planes [planes][rows][ld], columns past `cols`
 // zero: three that sum to a float32 matrix exactly, or a copy of a bf16 one
-// whose rows TMA cannot address.  ld is a multiple of 8.
+// whose rows TMA cannot address.  ld is a multiple of 8.  Rows without a target
+// (where keep.p is not null) come out as zeros.
 template <typename T, typename Index>
 __global__ void __launch_bounds__(256) planes_kernel(const T* __restrict__ X, int64_t ldx, int64_t rows,
                                                      int64_t cols, int planes,
-                                                     __nv_bfloat16* __restrict__ out, int64_t ld) {
+                                                     __nv_bfloat16* __restrict__ out, int64_t ld,
+                                                     const Targets keep) {
   wait_for_previous_kernel();
   const int64_t plane = rows * ld;
   const Index vecs = (Index)(ld / 8), n = (Index)rows * vecs, step = (Index)gridDim.x * 256;
@@ -823,7 +825,8 @@ __global__ void __launch_bounds__(256) planes_kernel(const T* __restrict__ X, in
     const Index r = i / vecs;
     const int64_t c = 8 * (int64_t)(i - r * vecs);
     float v[8];
-    load8(X + (int64_t)r * ldx + c, cols - c, v);
+    const bool kept = !keep.p || keep.at((int64_t)r) >= 0;
+    load8(X + (int64_t)r * ldx + c, kept ? cols - c : 0, v);
     __nv_bfloat16* dst = out + (int64_t)r * ld + c;
     for (int p = 0; p < planes; ++p)
       *reinterpret_cast<uint4*>(dst + p * plane) =
@@ -1103,13 +1106,13 @@ Plan make_plan(int dtype, int trans_w, int64_t rows, int64_t classes, int64_t wi
 
 template <typename T>
 int write_planes(const T* X, int64_t ldx, int64_t rows, int64_t cols, int planes, __nv_bfloat16* out,
-                 int64_t ld, cudaStream_t st) {
+                 int64_t ld, const Targets& keep, cudaStream_t st) {
   const int64_t vecs = rows * (ld / 8);
   const dim3 grid((unsigned)std::min<int64_t>((vecs + 255) / 256, 32LL * sm_count()));
   // the index steps past the end by at most the grid's threads
   return vecs < (1LL << 31)
-             ? launch(planes_kernel<T, uint32_t>, grid, 256, 0, st, X, ldx, rows, cols, planes, out, ld)
-             : launch(planes_kernel<T, uint64_t>, grid, 256, 0, st, X, ldx, rows, cols, planes, out, ld);
+             ? launch(planes_kernel<T, uint32_t>, grid, 256, 0, st, X, ldx, rows, cols, planes, out, ld, keep)
+             : launch(planes_kernel<T, uint64_t>, grid, 256, 0, st, X, ldx, rows, cols, planes, out, ld, keep);
 }
 
 // Whether TMA can address a matrix of the call's type as it is.
@@ -1117,11 +1120,12 @@ bool direct(const Call& c, const void* X, int64_t ldx) {
   return !c.f32() && ldx % 8 == 0 && aligned_to(X, 16);
 }
 
-// rows x cols of X as planes: itself where TMA can address it, else a copy
-// (or `copy`).  A copy's rows start at multiples of 128 bytes: a box's rows of 128
-// bytes then are one cache line each, not two.
+// rows x cols of X as planes: itself where TMA can address it, else (or with
+// `copy`) a copy, without the rows that `keep` names no class for.  A copy's rows
+// start at multiples of 128 bytes: a box's rows of 128 bytes then are one cache
+// line each, not two.
 int as_planes(const Call& c, const void* X, int64_t ldx, int64_t rows, int64_t cols, int64_t scratch_at,
-              bool copy, Planes* out) {
+              bool copy, const Targets& keep, Planes* out) {
   if (!copy && direct(c, X, ldx)) {
     *out = {static_cast<const __nv_bfloat16*>(X), 1, rows, cols, ldx};
     return TL_OK;
@@ -1129,23 +1133,27 @@ int as_planes(const Call& c, const void* X, int64_t ldx, int64_t rows, int64_t c
   __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(c.scratch + scratch_at);
   *out = {dst, c.planes(), rows, cols, up_to(cols, 64)};
   if (c.f32())
-    return write_planes(static_cast<const float*>(X), ldx, rows, cols, 3, dst, out->ld, c.st);
-  return write_planes(static_cast<const __nv_bfloat16*>(X), ldx, rows, cols, 1, dst, out->ld, c.st);
+    return write_planes(static_cast<const float*>(X), ldx, rows, cols, 3, dst, out->ld, keep, c.st);
+  return write_planes(static_cast<const __nv_bfloat16*>(X), ldx, rows, cols, 1, dst, out->ld, keep, c.st);
 }
 
 // classes c0 .. c0 + n of W
 int w_planes(const Call& c, const Plan& q, int64_t c0, int64_t n, Planes* out) {
   const int64_t es = (int64_t)elem_bytes(c.dtype);
   const char* w = static_cast<const char*>(c.w) + (c.trans_w ? c0 * c.ldw : c0) * es;
-  return c.trans_w ? as_planes(c, w, c.ldw, n, c.width, q.wplanes, false, out)
-                   : as_planes(c, w, c.ldw, c.width, n, q.wplanes, false, out);
+  return c.trans_w ? as_planes(c, w, c.ldw, n, c.width, q.wplanes, false, Targets{}, out)
+                   : as_planes(c, w, c.ldw, c.width, n, q.wplanes, false, Targets{}, out);
 }
-// x, read by every tile: where its rows straddle cache lines, and rows and classes
-// are many enough for a copy to pay (1537 x 1000 against 50021 classes: products
-// 142 -> 136 and 170 -> 159 us; 5000 x 2000 against 600 classes 118 -> 136 us in all).
-int x_planes(const Call& c, const Plan& q, Planes* out) {
+// x, read by every tile: a copy where its rows straddle cache lines, and rows and
+// classes are many enough for that to pay (1537 x 1000 against 50021 classes:
+// products 142 -> 136 and 170 -> 159 us; 5000 x 2000 against 600 classes 118 -> 136
+// us in all).  For dW a copy always, with zeros in the rows without a target: their
+// g is 0, but 0 times an infinity or NaN in a padded row is NaN in all of dW.
+int x_planes(const Call& c, const Plan& q, bool for_dw, Planes* out) {
   const bool straddles = c.ldx % 64 || !aligned_to(c.x, 128);
-  return as_planes(c, c.x, c.ldx, c.rows, c.width, q.xplanes, straddles && c.rows >= 512 && c.classes >= 8192, out);
+  return as_planes(c, c.x, c.ldx, c.rows, c.width, q.xplanes,
+                   for_dw || (straddles && c.rows >= 512 && c.classes >= 8192),
+                   for_dw ? c.targets() : Targets{}, out);
 }
 
 // The logits' product over classes c0 .. c0 + n, with epilogue EPI.
@@ -1169,7 +1177,7 @@ int logits(const Call& c, const Planes& x, const Planes& w, const CUtensorMap& o
 
 int forward(const Call& c, const Plan& q, float* loss, float* row_loss, float* lse) {
   Planes x, w;
-  TL_TRY(x_planes(c, q, &x));
+  TL_TRY(x_planes(c, q, false, &x));
   TileParams p{};
   p.part = reinterpret_cast<float2*>(c.scratch + q.part);
   p.part_ld = q.part_ld;
@@ -1184,10 +1192,10 @@ int forward(const Call& c, const Plan& q, float* loss, float* row_loss, float* l
     TL_TRY(logits<kStats>(c, x, w, none, p, c0, n));
     // few rows: more threads for each
     auto join_rows = [&](auto kern, int64_t r) {
-      return launch(
-          kern, dim3((unsigned)((c.rows + r - 1) / r)), 256, 0, c.st, p.part, q.part_ld, stat_slots(c.rows, n, !c.trans_w), c.targets(), p.zt,
-          reinterpret_cast<float2*>(c.scratch + q.run), c0 == 0, c0 + n == c.classes, c.divisor, row_loss,
-          lse, loss, reinterpret_cast<Head*>(c.scratch));
+      return launch(kern, dim3((unsigned)((c.rows + r - 1) / r)), 256, 0, c.st, p.part, q.part_ld,
+                    stat_slots(c.rows, n, !c.trans_w), c.targets(), p.zt,
+                    reinterpret_cast<float2*>(c.scratch + q.run), c0 == 0, c0 + n == c.classes,
+                    c.divisor, row_loss, lse, loss, reinterpret_cast<Head*>(c.scratch));
     };
     TL_TRY(c.rows >= 4096 ? join_rows(join_kernel<32>, 32) : join_rows(join_kernel<4>, 4));
   }
@@ -1198,7 +1206,7 @@ int backward(const Call& c, const Plan& q, const float* lse, const float* upstre
              void* dW, int64_t lddw, float* dbias, int accumulate) {
   float* scale = &reinterpret_cast<Head*>(c.scratch)->scale;
   Planes x, w;
-  TL_TRY(x_planes(c, q, &x));
+  TL_TRY(x_planes(c, q, dW != nullptr, &x));
   const int64_t es = (int64_t)elem_bytes(c.dtype);
   float* sums = reinterpret_cast<float*>(c.scratch + q.sums);
   float* colsum = reinterpret_cast<float*>(c.scratch + q.colsum);
@@ -1210,7 +1218,7 @@ int backward(const Call& c, const Plan& q, const float* lse, const float* upstre
     CUtensorMap o;
     if (!make_map3(&o, g.p, false, g.planes, g.rows, g.cols, g.ld, 64, 32)) return TL_ERR_UNSUPPORTED;
     TileParams p{};
-      p.lse = lse;
+    p.lse = lse;
     p.planes = c.planes();
     p.divisor = c.divisor;
     p.upstream = upstream;

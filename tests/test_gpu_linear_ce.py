@@ -215,6 +215,24 @@ def test_nan_rows_stay_their_own():
     assert np.isfinite(out["dx"][keep]).all()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,trans", [(20, 0), (300, 1)])
+def test_padded_rows_may_hold_anything(dtype, rows, trans):
+    """Rows without a target hold NaN and infinities: nothing of them reaches
+    the loss or the gradients."""
+    x, w, b, t = inputs(rows, 500, 72, dtype, seed=9)
+    t[[2, rows - 1]], t[5:9] = -100, 500
+    clean = x.copy()
+    pad = (t < 0) | (t >= 500)
+    clean[pad] = 0.0
+    x[pad] = np.nan
+    x[2] = np.inf
+    out = run(x, w, b, t, dtype, trans)
+    out.pop("lse")
+    assert not out["row_loss"][pad].any() and not out["dx"][pad].any()
+    compare(out, clean, w, b, t, dtype)
+
+
 def test_pieces_of_the_vocabulary():
     """A width whose weights' terms make the vocabulary two pieces, in both
     directions (512 MB of terms: 10752 classes of 8192 floats)."""
