@@ -572,7 +572,7 @@ int tl_distill_topk(int dtype, int64_t rows, int64_t classes, int64_t top, const
   TL_TRY(tl::check(dtype, a, top));
   a.k2 = (float)(1.4426950408889634 / (double)temperature);
   a.inv_tau = (float)(1.0 / (double)temperature);
-  if (!loss && !row_loss && !lse && !dz) return TL_ERR_INVALID_ARG;
+  if (rows > 0 && !loss && !row_loss && !lse && !dz) return TL_ERR_INVALID_ARG;
   if (!scratch || !tl::aligned_to(scratch, 16) || scratch_bytes < tl_distill_topk_scratch_bytes(rows))
     return TL_ERR_INVALID_ARG;
   a.counters = static_cast<unsigned*>(scratch);

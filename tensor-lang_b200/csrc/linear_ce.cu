@@ -1310,7 +1310,7 @@ int tl_linear_ce(int dtype, int trans_w, int64_t rows, int64_t classes, int64_t 
   tl::Call c{dtype, trans_w, index_type, rows, classes, width, x, ldx, W, ldw, bias, target, divisor,
              static_cast<char*>(scratch), nullptr};
   TL_TRY(tl::check(c, scratch_bytes, false));
-  if (!loss && !row_loss && !lse) return TL_ERR_INVALID_ARG;
+  if (rows > 0 && !loss && !row_loss && !lse) return TL_ERR_INVALID_ARG;
   c.st = tl::stream_or_default(stream);
   if (rows == 0) {
     if (loss) TL_CUDA_TRY(cudaMemsetAsync(loss, 0, sizeof(float), c.st));
@@ -1328,7 +1328,7 @@ int tl_linear_ce_backward(int dtype, int trans_w, int64_t rows, int64_t classes,
   tl::Call c{dtype, trans_w, index_type, rows, classes, width, x, ldx, W, ldw, bias, target, divisor,
              static_cast<char*>(scratch), nullptr};
   TL_TRY(tl::check(c, scratch_bytes, true));
-  if ((rows > 0 && !lse) || (!dx && !dW && !dbias)) return TL_ERR_INVALID_ARG;
+  if (rows > 0 && (!lse || (!dx && !dW && !dbias))) return TL_ERR_INVALID_ARG;
   if (accumulate & ~(TL_ACC_DX | TL_ACC_DW | TL_ACC_DBIAS)) return TL_ERR_INVALID_ARG;
   if ((dx && lddx < width) || (dW && lddw < (trans_w ? width : classes))) return TL_ERR_INVALID_ARG;
   // the gradients are written piece by piece, while x and W are still read

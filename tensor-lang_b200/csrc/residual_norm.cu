@@ -552,8 +552,9 @@ __global__ void __launch_bounds__(1024) norm_sums_kernel(NormArgs a, int64_t blo
     float t = 0.f;
 #pragma unroll
     for (int k = 0; k < 32; ++k) t += sh[k][lane];
-    if (which == 0 && channel) t *= to_f32(static_cast<const T*>(a.gate)[c]);
-    if (which == 2 && a.w_post) t *= to_f32(static_cast<const T*>(a.w_post)[c]);
+    // (no rows: a gate may not exist, and 0 times an infinity is not 0)
+    if (which == 0 && channel && blocks > 0) t *= to_f32(static_cast<const T*>(a.gate)[c]);
+    if (which == 2 && a.w_post && blocks > 0) t *= to_f32(static_cast<const T*>(a.w_post)[c]);
     const int flag = which == 0 ? TL_ACC_DW_POST : which == 1 ? TL_ACC_DW_PRE : TL_ACC_DGATE;
     from_f32(out + c, (a.accumulate & flag) ? to_f32(out[c]) + t : t);
   }
@@ -896,8 +897,9 @@ int tl_residual_norm_backward(int dtype, int kind, int64_t rows, int64_t cols, c
                               int accumulate, void* scratch, size_t scratch_bytes, void* stream) {
   tl::NormArgs a{};
   a.rows = rows; a.cols = cols; a.x = x; a.ldx = ldx; a.u = u; a.ldu = ldu;
-  a.w_post = u ? w_post : nullptr;
-  a.gate_mode = u ? gate_mode : TL_GATE_NONE;
+  const bool block = u || rows == 0;  // arrays of no rows are null as well
+  a.w_post = block ? w_post : nullptr;
+  a.gate_mode = block ? gate_mode : TL_GATE_NONE;
   a.gate = a.gate_mode == TL_GATE_NONE ? nullptr : gate;
   a.ldg = ldg; a.alpha = alpha; a.w_pre = w_pre; a.eps = eps;
   a.dy = dy; a.lddy = lddy; a.dn = dn; a.lddn = lddn;
@@ -909,11 +911,12 @@ int tl_residual_norm_backward(int dtype, int kind, int64_t rows, int64_t cols, c
   if ((dy && lddy < cols) || (dn && lddn < cols) || (dx && lddx < cols) || (du && lddu < cols))
     return TL_ERR_INVALID_ARG;
   // gradients of what the call does not have
-  if (!u && (du || dw_post || dgate)) return TL_ERR_INVALID_ARG;
+  if (!block && (du || dw_post || dgate)) return TL_ERR_INVALID_ARG;
   if (dgate && (gate_mode == TL_GATE_NONE || dgate == gate)) return TL_ERR_INVALID_ARG;
   if (dgate && gate_mode == TL_GATE_FULL && lddg < cols) return TL_ERR_INVALID_ARG;
   if (accumulate < 0 || accumulate > 31) return TL_ERR_INVALID_ARG;
-  if (!dx && !du && !dgate && !dw_post && !dw_pre) return TL_ERR_INVALID_ARG;
+  if ((dx && dx == du) || (dw_post && dw_post == dw_pre)) return TL_ERR_INVALID_ARG;
+  if (rows > 0 && !dx && !du && !dgate && !dw_post && !dw_pre) return TL_ERR_INVALID_ARG;
   if (!scratch || !tl::aligned_to(scratch, 16) ||
       scratch_bytes < tl_residual_norm_scratch_bytes(rows, cols))
     return TL_ERR_INVALID_ARG;

@@ -197,6 +197,24 @@ def test_no_rows():
         np.testing.assert_array_equal(D.get(dw, (40,)), 0.0)
 
 
+@pytest.mark.parametrize("mode", [rt.GATE_CHANNEL, rt.GATE_TOKEN, rt.GATE_FULL])
+def test_no_rows_and_no_arrays_of_rows(mode):
+    """Arrays without rows are null; the weights' gradients are zero, whatever the
+    weights hold."""
+    with Dev() as D:
+        L = rt.lib()
+        nb = L.tl_residual_norm_scratch_bytes(0, 40)
+        o = [D.new(40) for _ in range(3)]
+        w = D.put(np.full(40, np.inf), "f32")
+        dgate = o[2] if mode == rt.GATE_CHANNEL else None
+        args = (0, 1, 0, 40, None, 40, None, 40, w, None, mode, 40, 1.0, w, 1e-5)
+        rt.check(L.tl_residual_norm(*args, None, 40, None, 40, D.stream))
+        rt.check(L.tl_residual_norm_backward(*args, None, 40, None, 40, None, 40, None, 40, dgate, 40,
+                                             o[0], o[1], 0, D.zeros(nb), nb, D.stream))
+        for p in o[:2] + ([dgate] if dgate else []):
+            np.testing.assert_array_equal(D.get(p, (40,)), 0.0)
+
+
 def test_many_rows_two_runs_agree():
     """More rows than blocks hold at once; the same call twice gives the same bits."""
     d = inputs(5000, 136, "channel", "bf16", seed=6)

@@ -53,6 +53,15 @@ def test_residual_norm_backward_refuses():
         ({"dx": None, "du": None, "dgate": None, "dw_post": None, "dw_pre": None}, BAD)])
 
 
+def test_residual_norm_backward_refuses_one_tensor_for_two_gradients():
+    nb = rt.load_library().tl_residual_norm_scratch_bytes(4, 8)
+    good = dict(NORM_GOOD, dy=P, lddy=8, dn=P, lddn=8, dx=2 * P, lddx=8, du=3 * P, lddu=8, dgate=4 * P,
+                lddg=8, dw_post=5 * P, dw_pre=6 * P, acc=0, scratch=7 * P, nb=nb)
+    order = NORM + ["dy", "lddy", "dn", "lddn", "dx", "lddx", "du", "lddu", "dgate", "lddg", "dw_post",
+                    "dw_pre", "acc", "scratch", "nb", "stream"]
+    refused("tl_residual_norm_backward", good, order, [({"du": 2 * P}, BAD), ({"dw_pre": 5 * P}, BAD)])
+
+
 def test_distill_refuses():
     nb = rt.load_library().tl_distill_topk_scratch_bytes(4)
     good = {"dtype": 0, "rows": 4, "classes": 100, "top": 8, "z": P, "ldz": 100, "teacher": 2 * P, "ldt": 8,
