@@ -465,7 +465,8 @@ int  tl_residual_norm_backward(int dtype, int kind, int64_t rows, int64_t cols, 
  * [rows, top] the index type; loss [1], row_loss and lse [rows] are float and
  * may be null.  dz may be z (not with accumulate, which adds to dz).  With dz
  * null this is the loss alone, with only dz the gradient alone; one read of z
- * gives both.  top <= 1024; classes * element size <= 1536 KB. */
+ * gives both.  top <= 1024; classes * element size <= 1536 KB; temperature from
+ * 1e-18 to 1e18. */
 size_t tl_distill_topk_scratch_bytes(int64_t rows);
 int  tl_distill_topk(int dtype, int64_t rows, int64_t classes, int64_t top, const void* z,
                      int64_t ldz, const void* teacher, int64_t ldt, const void* index,

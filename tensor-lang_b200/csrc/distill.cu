@@ -544,8 +544,8 @@ int check(int dtype, const DistillArgs& a, int64_t top) {
   if (a.dz && a.lddz < a.classes) return TL_ERR_INVALID_ARG;
   // dz over z: only row on row
   if (a.dz == a.z && a.dz && (a.lddz != a.ldz || a.accumulate)) return TL_ERR_INVALID_ARG;
-  if (!(a.temperature > 0.f) || a.temperature > 3e38f || !(a.divisor >= 0.f))
-    return TL_ERR_INVALID_ARG;
+  // its square is a factor, its inverse another
+  if (!(a.temperature >= 1e-18f && a.temperature <= 1e18f) || !(a.divisor >= 0.f)) return TL_ERR_INVALID_ARG;
   return TL_OK;
 }
 

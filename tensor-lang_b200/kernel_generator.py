@@ -297,7 +297,7 @@ class KernelGenerator:
                 tuple(teacher_shape) != tuple(index_shape) or teacher_shape[0] != logits_shape[0]:
             raise NotImplementedError(f"distill_topk of {tuple(logits_shape)} vs "
                                       f"{tuple(teacher_shape)}, {tuple(index_shape)}")
-        if not 0 < float(temperature) < float("inf"):
+        if not 1e-18 <= float(temperature) <= 1e18:
             raise ValueError(f"distill_topk temperature {temperature}")
         return "", (op_type, name, logits_name, teacher_name, index_name, int(logits_shape[0]),
                     int(logits_shape[1]), int(teacher_shape[1]), float(temperature),

@@ -80,6 +80,19 @@ def test_distill_refuses():
         ({"nb": nb - 1}, BAD), ({"rows": 1 << 30}, UNSUP)])
 
 
+def test_distill_refuses_temperatures_whose_square_or_inverse_overflows():
+    nb = rt.load_library().tl_distill_topk_scratch_bytes(4)
+    good = {"dtype": 0, "rows": 4, "classes": 100, "top": 8, "z": P, "ldz": 100, "teacher": 2 * P, "ldt": 8,
+            "index": 3 * P, "ldi": 8, "it": 2, "tau": 1.0, "div": 0.0, "up": None, "loss": 4 * P,
+            "row_loss": None, "lse": None, "dz": 5 * P, "lddz": 100, "acc": 0, "scratch": 6 * P, "nb": nb,
+            "stream": None}
+    refused("tl_distill_topk", good, list(good), [({"tau": t}, BAD) for t in (1e-40, 1e-19, 1e19, 3e38)])
+    g = tl.KernelGenerator()
+    for t in (1e-40, 1e30):
+        with pytest.raises(ValueError):
+            g.distill_topk("distill_topk", "l", "z", "v", "i", (4, 8), (4, 3), (4, 3), temperature=t)
+
+
 def _difference(f, a, at, h=1e-5):
     up, dn = a.copy(), a.copy()
     up[at] += h
