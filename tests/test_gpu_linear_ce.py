@@ -240,6 +240,23 @@ def test_pieces_of_the_vocabulary():
     compare(run(*a, "f32", 1), *a, "f32")
 
 
+def test_many_rows():
+    """More rows than 2^16, the last tile cut.  dW sums 274 chunks of K (256 rows
+    each) in float32: 274 * 2^-24 = 1.7e-5 of the magnitudes, beside a chunk's own."""
+    x, w, b, t = a = inputs(70001, 130, 24, "f32", seed=10)
+    out = run(*a, "f32")
+    dw = out.pop("dw")
+    compare(out, *a, "f32")
+    ref = lm_ops.linear_ce(x, w, t, b)
+    ez = 4e-6 * (np.abs(x) @ np.abs(w) + np.abs(b)).max() + 4e-6 + 2.0 ** -23 * np.abs(ref["lse"]).max()
+    g = np.abs(ref["g"])
+    r = np.nonzero(t >= 0)[0]
+    p = g.copy()
+    p[r, t[r]] = np.abs(ref["g"][r, t[r]] + 1.0 / len(r))
+    ax = np.abs(x).T
+    within(dw, ref["dw"], ax @ (p * (2 * ez + 4e-6)) + (4e-6 + 1.7e-5) * (ax @ g) + 2e-6 * np.abs(ref["dw"]), "dw")
+
+
 def test_two_runs_agree():
     a = inputs(700, 2500, 520, "bf16", seed=8)
     p, q = run(*a, "bf16", 1), run(*a, "bf16", 1)
