@@ -226,6 +226,13 @@ __device__ __forceinline__ float exp_fast(float x) {  // e^x within 2 ulp of 2^(
   return r;
 }
 
+// (maximum, sum of exponentials) of two sets of logits
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+  const float M = fmaxf(m, m2), base = M == -INFINITY ? 0.f : M;
+  s = s * exp_fast(m - base) + s2 * exp_fast(m2 - base);
+  m = M;
+}
+
 // bits of two bf16, and what their rounding left over
 __device__ __forceinline__ uint32_t take_bf16(float& a, float& b) {
   const uint32_t w = pack2_bf16(a, b);
@@ -397,6 +404,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         }
       }
+      // gave up: nobody leaves while the stages' last copies are on their way (the
+      // leader's barriers count both CTAs'; the wait is bounded)
+      bool landed = !ok && leader;
+      for (int i = 0; i < p.stages && landed; ++i)
+        if (i < s || turn > 0) landed = mbar_wait(smem_u32(&full[i]), (i < s ? turn : turn - 1) & 1);
     }
     if (warp == 1 && leader && lane == 0) {
       // -------------------------------------------------------- MMA (leader)
@@ -461,6 +473,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     float* stage = reinterpret_cast<float*>(staging + e * STG_TILE);
     const uint32_t stg = smem_u32(stage);
     float v[CW];
+    float2 row_stats = make_float2(-INFINITY, 0.f);  // kStats, CG 1: of this CTA's tiles
     bool ok = true;
     uint32_t cg = 0;
     for (int g = first; g < tiles && ok; g += step) {
@@ -529,8 +542,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           float s = 0.f;
 #pragma unroll
           for (int j = 0; j < CW; ++j) s += exp_fast(v[j] - base);
+          if constexpr (CG == 1)
+            join(row_stats.x, row_stats.y, m, s);
           if (live) {
-            p.part[(int64_t)(t.n0 / p.nt * (p.nt > CW ? 2 : 1) + group) * p.part_ld + row] = make_float2(m, s);
+            if constexpr (CG == 2)
+              p.part[(int64_t)(t.n0 / p.nt * (p.nt > CW ? 2 : 1) + group) * p.part_ld + row] = make_float2(m, s);
             if (target >= 0 && target < cols) {
               float z = 0.f;
 #pragma unroll
@@ -647,6 +663,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
     }
+    if constexpr (EPI == kStats && CG == 1) {  // every tile has all rows: one partial per CTA
+      if (group == 0 && quarter * 32 + lane < p.M)
+        p.part[(int64_t)blockIdx.x * p.part_ld + quarter * 32 + lane] = row_stats;
+    }
     if (lane == 0) bulk_wait_all();  // the staging outlives every TMA store's read
     __syncwarp();
   }
@@ -691,43 +711,45 @@ __device__ __forceinline__ int64_t count_targets(const Targets& t, long long* sh
   return n;
 }
 
-__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
-  const float M = fmaxf(m, m2), base = M == -INFINITY ? 0.f : M;
-  s = s * exp_fast(m - base) + s2 * exp_fast(m2 - base);
-  m = M;
-}
-
-// Joins a piece's partials of R rows per block, 256 / R threads a row; the last
-// piece writes lse and the losses, and the last block the mean.
-template <int R>
-__global__ void __launch_bounds__(256) join_kernel(const float2* part, int64_t part_ld, int slots,
+// Joins a piece's partials of R rows per block, NT / R threads a row; the last
+// piece writes lse and the losses, and the last block the mean (the only block:
+// from its own rows' losses, without a ticket).
+template <int R, int NT>
+__global__ void __launch_bounds__(NT) join_kernel(const float2* part, int64_t part_ld, int slots,
                                                    Targets target, const float* zt, float2* run,
                                                    int first, int last, float divisor,
                                                    float* row_loss, float* lse, float* loss,
                                                    Head* head) {
-  constexpr int L = 256 / R;
+  constexpr int L = NT / R, NW = NT / 32;
   __shared__ float2 sh[L][R + 1];
   __shared__ unsigned ticket;
-  __shared__ long long shn[8];
-  __shared__ double shd[8];
+  __shared__ long long shn[NW];
+  __shared__ double shd[NW];
   wait_for_previous_kernel();
   const int r = threadIdx.x % R, l = threadIdx.x / R;
   const int64_t row = (int64_t)blockIdx.x * R + r, rows = target.rows;
+  const bool writes = l == 0 && row < rows;
+  const bool counts = writes && last && target.at(row) >= 0;
+  const float z = counts ? zt[row] : 0.f;
   float m = -INFINITY, s = 0.f;
   if (row < rows) {
     const float2* q = part + row;
     int i = l;
-    for (; i + 3 * L < slots; i += 4 * L) {  // four loads on their way
-      float2 v[4];
+    constexpr int K = NT == 256 ? 4 : 8;  // loads on their way
+    for (; i + (K - 1) * L < slots; i += K * L) {
+      float2 v[K];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = __ldcs(q + (int64_t)(i + k * L) * part_ld);
-      const float M = fmaxf(fmaxf(fmaxf(v[0].x, v[1].x), fmaxf(v[2].x, v[3].x)), m);
+      for (int k = 0; k < K; ++k) v[k] = __ldcs(q + (int64_t)(i + k * L) * part_ld);
+      float M = m;
+#pragma unroll
+      for (int k = 0; k < K; ++k) M = fmaxf(M, v[k].x);
       const float base = M == -INFINITY ? 0.f : M;
       s *= exp_fast(m - base);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s += v[k].y * exp_fast(v[k].x - base);
+      for (int k = 0; k < K; ++k) s += v[k].y * exp_fast(v[k].x - base);
       m = M;
     }
+#pragma unroll 2
     for (; i < slots; i += L) {
       const float2 v = __ldcs(q + (int64_t)i * part_ld);
       join(m, s, v.x, v.y);
@@ -741,20 +763,31 @@ __global__ void __launch_bounds__(256) join_kernel(const float2* part, int64_t p
       sh[l][r] = make_float2(m, s);
     }
   }
-  if (l == 0 && row < rows) {
+  float row_v = 0.f;
+  if (writes) {
     if (!first) join(m, s, run[row].x, run[row].y);
     if (!last) {
       run[row] = make_float2(m, s);
     } else {
       const float log_s = logf(s);  // a row of -inf: -inf
       if (lse) lse[row] = m + log_s;
-      float v = 0.f;
-      // (m - zt) + log s: lse - zt would round lse first
-      if (target.at(row) >= 0) v = zt[row] == -INFINITY ? INFINITY : (m - zt[row]) + log_s;
-      row_loss[row] = v;
+      // (m - z) + log s: lse - z would round lse first
+      if (counts) row_v = z == -INFINITY ? INFINITY : (m - z) + log_s;
+      row_loss[row] = row_v;
     }
   }
   if (!last || !loss) return;
+  if (gridDim.x == 1) {
+    const double own = warp_sum((double)row_v);
+    if ((threadIdx.x & 31) == 0) shd[threadIdx.x >> 5] = own;
+    const int n = __syncthreads_count(counts);
+    if (threadIdx.x == 0) {
+      double t = 0.0;
+      for (int i = 0; i < (R + 31) / 32; ++i) t += shd[i];  // the warps with l == 0
+      *loss = (float)(t / (double)(divisor > 0.f ? divisor : fmaxf(1.f, (float)n)));
+    }
+    return;
+  }
   __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) ticket = atomicAdd(&head->joined, 1u);
@@ -763,14 +796,14 @@ __global__ void __launch_bounds__(256) join_kernel(const float2* part, int64_t p
   __threadfence();
   double t = 0.0;
 #pragma unroll 4
-  for (int64_t i = threadIdx.x; i < rows; i += 256) t += (double)__ldcg(row_loss + i);
+  for (int64_t i = threadIdx.x; i < rows; i += NT) t += (double)__ldcg(row_loss + i);
   t = warp_sum(t);
   if ((threadIdx.x & 31) == 0) shd[threadIdx.x >> 5] = t;
   const int64_t n = divisor > 0.f ? 1 : count_targets(target, shn);
   __syncthreads();
   if (threadIdx.x == 0) {
     t = 0.0;
-    for (int i = 0; i < 8; ++i) t += shd[i];
+    for (int i = 0; i < NW; ++i) t += shd[i];
     const float d = divisor > 0.f ? divisor : fmaxf(1.f, (float)n);
     *loss = (float)(t / (double)d);
     head->joined = 0u;
@@ -947,9 +980,11 @@ bool one_cta(int64_t M) { return M <= 128; }
 //    what the epilogue's slabs and B's boxes allow);
 //  - between one and four waves of a K-major B: fewer where that ends sooner (a
 //    wave costs its tiles' columns and a fixed part worth about 32).
-//    Scoring 1 token x 32768 classes x 4096: 224 columns, 57 us; 256, 71 us.
+//    Scoring 1 token x 32768 classes x 4096 by pairs: 224 columns, 57 us; 256, 71 us.
 //    An MN-major B's boxes are 64 columns of 128 bytes: with 128-column tiles
 //    of CTA pairs 96 tokens x 65536 classes x 2048 took 90 us, with 256 60 us.
+//    Tiles of one CTA gain nothing (1 token: 112 columns 60.9 us, 128 60.2): their
+//    loads share the memory's rate, so a wave with fewer tiles ends sooner anyway.
 template <int EPI>
 int tile_columns(int64_t M, int64_t N, int splits, bool b_mn_major, bool one) {
   const int wide = one ? 128 : 256;
@@ -963,7 +998,7 @@ int tile_columns(int64_t M, int64_t N, int splits, bool b_mn_major, bool one) {
       if (mt * ((N + nt - 1) / nt) <= slots) return nt;
     return wide;
   }
-  if (b_mn_major) return wide;
+  if (b_mn_major || one) return wide;
   int best = wide;
   int64_t cost = INT64_MAX;
   for (int nt = wide; nt >= wide / 4 * 3; nt -= step) {
@@ -1008,9 +1043,10 @@ int launch_tiles(const Planes& A, const Planes& B, const CUtensorMap& c, const T
 }
 
 // The partials a product of kStats leaves per row: one for each epilogue warp's
-// columns, none for columns that do not exist.
+// columns, none for columns that do not exist; tiles of one CTA: one for each CTA.
 int stat_slots(int64_t M, int64_t N, bool b_mn_major) {
   const int nt = tile_columns<kStats>(M, N, 1, b_mn_major, one_cta(M));
+  if (one_cta(M)) return (int)std::min<int64_t>((N + nt - 1) / nt, std::max(1, sm_count()));
   const int64_t before = (N - 1) / nt;
   return (int)(before * (nt > CW ? 2 : 1) + (N - before * nt > CW ? 2 : 1));
 }
@@ -1190,14 +1226,20 @@ int forward(const Call& c, const Plan& q, float* loss, float* row_loss, float* l
     const int64_t n = std::min(piece, c.classes - c0);
     TL_TRY(w_planes(c, q, c0, n, &w));
     TL_TRY(logits<kStats>(c, x, w, none, p, c0, n));
-    // few rows: more threads for each
-    auto join_rows = [&](auto kern, int64_t r) {
-      return launch(kern, dim3((unsigned)((c.rows + r - 1) / r)), 256, 0, c.st, p.part, q.part_ld,
+    auto join_rows = [&](auto kern, int64_t r, int threads) {
+      return launch(kern, dim3((unsigned)((c.rows + r - 1) / r)), threads, 0, c.st, p.part, q.part_ld,
                     stat_slots(c.rows, n, !c.trans_w), c.targets(), p.zt,
                     reinterpret_cast<float2*>(c.scratch + q.run), c0 == 0, c0 + n == c.classes,
                     c.divisor, row_loss, lse, loss, reinterpret_cast<Head*>(c.scratch));
     };
-    TL_TRY(c.rows >= 4096 ? join_rows(join_kernel<32>, 32) : join_rows(join_kernel<4>, 4));
+    // tiles of one CTA leave at most sm_count() partials a row: one block joins them
+    // (scoring 96 tokens x 65536 classes x 2048 69 -> 61 us, 1 token x 32768 x 4096 61 -> 57 us); else few rows:
+    // more threads for each
+    TL_TRY(c.rows <= 4          ? join_rows(join_kernel<4, 1024>, 4, 1024)
+           : c.rows <= 32       ? join_rows(join_kernel<32, 1024>, 32, 1024)
+           : one_cta(c.rows)    ? join_rows(join_kernel<128, 1024>, 128, 1024)
+           : c.rows < 4096      ? join_rows(join_kernel<4, 256>, 4, 256)
+                                : join_rows(join_kernel<32, 256>, 32, 256));
   }
   return TL_OK;
 }
