@@ -45,7 +45,7 @@
 
 #include <algorithm>
 #include <cstring>
-#include <mutex>
+#include <type_traits>
 
 #include "lm_common.cuh"
 #include "tc_ptx.cuh"
@@ -810,6 +810,14 @@ __global__ void __launch_bounds__(NT) join_kernel(const float2* part, int64_t pa
   }
 }
 
+}  // namespace
+}  // namespace tl
+
+#include "linear_ce_few.cuh"
+
+namespace tl {
+namespace {
+
 // Eight elements of a row from any element offset, those past `left` zero.
 __device__ __forceinline__ void load8(const float* p, int64_t left, float (&v)[8]) {
   if (left >= 8 && ((uintptr_t)p & 15) == 0) {
@@ -1071,6 +1079,12 @@ struct Call {
   int kc() const { return f32() ? 4 : 16; }
 };
 
+// Few rows of float32: W as it is (linear_ce_few.cuh, with the figures).
+bool few(int dtype, int64_t rows, int64_t classes, int64_t width) {
+  constexpr int64_t kMost = 1 << 22;  // of the grids' second dimension, and the kept logits
+  return dtype == TL_F32 && rows <= kFewRows && classes <= kMost && width <= kMost;
+}
+
 // How a call is cut: classes per piece, and where its arrays are in scratch.
 struct Plan {
   int64_t fpiece, bpiece;          // classes per piece, forward and backward
@@ -1078,6 +1092,10 @@ struct Plan {
   int64_t part_ld;                 // rows of the forward's partials
   int splits;                      // of K in dx
   int64_t xplanes, wplanes, zt, run, row_loss, part, g, sums, colsum, total;  // offsets
+  // few rows: logits and g [rows][zld], the logits in zsplits sums
+  bool few;
+  int zsplits;
+  int64_t z, zld;
 };
 
 // splits of K that let few tiles of dx fill the GPU: whole waves of clusters
@@ -1118,6 +1136,20 @@ Plan make_plan(int dtype, int trans_w, int64_t rows, int64_t classes, int64_t wi
     at = up_to(at + bytes, 1024);
     return o;
   };
+  q.few = few(dtype, rows, classes, width);
+  if (q.few) {
+    q.zsplits = trans_w ? rowdot_splits(classes, width) : coldot_splits(width, classes);
+    q.splits = trans_w ? coldot_splits(classes, width) : rowdot_splits(width, classes);
+    q.zld = up_to(classes, 32);
+    q.zt = take(rows * 4);
+    q.row_loss = take(rows * 4);
+    q.part = take(kStatBlocks * q.part_ld * 8);
+    q.z = take((int64_t)q.zsplits * rows * q.zld * 4);
+    q.g = take(backward ? rows * q.zld * 4 : 0);
+    q.sums = take(backward ? (int64_t)q.splits * rows * up_to(width, 4) * 4 : 0);
+    q.total = at;
+    return q;
+  }
   q.xplanes = take(P * rows * up_to(width, 64) * 2);
   const int64_t wp = backward ? std::max(q.fpiece, q.bpiece) : q.fpiece;
   q.wplanes = take(P * (trans_w ? wp * up_to(width, 64) : width * up_to(wp, 64)) * 2);
@@ -1211,7 +1243,63 @@ int logits(const Call& c, const Planes& x, const Planes& w, const CUtensorMap& o
                    : launch_tiles<0, 0, EPI>(x, w, out, p, c.st);
 }
 
+// z [split][rows][zld] = x W, without the bias
+int few_logits(const Call& c, const Plan& q) {
+  float* z = reinterpret_cast<float*>(c.scratch + q.z);
+  const float *x = static_cast<const float*>(c.x), *w = static_cast<const float*>(c.w);
+  return c.trans_w ? few_product(true, w, c.ldw, c.classes, c.width, x, c.ldx, c.rows, z, q.zld, c.st)
+                   : few_product(false, w, c.ldw, c.width, c.classes, x, c.ldx, c.rows, z, q.zld, c.st);
+}
+
+int few_forward(const Call& c, const Plan& q, float* loss, float* row_loss, float* lse) {
+  TL_TRY(few_logits(c, q));
+  float2* part = reinterpret_cast<float2*>(c.scratch + q.part);
+  float* zt = reinterpret_cast<float*>(c.scratch + q.zt);
+  if (!row_loss) row_loss = reinterpret_cast<float*>(c.scratch + q.row_loss);
+  const int blocks = (int)std::min<int64_t>(kStatBlocks, (c.classes + 2047) / 2048);
+  TL_TRY(launch(few_stats_kernel, dim3((unsigned)c.rows, (unsigned)blocks), 256, 0, c.st,
+                reinterpret_cast<const float*>(c.scratch + q.z), q.zsplits, q.zld, c.bias, c.targets(), part,
+                q.part_ld, zt));
+  auto join_rows = [&](auto kern) {
+    return launch(kern, dim3(1), 1024, 0, c.st, part, q.part_ld, blocks, c.targets(), zt, nullptr, 1, 1, c.divisor,
+                  row_loss, lse, loss, reinterpret_cast<Head*>(c.scratch));
+  };
+  return c.rows <= 4 ? join_rows(join_kernel<4, 1024>) : join_rows(join_kernel<32, 1024>);
+}
+
+int few_backward(const Call& c, const Plan& q, const float* lse, const float* upstream, void* dx, int64_t lddx,
+                 void* dW, int64_t lddw, float* dbias, int accumulate) {
+  float* scale = &reinterpret_cast<Head*>(c.scratch)->scale;
+  float* g = reinterpret_cast<float*>(c.scratch + q.g);
+  float* sums = reinterpret_cast<float*>(c.scratch + q.sums);
+  const float *x = static_cast<const float*>(c.x), *w = static_cast<const float*>(c.w);
+  TL_TRY(few_logits(c, q));
+  TL_TRY(launch(few_grad_kernel, dim3((unsigned)((c.classes + 255) / 256)), 256, 0, c.st,
+                reinterpret_cast<const float*>(c.scratch + q.z), q.zsplits, q.zld, c.bias, c.targets(), lse,
+                c.divisor, upstream, scale, g, q.zld, dbias, accumulate & TL_ACC_DBIAS));
+  if (dx) {
+    const int64_t ld = up_to(c.width, 4);
+    TL_TRY(c.trans_w ? few_product(false, w, c.ldw, c.classes, c.width, g, q.zld, c.rows, sums, ld, c.st)
+                     : few_product(true, w, c.ldw, c.width, c.classes, g, q.zld, c.rows, sums, ld, c.st));
+    TL_TRY(launch(dx_kernel<float>, dim3((unsigned)c.rows), 256, 0, c.st, sums, q.splits, c.rows, c.width, ld, scale,
+                  static_cast<float*>(dx), lddx, accumulate & TL_ACC_DX));
+  }
+  if (dW) {
+    const int64_t R = c.trans_w ? c.classes : c.width, C = c.trans_w ? c.width : c.classes;
+    const float *p = c.trans_w ? g : x, *r = c.trans_w ? x : g;
+    const int64_t ldp = c.trans_w ? q.zld : c.ldx, ldr = c.trans_w ? c.ldx : q.zld;
+    TL_TRY(few_rows(c.rows, lddw % 4 == 0 && aligned_to(dW, 16), [&](auto tt, auto v) {
+      return launch(few_outer_kernel<decltype(tt)::value, decltype(v)::value>,
+                    dim3((unsigned)((C + 127) / 128), (unsigned)((R + kFewOuterRows - 1) / kFewOuterRows)),
+                    kFewThreads, 0, c.st, p, ldp, r, ldr, (int)c.rows, c.targets(), R, C, scale,
+                    static_cast<float*>(dW), lddw, accumulate & TL_ACC_DW);
+    }));
+  }
+  return TL_OK;
+}
+
 int forward(const Call& c, const Plan& q, float* loss, float* row_loss, float* lse) {
+  if (q.few) return few_forward(c, q, loss, row_loss, lse);
   Planes x, w;
   TL_TRY(x_planes(c, q, false, &x));
   TileParams p{};
@@ -1246,6 +1334,7 @@ int forward(const Call& c, const Plan& q, float* loss, float* row_loss, float* l
 
 int backward(const Call& c, const Plan& q, const float* lse, const float* upstream, void* dx, int64_t lddx,
              void* dW, int64_t lddw, float* dbias, int accumulate) {
+  if (q.few) return few_backward(c, q, lse, upstream, dx, lddx, dW, lddw, dbias, accumulate);
   float* scale = &reinterpret_cast<Head*>(c.scratch)->scale;
   Planes x, w;
   TL_TRY(x_planes(c, q, dW != nullptr, &x));

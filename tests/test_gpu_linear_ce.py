@@ -148,6 +148,30 @@ def test_sizes(dtype, trans, rows, classes, width):
     compare(run(*a, dtype, trans), *a, dtype)
 
 
+@pytest.mark.parametrize("trans", [0, 1])
+@pytest.mark.parametrize("pad", [0, 3])
+@pytest.mark.parametrize("rows", [1, 2, 4, 7, 8, 11, 16, 17])
+def test_few_rows_of_float32(rows, pad, trans):
+    """Up to 16 rows the float32 units read W as it is; odd leading dimensions,
+    sizes that cut every block, gradients that are added to."""
+    x, w, b, t = a = inputs(rows, 2111, 780, "f32", seed=11, ignored=False)
+    if rows > 2:
+        t[1] = -100
+    rng = np.random.default_rng(rows)
+    start = {"dx": rounded(rng.standard_normal(x.shape) * 0.01, "f32"),
+             "dw": rounded(rng.standard_normal(w.shape) * 0.01, "f32"),
+             "dbias": rounded(rng.standard_normal(b.shape) * 0.01, "f32")}
+    compare(run(*a, "f32", trans, pad=pad, calls=1, start=start), *a, "f32", start=start)
+    compare(run(*a, "f32", trans, pad=pad, calls=2, divisor=3.0, up=0.5), *a, "f32", 3.0, 0.5)
+    compare(run(x, w, None, t, "f32", trans), x, w, None, t, "f32")
+    if rows > 2:
+        clean, bad = x.copy(), x.copy()
+        clean[1], bad[1] = 0.0, np.nan
+        out = run(bad, w, b, t, "f32", trans)
+        out.pop("lse")
+        compare(out, clean, w, b, t, "f32")
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("pad,lead", [(8, 0), (3, 0), (0, 1), (5, 3)])
 @pytest.mark.parametrize("trans", [0, 1])
