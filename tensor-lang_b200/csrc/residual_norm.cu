@@ -16,6 +16,11 @@
 //   dw_pre = sum_rows dn hat(y)
 // y is recomputed from x and u in the backward: it costs the same bytes as
 // reading a saved y, and is the unrounded value the forward's n came from.
+//
+// Memory bounds the forward: 65536 x 4096 bf16 356 us, 6.0 TB/s, 0.93 of a
+// copy's rate; 4096 x 8192 55 us.  The backward's 640 us are 5.0 TB/s: its
+// instructions (five sums over the row and the column sums beside the loads)
+// take as long as the bytes.  The column sums' second kernel takes 8 us.
 #include <math.h>
 
 #include <algorithm>
