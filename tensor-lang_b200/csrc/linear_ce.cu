@@ -45,7 +45,7 @@
 // and the float32 plain form's error is below 1e-6.
 //
 // g of bf16 operands is held in bf16, unscaled: each element is off by at most
-// 2^-9 of itself, independently of the others, so the sums dx and dW are off by
+// 2^-8 of itself, independently of the others, so the sums dx and dW are off by
 // less than their own rounding to bf16.  The scale upstream / divisor is applied
 // in float32 afterwards.
 #include <math.h>

@@ -18,9 +18,10 @@
 // reading a saved y, and is the unrounded value the forward's n came from.
 //
 // Memory bounds the forward: 65536 x 4096 bf16 356 us, 6.0 TB/s, 0.93 of a
-// copy's rate; 4096 x 8192 55 us.  The backward's 640 us are 5.0 TB/s: its
-// instructions (five sums over the row and the column sums beside the loads)
-// take as long as the bytes.  The column sums' second kernel takes 8 us.
+// copy's rate; 4096 x 8192 55 us.  The backward's 640 us are 5.0 TB/s:
+// registers (column sums and three values an element) leave two rows of 256
+// threads an SM, whose sums over the row wait for one another; issue slots are
+// 47% used.  The column sums' second kernel takes 8 us.
 #include <math.h>
 
 #include <algorithm>

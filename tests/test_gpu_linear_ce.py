@@ -172,6 +172,35 @@ def test_few_rows_of_float32(rows, pad, trans):
         compare(out, clean, w, b, t, "f32")
 
 
+@pytest.mark.parametrize("trans", [0, 1])
+@pytest.mark.parametrize("rows,classes,width", [(2, 100003, 3), (3, 2, 5003), (16, 40000, 513), (5, 1, 1)])
+def test_few_rows_of_long_and_short_axes(rows, classes, width, trans):
+    a = inputs(rows, classes, width, "f32", seed=12, ignored=False)
+    compare(run(*a, "f32", trans), *a, "f32")
+    p, q = run(*a, "f32", trans), run(*a, "f32", trans)
+    for k in p:
+        np.testing.assert_array_equal(p[k], q[k])
+
+
+def test_few_rows_with_masked_classes():
+    x, w, b, t = inputs(8, 300, 64, "f32", seed=13, ignored=False)
+    b[100:200] = -np.inf
+    b[250:] = np.finfo(np.float32).min
+    t[:] = np.arange(8)
+    t[3] = 150                              # a masked target: loss +inf
+    with np.errstate(invalid="ignore"):
+        out, ref = run(x, w, b, t, "f32"), lm_ops.linear_ce(x, w, t, b)
+    assert np.isposinf(out["row_loss"][3]) and np.isposinf(out["loss"][0])
+    good = np.arange(8) != 3
+    within(out["row_loss"][good], ref["row_loss"][good], 1e-3, "row_loss")
+    compare({k: out[k] for k in ("lse", "dx", "dw", "dbias")}, x, w, b, t, "f32")
+    out = run(x, w, np.full(300, -np.inf), t, "f32")
+    assert np.isneginf(out["lse"]).all() and np.isposinf(out["loss"][0])
+    assert np.isfinite(out["dx"]).all() and np.isfinite(out["dw"]).all()
+    out = run(x, w, None, np.full(8, -100), "f32")
+    assert out["loss"][0] == 0 and not out["row_loss"].any() and not out["dx"].any() and not out["dw"].any()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("pad,lead", [(8, 0), (3, 0), (0, 1), (5, 3)])
 @pytest.mark.parametrize("trans", [0, 1])
