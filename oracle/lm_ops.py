@@ -1,7 +1,7 @@
 """Definitions of the language-model operators in float64.
 
-Plain NumPy restatements of the formulas in ``include/tlb200.h``: the checker
-of the GPU kernels and the forward and VJP rules of ``OracleProgram`` for the
+Plain NumPy restatements of the formulas in ``include/tlb200.h``, which
+the GPU kernels are tested against, and the forward and VJP rules of ``OracleProgram`` for the
 ops of the same names.  Arguments are float64 arrays; class indices are integer
 arrays in which a value outside [0, classes) names no class.
 """

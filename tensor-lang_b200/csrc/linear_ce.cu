@@ -33,6 +33,7 @@
 // eight warps drain finished chunks of K into registers and run the epilogue
 // while the next chunk or tile is multiplied.  Operands are read in the major
 // order they have in memory (K-major or MN-major boxes); nothing is transposed.
+// Up to 16 rows of float32 take other kernels (linear_ce_few.cuh).
 //
 // float32 operands: each is split exactly into three bf16 terms, a = a0 + a1 +
 // a2 (8 bits of the significand each), and six of the nine products are kept
