@@ -13,11 +13,16 @@ Forward: nothing between the two steps writes y, the second weight or anything
 the first step writes or reads, or touches n.  Backward: the second norm's VJP
 is the last to write y's gradient, the first's VJP its only reader after that,
 and no one else keeps it; the weight gradient of the second norm is not
-touched between them.
+touched between them.  The fused call recomputes y from x, u, the weight and
+the gate, where the second norm's own VJP reads the stored y: the forward step
+that stored it runs in the same loop body as both VJPs (or all of them outside
+of loops), and no step between it and them writes y or one of its operands'
+buffers.
 """
 from __future__ import annotations
 
 from .epilogue import _flat
+from .order import ordered, writes_any
 from .steps import LibCall
 
 # argument slots of tl_residual_norm and of tl_residual_norm_backward
@@ -82,8 +87,8 @@ def _forward_once(P, aliased) -> bool:
 
 
 def _backward_once(P, aliased, pinned) -> bool:
-    flat = _flat(P)
-    steps = [s for _, s in flat]
+    flat = ordered(P)
+    steps = [s for _, _, s in flat]
     for i, inner in enumerate(steps):  # the VJP of n = scaled_norm(y)
         if not _is(inner, "tl_residual_norm_backward") or inner.args[_U] != NULL or \
                 inner.args[_DX] == NULL or inner.args[_DY] != NULL:
@@ -93,7 +98,7 @@ def _backward_once(P, aliased, pinned) -> bool:
         if gy in pinned or gy in aliased:
             continue
         j = next((k for k in range(i + 1, len(steps)) if gy in steps[k].reads or gy in steps[k].writes), None)
-        if j is None or flat[j][0] is not flat[i][0]:
+        if j is None or flat[j][1] is not flat[i][1]:
             continue
         outer = steps[j]  # the VJP of y = residual_norm(x, u)
         b = outer.args
@@ -102,16 +107,19 @@ def _backward_once(P, aliased, pinned) -> bool:
                 _touched(steps[j + 1:], gy):
             continue
         y = a[_X][1]
-        # y is what the outer VJP recomputes: the output of the same operands
-        made = next((s for s in steps[:i] if _is(s, "tl_residual_norm") and s.args[_Y] == ("ptr", y)), None)
-        if made is None or made.args[_ROWS:_WPRE] != b[_ROWS:_WPRE]:
+        # y is what the outer VJP recomputes: the last step to write it had the same
+        # operands, in the same body, and they are what they were
+        at = next((k for k in reversed(range(i)) if writes_any(P, [steps[k]], [y])), None)
+        if at is None or flat[at][0] is not flat[i][0]:
+            continue
+        made = steps[at]
+        if not _is(made, "tl_residual_norm") or made.args[_Y] != ("ptr", y) or \
+                made.args[_ROWS:_WPRE] != b[_ROWS:_WPRE] or \
+                writes_any(P, steps[at:j], made.reads):
             continue
         dn, w, dw = a[_DN][1], a[_WPRE], a[_DWPRE]
-        between = steps[i + 1:j]
-        operands = [dn] + ([w[1]] if w != NULL else [])
-        made_at = steps.index(made)
-        if _written(between, operands + list(made.reads)) or \
-                _written(steps[made_at + 1:i], [y] + list(made.reads)):
+        between, operands = steps[i + 1:j], [dn] + ([w[1]] if w != NULL else [])
+        if writes_any(P, between, [y] + operands):
             continue
         if dw != NULL and (_touched(between, dw[1]) or dw[1] in outer.reads or dw[1] in outer.writes):
             continue
@@ -123,7 +131,7 @@ def _backward_once(P, aliased, pinned) -> bool:
                         [r for r in outer.reads if others or r != gy] + operands +
                         ([dw[1]] if dw != NULL and a[_ACC][1] & ACC_DW_PRE else []),
                         list(outer.writes) + ([dw[1]] if dw != NULL else []))
-        lst = flat[j][0]
+        lst = flat[j][1]
         lst[lst.index(outer)] = fused
         lst.remove(inner)
         return True

@@ -1,0 +1,70 @@
+"""What the planner may do with the language-model operators of a program, by
+the steps that it lowers to: where a backward recomputes a value of the forward,
+the two have to be the same value."""
+import pytest
+
+from conftest import load_backend
+
+tl = load_backend()
+L, F, C = tl.programs._let, tl.programs._fill, tl.programs._call
+BW = {"type": "backward", "loss_tensor": "s"}
+Y = L("y", {"type": "residual_norm", "args": ["x", "u", "w"]})
+N = L("n", {"type": "scaled_norm", "args": ["y", "wn"]})
+S = L("s", {"type": "sum", "tensor": "n", "axis": None})
+
+
+def _sgd(*params):
+    out = []
+    for p in params:
+        out += [L(f"{p}_step", C("mult", f"{p}_grad", "lr")), L(f"{p}_new", C("minus", p, f"{p}_step"))]
+    return out + [{"type": "rebind", "name": p, "expr": {"type": "name", "name": f"{p}_new"}} for p in params]
+
+
+def _loop(*body, n=3):
+    return {"type": "for", "loop_var": "i", "iterations": n, "body": list(body)}
+
+
+def norms(*nodes):
+    """A program over x, u [4, 6] and the weights w, wn, whose gradients it takes."""
+    return [L("x", F((4, 6)), (4, 6)), L("u", F((4, 6)), (4, 6)), L("w", F((6,)), (6,), grad=True),
+            L("wn", F((6,)), (6,), grad=True), L("lr", tl.programs._lit([0.1], (1,)), (1,))] + list(nodes)
+
+
+def calls(ast, fetch=("s", "w", "wn")):
+    P = tl.Program(ast, None, fetch=list(fetch))
+    P._fuse_all()
+    return P, [s for s in P._all_steps() if hasattr(s, "fname")]
+
+
+def count(ast, fname, **kw):
+    return sum(s.fname == fname for s in calls(ast, **kw)[1])
+
+
+BWD = "tl_residual_norm_backward"
+
+
+@pytest.mark.parametrize("inside", [(N, S, BW), (S, BW), (BW,)])
+def test_norms_of_a_forward_outside_the_loop_keep_their_own_backward(inside):
+    """y was made before the loop that updates its weight: recomputed in the loop
+    it would follow the weight, which the stored y does not."""
+    outside = [n for n in (Y, N, S) if n not in inside]
+    ast = norms(*outside, _loop(*inside, *_sgd("w", "wn")))
+    P, steps = calls(ast)
+    assert P.alias.get("w_new") == "w"  # the update writes the weight's buffer
+    assert sum(s.fname == BWD for s in steps) == 2
+
+
+def test_norms_apart_where_a_loop_updates_the_weight_before_a_top_level_backward():
+    step = [L("w_step", C("mult", "w", "lr")), L("w_new", C("minus", "w", "w_step")),
+            {"type": "rebind", "name": "w", "expr": {"type": "name", "name": "w_new"}}]
+    P, steps = calls(norms(Y, N, S, _loop(*step), BW), fetch=("s", "w_grad", "wn_grad"))
+    assert P.alias.get("w_new") == "w"
+    assert sum(s.fname == BWD for s in steps) == 2
+
+
+def test_norms_of_one_body_are_one_backward():
+    assert count(norms(_loop(Y, N, S, BW, *_sgd("w", "wn"))), BWD) == 1
+    assert count(norms(Y, N, S, BW), BWD, fetch=("s", "w_grad", "wn_grad")) == 1
+    # a loop between that leaves the operands alone
+    other = _loop(L("q", C("mult", "lr", "lr")))
+    assert count(norms(Y, N, S, other, BW), BWD, fetch=("s", "w_grad", "wn_grad")) == 1
