@@ -351,7 +351,8 @@ def kinfo_to_step(k: tuple, shapes: Dict[str, Shape], divisor_scale: Optional[di
     if kind == "linear_cross_entropy":
         x, w, b, t, rows, width, classes, divisor = k[2:10]
         lse = lse_of(name)
-        shapes[lse] = (rows,)
+        # a program may give two losses of different batches one name
+        shapes[lse] = (max(rows, shapes.get(lse, (0,))[0]),)
         scratch = zeroed_scratch(shapes, "linear_ce", rt.lib().tl_linear_ce_scratch_bytes(
             rt.F32, 0, rows, classes, width, 1))
         return LibCall(f"linear_cross_entropy:{name}", "tl_linear_ce",

@@ -68,3 +68,27 @@ def test_norms_of_one_body_are_one_backward():
     # a loop between that leaves the operands alone
     other = _loop(L("q", C("mult", "lr", "lr")))
     assert count(norms(Y, N, S, other, BW), BWD, fetch=("s", "w_grad", "wn_grad")) == 1
+
+
+def head(*nodes, rows=(4, 4)):
+    """A program over two batches x0, t0 and x1, t1 and the head W, b."""
+    out = []
+    for i, r in enumerate(rows):
+        out += [L(f"x{i}", F((r, 5)), (r, 5)), L(f"t{i}", F((r,)), (r,))]
+    return out + [L("W", F((5, 7)), (5, 7), grad=True), L("b", F((7,)), (7,), grad=True),
+                  L("lr", tl.programs._lit([0.1], (1, 1)), (1, 1))] + list(nodes)
+
+
+def loss(batch=0, name="ce"):
+    return L(name, C("linear_cross_entropy", f"x{batch}", "W", "b", f"t{batch}"))
+
+
+@pytest.mark.parametrize("rows", [(12, 4), (4, 12)])
+@pytest.mark.parametrize("loop", [False, True])
+def test_two_losses_of_one_name_have_room_for_their_rows(rows, loop):
+    """Each call writes the log sums of its own rows into the loss's tensor."""
+    ast = head(loss(0), _loop(loss(1)) if loop else loss(1), rows=rows)
+    P, steps = calls(ast, fetch=("ce",))
+    for s in steps:
+        if s.fname == "tl_linear_ce":
+            assert P.shapes[s.args[15][1]][0] >= s.args[2][1]
