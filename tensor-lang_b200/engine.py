@@ -32,6 +32,7 @@ from .blocknorm import fuse_block_norms
 from .dataio import check_shape, load_data_file
 from .epilogue import fuse_gemm_epilogues
 from .head import fuse_classifier_head
+from .order import refresh_log_sums
 from .pairs import fuse_bias_colsums, plan_gemm_pairs
 from .kernel_generator import KernelGenerator
 from .shapes import Shape, broadcast, complete_env, expr_inputs, numel
@@ -407,6 +408,7 @@ class Program:
                     self.top_grads = sorted(set(self.top_grads) | set(exposed))
                     self.exposed_grads = sorted(set(self.exposed_grads) | set(exposed))
         self.saves = [n for n in ast if n["type"] == "save"]
+        refresh_log_sums(self)
 
     def _build_loop(self, node, body_steps: Dict[int, Step], label: str) -> _Loop:
         body = node["body"]

@@ -92,3 +92,55 @@ def test_two_losses_of_one_name_have_room_for_their_rows(rows, loop):
     for s in steps:
         if s.fname == "tl_linear_ce":
             assert P.shapes[s.args[15][1]][0] >= s.args[2][1]
+
+
+CE_BW = {"type": "backward", "loss_tensor": "ce"}
+
+
+def sums_before_backward(ast, fetch=("ce", "W", "b")):
+    """For each backward of the head: whether the step just before it in its list
+    computes the log sums it subtracts."""
+    P = tl.Program(ast, None, fetch=list(fetch), fuse_ops=False)
+    out = []
+    for lst in [P.phase_bw] + [lp.bw for lp in P.loops]:
+        for s, before in zip(lst, [None] + lst[:-1]):
+            if getattr(s, "fname", "") == "tl_linear_ce_backward":
+                out.append(getattr(before, "fname", "") == "tl_linear_ce" and before.args[13] == ("null",)
+                           and before.args[15] == s.args[13] and before.args[:11] == s.args[:11])
+    return out
+
+
+def _sgd2(*params):
+    """_sgd with a rate that matrices take."""
+    out = []
+    for p in params:
+        out += [L(f"{p}_step", C("mult", "lr", f"{p}_grad")), L(f"{p}_new", C("minus", p, f"{p}_step"))]
+    return out + [{"type": "rebind", "name": p, "expr": {"type": "name", "name": f"{p}_new"}} for p in params]
+
+
+def test_log_sums_follow_the_operands_where_the_forward_is_outside_the_loop():
+    assert sums_before_backward(head(loss(), _loop(CE_BW, *_sgd2("W")))) == [True]
+
+
+def test_log_sums_follow_an_update_before_a_top_level_backward():
+    step = [L("W_new", C("mult", "W", "lr")), {"type": "rebind", "name": "W", "expr": {"type": "name", "name": "W_new"}}]
+    assert sums_before_backward(head(loss(), _loop(*step), CE_BW), fetch=("W_grad",)) == [True]
+
+
+def test_log_sums_of_another_loss_of_the_same_name():
+    """Both losses' backwards run; the second loss's log sums are what is kept."""
+    assert sorted(sums_before_backward(head(loss(0), loss(1), CE_BW), fetch=("W_grad",))) == [False, True]
+
+
+def test_log_sums_are_computed_once_where_nothing_changes():
+    assert sums_before_backward(head(_loop(loss(), CE_BW, *_sgd2("W")))) == [False]
+    assert sums_before_backward(head(loss(), CE_BW), fetch=("W_grad",)) == [False]
+    other = _loop(L("q", C("mult", "lr", "lr")))
+    assert sums_before_backward(head(loss(), other, CE_BW), fetch=("W_grad",)) == [False]
+
+
+def test_log_sums_computed_again_are_not_taken_for_the_forwards():
+    """Two backwards of two losses of one name: the first one's second call leaves
+    the first loss's log sums, which the second backward must not meet."""
+    got = sums_before_backward(head(loss(0), loss(1), CE_BW, CE_BW), fetch=("W_grad",))
+    assert got == [False, True, True, True]
