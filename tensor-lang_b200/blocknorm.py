@@ -50,10 +50,6 @@ def _touched(steps, name) -> bool:
     return any(name in s.reads or name in s.writes for s in steps)
 
 
-def _written(steps, names) -> bool:
-    return any(set(names) & set(s.writes) for s in steps)
-
-
 def _forward_once(P, aliased) -> bool:
     flat = _flat(P)
     steps = [s for _, s in flat]
@@ -73,8 +69,8 @@ def _forward_once(P, aliased) -> bool:
                 continue
             n, between = b[_N][1], steps[i + 1:j]
             weights = [b[_WPRE][1]] if b[_WPRE] != NULL else []
-            if n in aliased or y in aliased or _touched(between, n) or \
-                    _written(between, [y] + weights) or n in first.reads:
+            if n in aliased or y in aliased or n == y or _touched(between, n) or \
+                    writes_any(P, between, [y] + weights) or n in first.reads:
                 continue
             fused = LibCall(f"{first.label}+{second.label}", first.fname,
                             _with(first.args, {_WPRE: b[_WPRE], _N: b[_N], _LDN: b[_LDN]}),

@@ -77,3 +77,7 @@ def test_a_longer_batch_under_the_same_loss_name(rows):
     """A loss of one batch before the loop, of another in it (the gradient is
     taken of both, as the names say)."""
     ce_agree(head(loss(0), _loop(loss(1), CE_BW, *_sgd2("W")), rows=rows), head_feeds(rows), ("ce", "W"))
+
+
+def test_a_norm_under_the_name_of_what_it_norms():
+    agree(norms(Y, L("y", {"type": "scaled_norm", "args": ["y", "wn"]})), norm_feeds(), ("y",))

@@ -144,3 +144,10 @@ def test_log_sums_computed_again_are_not_taken_for_the_forwards():
     the first loss's log sums, which the second backward must not meet."""
     got = sums_before_backward(head(loss(0), loss(1), CE_BW, CE_BW), fetch=("W_grad",))
     assert got == [False, True, True, True]
+
+
+def test_a_norm_under_the_name_of_what_it_norms_stays_a_call_of_its_own():
+    """One call may not write y and n to one tensor (tl_residual_norm refuses it)."""
+    again = L("y", {"type": "scaled_norm", "args": ["y", "wn"]})
+    got = [s for s in calls(norms(Y, again), fetch=("y",))[1] if s.fname == "tl_residual_norm"]
+    assert len(got) == 2 and all(s.args[15] != s.args[17] for s in got)
