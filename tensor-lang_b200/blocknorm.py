@@ -100,8 +100,9 @@ def _backward_once(P, aliased, pinned) -> bool:
         b = outer.args
         if not _is(outer, "tl_residual_norm_backward") or b[_DY] != ("ptr", gy) or b[_DN] != NULL or \
                 any(b[k] != a[k] for k in _SAME) or gy in outer.writes or \
-                _touched(steps[j + 1:], gy):
-            continue
+                _touched(steps[j + 1:], gy) or \
+                any(gy in s.reads for s, f in zip(steps[:i], flat) if f[1] is not flat[i][1]):
+            continue  # (the last: a step before the backward reads the last iteration's)
         y = a[_X][1]
         # y is what the outer VJP recomputes: the last step to write it had the same
         # operands, in the same body, and they are what they were

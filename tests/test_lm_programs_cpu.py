@@ -151,3 +151,13 @@ def test_a_norm_under_the_name_of_what_it_norms_stays_a_call_of_its_own():
     again = L("y", {"type": "scaled_norm", "args": ["y", "wn"]})
     got = [s for s in calls(norms(Y, again), fetch=("y",))[1] if s.fname == "tl_residual_norm"]
     assert len(got) == 2 and all(s.args[15] != s.args[17] for s in got)
+
+
+def test_a_gradient_that_the_next_iteration_reads_is_kept():
+    """q reads the gradient of y that the iteration before left."""
+    q = L("q", {"type": "sum", "tensor": "y_grad", "axis": None})
+    ast = norms(_loop(q, Y, N, S, BW, *_sgd("w", "wn")))
+    P = tl.Program(ast, {"y_grad": {"shape": (4, 6)}}, fetch=["q", "w"])
+    P._fuse_all()
+    assert any("y_grad" in s.writes for s in P._all_steps())
+    assert sum(getattr(s, "fname", "") == BWD for s in P._all_steps()) == 2
