@@ -435,7 +435,8 @@ int  tl_residual_norm(int dtype, int kind, int64_t rows, int64_t cols, const voi
  * (either may be null: zero): dx, du, dgate (gate's shape), dw_post, dw_pre
  * [cols]; each may be null (not wanted).  accumulate: a sum of TL_ACC_*, for
  * outputs to be added to instead of overwritten.  dx may be dy and du may be
- * dn, with the same leading dimension. */
+ * dn, with the same leading dimension; no other output may be an operand or
+ * another output. */
 #define TL_ACC_DX 1
 #define TL_ACC_DU 2
 #define TL_ACC_DGATE 4

@@ -883,6 +883,13 @@ int tl_residual_norm(int dtype, int kind, int64_t rows, int64_t cols, const void
   TL_TRY(tl::check(dtype, kind, a));
   if ((rows > 0 && !y && !n) || (y && ldy < cols) || (n && ldn < cols)) return TL_ERR_INVALID_ARG;
   if (y && y == n) return TL_ERR_INVALID_ARG;
+  // an output over an operand: row on row
+  auto other_rows = [&](const void* p, int64_t ldp, const void* q, int64_t ldq) {
+    return p && p == q && ldp != ldq && rows > 1;
+  };
+  if (other_rows(y, ldy, x, ldx) || other_rows(y, ldy, u, ldu) || other_rows(n, ldn, x, ldx) ||
+      other_rows(n, ldn, u, ldu))
+    return TL_ERR_INVALID_ARG;
   if (rows == 0) return TL_OK;
   cudaStream_t st = tl::stream_or_default(stream);
   return dtype == TL_BF16 ? tl::run_forward<__nv_bfloat16>(a, kind, st)
@@ -922,6 +929,16 @@ int tl_residual_norm_backward(int dtype, int kind, int64_t rows, int64_t cols, c
   if (dgate && gate_mode == TL_GATE_FULL && lddg < cols) return TL_ERR_INVALID_ARG;
   if (accumulate < 0 || accumulate > 31) return TL_ERR_INVALID_ARG;
   if ((dx && dx == du) || (dw_post && dw_post == dw_pre)) return TL_ERR_INVALID_ARG;
+  // an output over an operand: row on row, and only where it is read first
+  auto other_rows = [&](const void* p, int64_t ldp, const void* q, int64_t ldq) {
+    return p && p == q && ldp != ldq && rows > 1;
+  };
+  if (other_rows(dx, lddx, dy, lddy) || other_rows(du, lddu, dn, lddn)) return TL_ERR_INVALID_ARG;
+  if (dgate && (dgate == dx || dgate == du || dgate == dw_post || dgate == dw_pre)) return TL_ERR_INVALID_ARG;
+  if (gate_mode == TL_GATE_FULL && gate && (dx == gate || du == gate)) return TL_ERR_INVALID_ARG;
+  if (gate_mode == TL_GATE_CHANNEL && ((dw_post && (dw_post == gate || dw_post == w_post)) ||
+                                       (dgate && dgate == w_post)))
+    return TL_ERR_INVALID_ARG;
   if (rows > 0 && !dx && !du && !dgate && !dw_post && !dw_pre) return TL_ERR_INVALID_ARG;
   if (!scratch || !tl::aligned_to(scratch, 16) ||
       scratch_bytes < tl_residual_norm_scratch_bytes(rows, cols))

@@ -245,3 +245,25 @@ def test_sharded_batches_name_their_divisor():
         if node["type"] == "let" and node["expr"]["type"] in ("linear_cross_entropy", "distill_topk"):
             node["expr"]["divisor"] = 64
     dp.check_loss_divisors(ast, derived)
+
+
+def test_residual_norm_refuses_outputs_over_other_rows_of_an_operand():
+    """In place is row on row: another leading dimension would write rows not read yet."""
+    good = dict(NORM_GOOD, x=P, u=5 * P, y=2 * P, ldy=9, n=3 * P, ldn=9)
+    refused("tl_residual_norm", good, NORM + ["y", "ldy", "n", "ldn", "stream"], [
+        ({"y": P}, BAD), ({"y": 5 * P}, BAD), ({"n": P}, BAD), ({"n": 5 * P}, BAD)])
+
+
+def test_residual_norm_backward_refuses_outputs_over_what_it_still_reads():
+    nb = rt.load_library().tl_residual_norm_scratch_bytes(4, 8)
+    good = dict(NORM_GOOD, x=8 * P, u=9 * P, w_post=10 * P, gate=11 * P, w_pre=12 * P, dy=13 * P, lddy=8,
+                dn=14 * P, lddn=8, dx=2 * P, lddx=8, du=3 * P, lddu=8, dgate=4 * P, lddg=8, dw_post=5 * P,
+                dw_pre=6 * P, acc=0, scratch=7 * P, nb=nb)
+    order = NORM + ["dy", "lddy", "dn", "lddn", "dx", "lddx", "du", "lddu", "dgate", "lddg", "dw_post",
+                    "dw_pre", "acc", "scratch", "nb", "stream"]
+    channel = {"gate_mode": 1}
+    refused("tl_residual_norm_backward", good, order, [
+        ({"dx": 13 * P, "lddx": 9}, BAD), ({"du": 14 * P, "lddu": 9}, BAD), ({"dx": 11 * P}, BAD),
+        ({"du": 11 * P}, BAD), ({"dgate": 2 * P}, BAD), ({"dgate": 3 * P}, BAD), ({"dgate": 5 * P}, BAD),
+        ({"dgate": 6 * P}, BAD), (dict(channel, dw_post=11 * P), BAD), (dict(channel, dw_post=10 * P), BAD),
+        (dict(channel, dgate=10 * P), BAD)])
