@@ -330,3 +330,153 @@ def test_no_rows():
         assert D.get(loss, (1,))[0] == 0
         m, rest = D.get_rows(dw, 8, 12, 13, "f32")
         assert not m.any() and np.all(rest == 7.0) and not D.get(db, (12,)).any()
+
+
+# -- more than one piece of the vocabulary ------------------------------------
+# 512 MB of scratch for the terms of W, for g and for the forward's partials cut
+# the vocabulary (make_plan in linear_ce.cu); each test says where its cut is.
+
+@pytest.mark.parametrize("trans", [0, 1])
+@pytest.mark.parametrize("rows", [17, 140])
+def test_pieces_of_float32_weights(rows, trans):
+    """10752 classes of 3 x 8192 terms a piece, both directions: the running
+    join, gradients added to, a last piece shorter than the first, for tiles of
+    one CTA and of two."""
+    x, w, b, t = a = inputs(rows, 11800, 8192, "f32", seed=20)
+    t[:3] = [10751, 10752, 11799]  # the classes around the cut, and the last
+    rng = np.random.default_rng(rows)
+    start = {"dx": rounded(rng.standard_normal(x.shape) * 0.01, "f32"),
+             "dw": rounded(rng.standard_normal(w.shape) * 0.01, "f32"),
+             "dbias": rounded(rng.standard_normal(b.shape) * 0.01, "f32")} if rows == 17 else None
+    compare(run(*a, "f32", trans, start=start), *a, "f32", start=start)
+
+
+@pytest.mark.parametrize("trans", [0, 1])
+def test_pieces_of_copied_bf16_weights(trans):
+    """Rows that TMA cannot address are copied: 32768 classes of 8192 a piece."""
+    rng = np.random.default_rng(21)
+    rows, classes, width = 20, 33000, 8192
+    x = rounded(rng.standard_normal((rows, width)), "bf16")
+    w = np.tile(rounded(rng.standard_normal((width, 997)) * 1.5 / np.sqrt(width), "bf16"), (1, 34))[:, :classes]
+    b = rounded(rng.standard_normal(classes) * 0.5, "f32")  # tells equal columns apart
+    t = rng.integers(0, classes, rows)
+    t[:4] = [32767, 32768, classes - 1, -100]
+    compare(run(x, w, b, t, "bf16", trans, pad=3), x, w, b, t, "bf16")
+
+
+def repeated(rows, classes, width, dtype, seed, distinct=509):
+    """A batch whose rows repeat `distinct` ones (the definition is computed for
+    those): (x, w, b, t of them, which row is which)."""
+    x, w, b, t = inputs(distinct, classes, width, dtype, seed=seed)
+    t[:3] = [0, classes - 1, -100]
+    return x, w, b, t, np.arange(rows) % distinct
+
+
+@pytest.mark.parametrize("trans", [0, 1])
+def test_pieces_of_many_rows(trans):
+    """1024 classes of g for 2^18 rows a piece, and 1024 tiles of rows in 128 bands.
+
+    dW adds 256 chunks of K (1024 rows each) in float32, 256 * 2^-24 = 1.6e-5 of
+    the magnitudes beside a chunk's own; dbias adds 8192 groups of 32 rows in eight
+    chains, 1024 * 2^-24 = 6.2e-5 beside a group's."""
+    rows = 1 << 18
+    x, w, b, t, which = repeated(rows, 1100, 40, "bf16", 22)
+    n = np.bincount(which, minlength=len(t)).astype(np.float64)
+    ok = t >= 0
+    div = float(n[ok].sum())
+    out = run(x[which], w, b, t[which], "bf16", trans)
+    for k in ("lse", "row_loss", "dx"):  # equal rows, equal results
+        np.testing.assert_array_equal(out[k], out[k][which], err_msg=k)
+    compare({k: out[k][:len(t)] for k in ("lse", "row_loss", "dx")}, x, w, b, t, "bf16", divisor=div)
+    ref = lm_ops.linear_ce(x, w, t, b, divisor=div)
+    e = 1.2e-5
+    size = (np.abs(x) @ np.abs(w) + np.abs(b)).max(axis=1)
+    ez = e * size + 4e-6 + 2.0 ** -23 * np.abs(ref["lse"])
+    within(out["loss"], np.array([(ref["row_loss"] * n).sum()]) / div,
+           2 * ez.max() + 1e-6 * np.abs(ref["lse"]).mean() + 1e-6, "loss")
+    g = np.abs(ref["g"]) * n[:, None]
+    p = g.copy()
+    r = np.nonzero(ok)[0]
+    p[r, t[r]] = np.abs(ref["g"][r, t[r]] + 1.0 / div) * n[r]
+    eg = p * (2 * ez + 4e-6)[:, None]
+    ax = np.abs(x).T
+    want = x.T @ (ref["g"] * n[:, None])
+    tol = ax @ (eg + BF16_STEP * g) + (e + 1.6e-5) * (ax @ g) + 2e-6 * np.abs(want)
+    within(out["dw"], want, tol + BF16_STEP * (np.abs(want) + tol), "dw")
+    within(out["dbias"], (ref["g"] * n[:, None]).sum(axis=0), eg.sum(axis=0) + (e + 6.2e-5) * g.sum(axis=0), "dbias")
+
+
+def test_pieces_of_a_forward_of_many_rows():
+    """8192 classes of partials for 2^20 rows a piece; the second has eight classes.
+    The mean of 2^20 losses is taken in float64."""
+    rows = 1 << 20
+    x, w, b, t, which = repeated(rows, 8200, 16, "bf16", 23)
+    t[3:5] = [8191, 8192]
+    n = np.bincount(which, minlength=len(t)).astype(np.float64)
+    out = run(x[which], w, b, t[which], "bf16", 1, want=())
+    for k in ("lse", "row_loss"):
+        np.testing.assert_array_equal(out[k], out[k][which], err_msg=k)
+    loss = out.pop("loss")
+    compare({k: out[k][:len(t)] for k in ("lse", "row_loss")}, x, w, b, t, "bf16")
+    ref = lm_ops.linear_ce(x, w, t, b)
+    tol = 2 * (1.2e-5 * (np.abs(x) @ np.abs(w) + np.abs(b)).max() + 4e-6) + 3e-7 * np.abs(ref["lse"]).max()
+    within(loss, np.array([(ref["row_loss"] * n).sum() / n[t >= 0].sum()]), tol, "loss")
+
+
+# -- masks, for every kind of tile and type ------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("trans", [0, 1])
+@pytest.mark.parametrize("rows", [8, 40, 300])
+def test_masked_classes_in_whole_blocks(rows, trans, dtype):
+    """Whole blocks of 128 classes of bias -inf (their maximum is -inf), others of
+    the type's lowest value; a masked target; every class masked; no targets.  A
+    class of the lowest value is one of -inf beside ordinary ones."""
+    low = float(np.finfo(np.float32).min)
+    x, w, b, t = inputs(rows, 1000, 72, dtype, seed=24, ignored=False)
+    b[100:520], b[900:] = -np.inf, -np.inf
+    t[:] = np.arange(rows) % 100
+    t[1], t[2] = 899, 520
+    masked = b.copy()
+    masked[640:800] = -np.inf
+    b[640:800] = low
+    compare(run(x, w, b, t, dtype, trans), x, w, masked, t, dtype)
+    t[3], t[4] = 300, 700  # masked targets: their losses are +inf and lowest's own
+    with np.errstate(invalid="ignore"):
+        out, ref = run(x, w, b, t, dtype, trans), lm_ops.linear_ce(x, w, t, masked)
+    assert np.isposinf(out["row_loss"][3]) and out["row_loss"][4] > 1e38 and np.isposinf(out["loss"][0])
+    good = (np.arange(rows) != 3) & (np.arange(rows) != 4)
+    ez = (1.2e-5 if dtype == "bf16" else 4e-6) * (np.abs(x) @ np.abs(w) + 3.0).max() + 1e-5
+    within(out["row_loss"][good], ref["row_loss"][good], 2 * ez, "row_loss")
+    compare({k: out[k] for k in ("lse", "dx", "dw", "dbias")}, x, w, masked, t, dtype)
+    out = run(x, w, np.full(1000, -np.inf), t, dtype, trans)
+    assert np.isneginf(out["lse"]).all() and np.isposinf(out["loss"][0])
+    # nothing left: g = -onehot / rows
+    g = np.zeros((rows, 1000))
+    g[np.arange(rows), t] = -1.0 / rows
+    step = 2 * BF16_STEP if dtype == "bf16" else 0.0
+    for k, want, mag in (("dx", g @ w.T, np.abs(g) @ np.abs(w).T), ("dw", x.T @ g, np.abs(x).T @ np.abs(g)),
+                         ("dbias", g.sum(axis=0), np.abs(g).sum(axis=0))):
+        within(out[k], want, (1.3e-5 + step) * mag + step * np.abs(want), k)
+    out = run(x, w, b, np.full(rows, -100), dtype, trans)
+    assert out["loss"][0] == 0 and not out["row_loss"].any()
+    assert not out["dx"].any() and not out["dw"].any() and not out["dbias"].any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_nan_rows_stay_their_own_in_tiles_of_two_ctas(dtype):
+    x, w, b, t = inputs(300, 500, 64, dtype, seed=25, ignored=False)
+    x[7, 3], x[200, 0] = np.nan, np.nan
+    out = run(x, w, b, t, dtype, divisor=300.0)
+    keep = np.ones(300, bool)
+    keep[[7, 200]] = False
+    assert np.isnan(out["row_loss"][~keep]).all() and np.isnan(out["dx"][~keep]).all()
+    compare({k: out[k][keep] for k in ("lse", "row_loss", "dx")}, x[keep], w, b, t[keep], dtype, divisor=300.0)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_more_than_one_band_of_row_tiles(dtype):
+    """Tiles go in bands of 2048 rows: two whole ones and a cut one."""
+    a = inputs(4700, 1300, 200, dtype, seed=26)
+    compare(run(*a, dtype, 1), *a, dtype)
+    compare(run(*a, dtype, 0, pad=8), *a, dtype)
