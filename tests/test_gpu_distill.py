@@ -177,3 +177,80 @@ def test_no_rows():
         rt.check(L.tl_distill_topk(0, 0, 10, 2, None, 10, None, 2, None, 2, 2, 1.0, 0.0, None, loss, None,
                                    None, None, 10, 0, D.zeros(nb), nb, D.stream))
         assert D.get(loss, (1,))[0] == 0
+
+
+# -- every cell to its own size ------------------------------------------------
+# dz = cf (p - q).  p = 2^((z - m) k2) / s: z - m, k2 and the product round (three
+# times 2^-24 of an exponent below 30 here), 2^x and the inverse add 2^-21: below 1e-5
+# of p.  q the same way.  So a class that no list names is held to 1e-5 of its own
+# p, however large the row's listed ones are.
+
+def cells(got, z, t, i, dtype, tau=1.0, divisor=0.0, up=1.0, start=None):
+    ref = lm_ops.distill_topk(z, t, i, tau, divisor, up)
+    ok = (i >= 0) & (i < z.shape[1]) & ~np.isneginf(t)
+    some = ok.any(axis=1)
+    cf = np.where(some, tau * up / (divisor if divisor > 0 else max(1, int(some.sum()))), 0.0)[:, None]
+    size = np.zeros(z.shape)  # cf (p + q)
+    for r in np.nonzero(some)[0]:
+        q = np.exp((t[r, ok[r]] - t[r, ok[r]].max()) / tau)
+        np.add.at(size[r], i[r, ok[r]].astype(int), 2 * np.abs(cf[r]) * q / q.sum())
+    size += np.abs(ref["dz"])  # p - q + 2 q
+    want = ref["dz"] if start is None else ref["dz"] + start
+    tol = 1e-5 * size + (0.0 if start is None else 2.0 ** -23 * (np.abs(start) + np.abs(want)))
+    if dtype == "bf16":
+        tol = tol + 2.0 ** -8 * (np.abs(want) + tol)
+    bad = ~(np.abs(got["dz"].astype(np.float64) - want) <= tol)
+    if bad.any():
+        at = np.unravel_index(np.argmax(np.where(bad, np.abs(got["dz"] - want) / (tol + 1e-300), -1)), want.shape)
+        raise AssertionError(f"dz: {int(bad.sum())} of {want.size} off; worst at {at}: got {got['dz'][at]!r}, "
+                             f"want {want[at]!r}, allowed {tol[at]:.3g}")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,classes,top", [
+    (1, 1, 1), (3, 5, 9), (7, 33, 3), (40, 500, 16), (2, 4097, 8), (3, 8192, 64), (2, 16391, 37), (9, 32000, 16),
+    (3, 50021, 33), (40, 50021, 37), (2, 131072, 64), (300, 16391, 20)])
+def test_every_cell(dtype, rows, classes, top):
+    z, t, i = inputs(rows, classes, top, dtype, seed=20, ragged=rows > 2)
+    cells(run(z, t, i, dtype, want=("dz",)), z, t, i, dtype)
+    cells(run(z, t, i, dtype, tau=2.0, divisor=7.0, up=0.5), z, t, i, dtype, 2.0, 7.0, 0.5)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("pad,lead", [(0, 1), (1, 0), (3, 5)])
+@pytest.mark.parametrize("rows,classes", [(5, 20011), (30, 20011)])
+def test_every_cell_of_odd_rows(dtype, pad, lead, rows, classes):
+    z, t, i = inputs(rows, classes, 7, dtype, seed=21)
+    cells(run(z, t, i, dtype, pad=pad, lead=lead), z, t, i, dtype)
+    start = rounded(np.random.default_rng(2).standard_normal(z.shape) * 1e-5, dtype)
+    cells(run(z, t, i, dtype, pad=pad, lead=lead, start=start), z, t, i, dtype, start=start)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [6, 60])
+def test_every_cell_of_masked_rows(dtype, rows):
+    """-inf in whole segments of a cluster, the type's lowest value beside ordinary
+    logits and alone, listed classes without probability, NaN in another row."""
+    low = float(rounded([-3.3e38], dtype)[0])
+    z, t, i = inputs(rows, 20000, 6, dtype, seed=22)
+    z[0, 3000:] = -np.inf
+    z[1, :17000] = -np.inf
+    z[2, 100:] = low
+    z[3] = low
+    z[4, i[4, 0]] = -np.inf
+    t[0, 2:] = -np.inf
+    z[5, 19999] = np.nan
+    got = run(z, t, i, dtype, divisor=float(rows))
+    keep = np.arange(rows) != 5
+    assert np.isnan(got["dz"][5]).all()
+    cells({"dz": got["dz"][keep]}, z[keep], t[keep], i[keep], dtype, divisor=float(rows))
+
+
+@pytest.mark.parametrize("dtype,classes", [("f32", 393216), ("bf16", 786432), ("f32", 393001), ("bf16", 786001)])
+@pytest.mark.parametrize("rows", [2, 20])
+def test_the_longest_rows_and_lists(dtype, classes, rows):
+    """Rows of 1536 KB (segments of 192 KB) beside lists of 1024."""
+    z, t, i = inputs(rows, classes, 1024, dtype, seed=23)
+    got = run(z, t, i, dtype)
+    cells(got, z, t, i, dtype)
+    compare({k: got[k] for k in ("loss", "row_loss", "lse")}, z, t, i, dtype)
