@@ -106,7 +106,7 @@ def lower_let(name: str, expr: dict, shapes: Dict[str, Shape], gen: KernelGenera
     if t == "linear_cross_entropy":
         x, w, b, q = expr["args"]
         return gen.linear_cross_entropy(t, name, x, w, b, q, shapes[x], shapes[w], shapes[q],
-                                        expr.get("divisor"))[1]
+                                        expr.get("divisor"), shapes[b])[1]
     if t == "distill_topk":
         z, tv, ti = expr["args"]
         return gen.distill_topk(t, name, z, tv, ti, shapes[z], shapes[tv], shapes[ti],

@@ -275,7 +275,7 @@ class KernelGenerator:
 
     # -- language-model head and block boundary --------------------------------
     def linear_cross_entropy(self, op_type, name, input_name, weight_name, bias_name, target_name,
-                             input_shape, weight_shape, target_shape, divisor=None):
+                             input_shape, weight_shape, target_shape, divisor=None, bias_shape=None):
         """Cross entropy of linear(x, W, b) with class-index targets, without
         keeping the logits; the mean over the rows that have a class, or the
         sum over a given divisor."""
@@ -284,6 +284,9 @@ class KernelGenerator:
                 tuple(target_shape) != (input_shape[0],):
             raise NotImplementedError(f"linear_cross_entropy of {tuple(input_shape)} @ "
                                       f"{tuple(weight_shape)} vs {tuple(target_shape)}")
+        if bias_shape is not None and tuple(bias_shape) != (weight_shape[1],):
+            raise NotImplementedError(f"linear_cross_entropy with bias {tuple(bias_shape)} for "
+                                      f"{int(weight_shape[1])} classes")
         return "", (op_type, name, input_name, weight_name, bias_name, target_name,
                     int(input_shape[0]), int(input_shape[1]), int(weight_shape[1]),
                     _divisor(divisor))

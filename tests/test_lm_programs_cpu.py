@@ -161,3 +161,11 @@ def test_a_gradient_that_the_next_iteration_reads_is_kept():
     P._fuse_all()
     assert any("y_grad" in s.writes for s in P._all_steps())
     assert sum(getattr(s, "fname", "") == BWD for s in P._all_steps()) == 2
+
+
+@pytest.mark.parametrize("bias", [(1,), (6,), (8,), (1, 7)])
+def test_a_bias_of_another_length_is_refused(bias):
+    """The kernels read a bias for every class."""
+    ast = [L("b2", F(bias), bias) if n.get("name") == "b" else n for n in head()]
+    with pytest.raises(NotImplementedError):
+        tl.Program(ast + [L("ce", C("linear_cross_entropy", "x0", "W", "b2", "t0"))], None, fetch=["ce"])
