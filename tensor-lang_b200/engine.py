@@ -35,7 +35,7 @@ from .head import fuse_classifier_head
 from .order import refresh_log_sums
 from .pairs import fuse_bias_colsums, plan_gemm_pairs
 from .kernel_generator import KernelGenerator
-from .shapes import Shape, broadcast, complete_env, expr_inputs, numel
+from .shapes import Shape, broadcast, complete_env, expr_inputs, numel, out_shape
 from .steps import (EW, ZEROED, Copy, LibCall, Memset0, RegionStep, Step, fuse,
                     kinfo_to_step)
 
@@ -103,6 +103,13 @@ def lower_let(name: str, expr: dict, shapes: Dict[str, Shape], gen: KernelGenera
     if t == "cross_entropy":
         p, q = expr["args"]
         return gen.cross_entropy("cross_entropy", name, p, shapes[p], shapes[q], q)[1]
+    if t in ("linear_cross_entropy", "distill_topk", "residual_norm", "scaled_norm"):
+        # these come without the frontend's type check: a result declared (or defined
+        # before) in another shape would be written past its end
+        want = out_shape(expr, shapes)
+        if tuple(shapes[name]) != want and (want or numel(shapes[name]) != 1):
+            raise NotImplementedError(f"{t} {name}: a result of shape {want} declared as "
+                                      f"{tuple(shapes[name])}")
     if t == "linear_cross_entropy":
         x, w, b, q = expr["args"]
         return gen.linear_cross_entropy(t, name, x, w, b, q, shapes[x], shapes[w], shapes[q],

@@ -169,3 +169,23 @@ def test_a_bias_of_another_length_is_refused(bias):
     ast = [L("b2", F(bias), bias) if n.get("name") == "b" else n for n in head()]
     with pytest.raises(NotImplementedError):
         tl.Program(ast + [L("ce", C("linear_cross_entropy", "x0", "W", "b2", "t0"))], None, fetch=["ce"])
+
+
+@pytest.mark.parametrize("node", [
+    L("y", {"type": "residual_norm", "args": ["x", "u", "w"]}, (3, 6)),
+    L("n", {"type": "scaled_norm", "args": ["x", "wn"]}, (4, 5)),
+    L("n", {"type": "scaled_norm", "args": ["x", "wn"]}, (24,)),
+    L("l", {"type": "distill_topk", "args": ["x", "u", "u"]}, (4,)),
+    L("l", C("linear_cross_entropy", "x", "W", "b", "t"), (4,))])
+def test_a_result_declared_in_another_shape_is_refused(node):
+    ast = norms(L("W", F((6, 7)), (6, 7)), L("b", F((7,)), (7,)), L("t", F((4,)), (4,)), node)
+    with pytest.raises(NotImplementedError):
+        tl.Program(ast, None, fetch=[node["name"]])
+
+
+def test_one_name_for_results_of_two_shapes_is_refused():
+    """The name's buffer has the first one's size."""
+    ast = norms(Y, L("x2", F((9, 6)), (9, 6)), L("y", {"type": "scaled_norm", "args": ["x2", "wn"]}))
+    with pytest.raises(NotImplementedError):
+        tl.Program(ast, None, fetch=["y"])
+    tl.Program(head(L("l", C("linear_cross_entropy", "x0", "W", "b", "t0"), (1,))), None, fetch=["l"])
