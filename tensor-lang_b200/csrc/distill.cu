@@ -24,8 +24,8 @@
 // pass looks the entry up.  (No atomics on values: sums are in list
 // order.)
 //
-// 8192 x 131072 bf16 with lists of 64: 983 to 993 us, 4.3 TB/s of the 6.5 a copy
-// reaches; 1537 x 50021 float32 142 us, 4.3 TB/s.  What bounds it now is
+// 8192 x 131072 bf16 with lists of 64: 984 us, 4.4 TB/s of the 6.5 a copy
+// reaches; 1537 x 50021 float32 141 us, 4.4 TB/s.  What bounds it now is
 // instruction issue (70% of the slots): 13 instructions an element (two passes
 // over shared memory, the exponential in each) and about 500 a warp for the
 // list, the reductions and the exchange.
@@ -494,8 +494,10 @@ __global__ void __launch_bounds__(1024) distill_mean_kernel(DistillArgs a) {
 
 // ------------------------------------------------------------- host side ---
 // About 16384 classes a CTA: 32 KB of bf16 (six CTAs an SM) or 64 KB of float32.
-// Measured on 8192 x 131072 bf16: 32 KB 1073 us, 64 KB 1161 us; on 1537 x 50021
-// float32: 32 KB 164 us, 64 KB 150 us.
+// With 8192, 16384 and 32768 classes, us (131072 and 100000 have eight segments at
+// most in the first two): 8192 x 131072 bf16 947, 947, 1020; 4096 x 65536 bf16 341,
+// 238, 249; 4096 x 100000 bf16 436, 436, 421; 4096 x 32000 float32 228, 212, 328;
+// 1537 x 50021 float32 142, 146, 164.
 // Few rows are spread wider: 8 x 32000 float32 takes 7.5 us in 4096 classes a
 // CTA, 8.9 us in 16384.
 int cluster_for(int64_t rows, int64_t classes) {

@@ -20,7 +20,7 @@
 //
 // The tensor cores bound it: 2048 x 32768 x 4096 bf16, the product with the
 // gradients' epilogue 371 us = 1.48 PFLOP/s (0.88 of the library's measured rate),
-// tensor pipe active 80%; 8192 x 131072 x 4096 forward and backward 27.8 ms under
+// tensor pipe active 80%; 8192 x 131072 x 4096 forward and backward 28.3 ms under
 // the power cap.  Two CTAs load 64 KB per step of 512 cycles, near what L2 gives;
 // the epilogues are hidden behind the next tile.  Few rows are bound by reading W:
 // 1 row x 32768 x 4096 60 us, 4.5 TB/s with the launches and the joining counted.
@@ -42,13 +42,19 @@
 // of K the small products come first: the tensor core's accumulator rounds
 // toward zero, and only a0 b0's additions meet a sum of full size.  The GEMM's
 // two-term scheme (gemm_tc.cu) has half the products and an error of 4e-6;
-// here that error would sit in gradients whose own size is a difference, p - 1,
-// and the float32 plain form's error is below 1e-6.
+// here that error would sit in gradients whose own size is a difference, p - 1.
+// Against 64 bits the gradients of 2048 x 32000 x 1024 are off by 3.5e-7 (of the
+// norm), those of float32 products and sums by 3.2e-6.
 //
 // g of bf16 operands is held in bf16, unscaled: each element is off by at most
-// 2^-8 of itself, independently of the others, so the sums dx and dW are off by
-// less than their own rounding to bf16.  The scale upstream / divisor is applied
-// in float32 afterwards.
+// 2^-8 of itself, so dx and dW are off by at most 2^-8 of the magnitudes that they
+// sum, beside their own rounding.  Where one term carries a sum that is as much
+// again as the output's rounding; where terms cancel it is that much of the terms.
+// Measured against 64 bits, of the norm: 1.7e-3 with g in bf16 and 1.7e-3 with g in
+// float32 for 1537 rows and for 8192, 2.0e-3 and 1.7e-3 for few rows.  Two terms of
+// g would double the products of dx and dW, half of a training pass.  A caller
+// who needs more gives float32 operands.  The scale upstream / divisor is applied in
+// float32 afterwards.
 #include <math.h>
 
 #include <algorithm>
@@ -72,7 +78,8 @@ constexpr int CW = 128;                  // columns of an epilogue warp
 // Three warpgroups: loads and MMAs (and two idle warps), then the epilogue's two.
 // A launch of 384 threads gives each 168 registers; the first group keeps 72 and
 // the others take 216 (128 * 72 + 256 * 216 = 384 * 168): an epilogue thread holds
-// 128 sums, and with 168 registers it spilled (2 to 4% slower).
+// 128 sums, and with 168 registers it spilled more (2 to 4% slower).  12 to 28 bytes
+// a thread still go to local memory in the kGrad and kSum kernels of a K-major A.
 constexpr int THREADS = 128 + 32 * EPI_WARPS;
 constexpr int kFewRegs = 72, kManyRegs = 216;
 constexpr int STG_TILE = 4096;           // per epilogue warp: 32 rows x 128 bytes
@@ -995,10 +1002,12 @@ bool one_cta(int64_t M) { return M <= 128; }
 //  - where half-size tiles still fit one wave: the narrowest that do (steps are
 //    what the epilogue's slabs and B's boxes allow);
 //  - between one and four waves of a K-major B: fewer where that ends sooner (a
-//    wave costs its tiles' columns and a fixed part worth about 32).
-//    Scoring 1 token x 32768 classes x 4096 by pairs: 224 columns, 57 us; 256, 71 us.
-//    An MN-major B's boxes are 64 columns of 128 bytes: with 128-column tiles
-//    of CTA pairs 96 tokens x 65536 classes x 2048 took 90 us, with 256 60 us.
+//    wave costs its tiles' columns and a fixed part worth about 32).  A training pass,
+//    with this and with 256 columns, us: 256 x 19456 x 4096 235 and 242, 256 x 38000 x
+//    2048 210 and 217, 1537 x 50021 x 1000 690 and 705 (dx); scoring by pairs is
+//    bound by memory and gains nothing (200 x 32768 x 4096 65.2 and 65.0).
+//    An MN-major B's boxes are 64 columns of 128 bytes: scoring 200 x 65536 x 2048
+//    takes 98 us with 128-column tiles of CTA pairs, 71 with 256.
 //    Tiles of one CTA gain nothing (1 token: 112 columns 60.9 us, 128 60.2): their
 //    loads share the memory's rate, so a wave with fewer tiles ends sooner anyway.
 template <int EPI>
@@ -1221,9 +1230,10 @@ int w_planes(const Call& c, const Plan& q, int64_t c0, int64_t n, Planes* out) {
                    : as_planes(c, w, c.ldw, c.width, n, q.wplanes, false, Targets{}, out);
 }
 // x, read by every tile: a copy where its rows straddle cache lines, and rows and
-// classes are many enough for that to pay (1537 x 1000 against 50021 classes:
-// products 142 -> 136 and 170 -> 159 us; 5000 x 2000 against 600 classes 118 -> 136
-// us in all).  For dW a copy always, with zeros in the rows without a target: their
+// classes are many enough for that to pay (as it is and copied, width 1000, us:
+// 4000 rows x 32000 classes 214 and 205; a training pass's products of 1537 x 50021
+// 142 and 136, 170 and 159; 4000 x 6000 66.3 and 67.5, 5000 x 600 118 and 136; near
+// the limits either is within 4%: 2000 x 8200 41.7 and 43.3, 400 x 50021 58.6 and 56.8).  For dW a copy always, with zeros in the rows without a target: their
 // g is 0, but 0 times an infinity or NaN in a padded row is NaN in all of dW.
 int x_planes(const Call& c, const Plan& q, bool for_dw, Planes* out) {
   const bool straddles = c.ldx % 64 || !aligned_to(c.x, 128);
@@ -1329,8 +1339,8 @@ int forward(const Call& c, const Plan& q, float* loss, float* row_loss, float* l
                     c.divisor, row_loss, lse, loss, reinterpret_cast<Head*>(c.scratch));
     };
     // tiles of one CTA leave at most sm_count() partials a row: one block joins them
-    // (scoring 96 tokens x 65536 classes x 2048 69 -> 61 us, 1 token x 32768 x 4096 61 -> 57 us); else few rows:
-    // more threads for each
+    // (a partial per tile and several blocks took 8 us longer for 96 tokens x 65536
+    // classes x 2048, 4 us for 1 x 32768 x 4096); else few rows: more threads for each
     TL_TRY(c.rows <= 4          ? join_rows(join_kernel<4, 1024>, 4, 1024)
            : c.rows <= 32       ? join_rows(join_kernel<32, 1024>, 32, 1024)
            : one_cta(c.rows)    ? join_rows(join_kernel<128, 1024>, 128, 1024)

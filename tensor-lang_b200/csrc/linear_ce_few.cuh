@@ -1,10 +1,14 @@
 // The products of linear_ce.cu for few rows of float32: W is read once for each
 // (4 bytes an element, what bounds them), by the ordinary float32 units.  The
 // tensor cores' way writes W as three bf16 terms first and reads those, 16 bytes
-// an element in all, and multiplies 128 rows however few exist.  20000 classes x
-// 2048, forward / whole training pass, us: 1 row 44 / 171 here, 199 / 534 there;
-// 16 rows 81 / 364, 203 / 532; 24 rows 129 / 739, 204 / 530 (here the
-// multiplications bound it by then, so 16 rows are the most).
+// an element in all, and multiplies 128 rows however few exist.  Forward / whole
+// training pass, us, here and there: 20000 classes x 2048, 1 row 47 / 171 and 198 /
+// 531, 16 rows 81 / 367 and 200 / 525, 24 rows 129 / 739 and 204 / 530 (here the
+// multiplications bound it by then, so 16 rows are the most); 32000 x 4096, 8 rows
+// 179 / 677 and 604 / 1609; 50021 x 1000, 16 rows 117 / 465 and 197 / 597; 131072 x
+// 1024, 16 rows 209 / 905 and 516 / 1438; 2000 x 512, 16 rows, training 82 and 89.
+// A training pass reads W three times (the logits, again in the backward, dx) and
+// writes dW: 101 us of the 171 at one row are those 655 MB.
 //
 //   few_rowdot_kernel   out[t][r] = sum_c a[t][c] W[r][c]
 //   few_coldot_kernel   out[t][c] = sum_r a[t][r] W[r][c]
